@@ -14,7 +14,7 @@ import threading
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsas.so")
 
 SAS_OK, SAS_EINVAL, SAS_ELAUNCH, SAS_ENOWS = 0, 1, 2, 3
-SAS_DT_BF16, SAS_DT_FP16, SAS_DT_FP8_E4M3_ROW656 = 0, 1, 2
+SAS_DT_BF16, SAS_DT_FP16, SAS_DT_FP8_E4M3_ROW656, SAS_DT_FP32 = 0, 1, 2, 3
 SAS_SWA, SAS_CFA, SAS_SCFA = 1, 2, 3
 SAS_META_SIZE = 1024
 SAS_FWD_NO_COMBINE = 1
@@ -22,9 +22,11 @@ SAS_BWD_WINDOW_TOKENS = 2   # backward: per-token adds for window rows
 SAS_BWD_WINDOW_KEYS = 4     # backward: the key-major window pass
 SAS_BWD_WORKSPACE = 8       # backward: fwd.workspace holds sas_bwd_plan's bytes
 SAS_BWD_DQ_DTYPE = 16       # backward: dq in the query dtype, written whole
+SAS_ROPE_HALF = 1           # rotated pairs (i, i + rope_dim / 2)
+SAS_ROPE_INVERSE = 2        # rotation by the negative angle
 
 EXPORTED = ("sas_metadata_v1", "sas_metadata_device_v1", "sas_fwd_plan", "sas_fwd_v1", "sas_fwd_noalloc_v1", "sas_combine_v1",
-            "sas_cache_write_v1", "sas_bwd_v1", "sas_bwd_plan", "sas_last_error", "sas_version",
+            "sas_cache_write_v1", "sas_cache_append_v1", "sas_norm_rope_v1", "sas_norm_rope_bwd_plan", "sas_norm_rope_bwd_v1", "sas_bwd_v1", "sas_bwd_plan", "sas_last_error", "sas_version",
             "sas_bench_atomic_add_v1")
 
 _i32p = C.POINTER(C.c_int32)
@@ -95,6 +97,34 @@ class SasCacheWriteArgs(C.Structure):
     ]
 
 
+class SasNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("kv", C.c_void_p), ("q_weight", C.c_void_p), ("kv_weight", C.c_void_p),
+        ("positions", C.c_void_p), ("table", C.c_void_p), ("q_out", C.c_void_p), ("kv_out", C.c_void_p),
+        ("T", C.c_int64), ("H", C.c_int64), ("D", C.c_int64),
+        ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("kv_stride_t", C.c_int64), ("table_rows", C.c_int64),
+        ("rope_dim", C.c_int32), ("q_norm_dim", C.c_int32), ("kv_norm_dim", C.c_int32), ("dtype", C.c_int32),
+        ("weight_dtype", C.c_int32), ("flags", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class SasNormRopeBwdArgs(C.Structure):
+    _fields_ = [
+        ("fwd", SasNormRopeArgs), ("dq_out", C.c_void_p), ("dkv_out", C.c_void_p), ("dq", C.c_void_p),
+        ("dkv", C.c_void_p), ("dq_weight", C.c_void_p), ("dkv_weight", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("dq_out_stride_t", C.c_int64), ("dq_out_stride_h", C.c_int64),
+        ("dkv_out_stride_t", C.c_int64),
+    ]
+
+
+class SasCacheAppendArgs(C.Structure):
+    _fields_ = [
+        ("rope", SasNormRopeArgs), ("cu_seqlens_q", C.c_void_p), ("act_kv", C.c_void_p),
+        ("block_table", C.c_void_p), ("cache", C.c_void_p), ("B", C.c_int64), ("bt_stride", C.c_int64),
+        ("block_size", C.c_int64), ("num_blocks", C.c_int64), ("cache_dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -128,6 +158,14 @@ def lib() -> C.CDLL:
                 L.sas_bwd_plan.restype = C.c_int
                 L.sas_cache_write_v1.argtypes = [C.POINTER(SasCacheWriteArgs), C.c_void_p]
                 L.sas_cache_write_v1.restype = C.c_int
+                L.sas_cache_append_v1.argtypes = [C.POINTER(SasCacheAppendArgs), C.c_void_p]
+                L.sas_cache_append_v1.restype = C.c_int
+                L.sas_norm_rope_v1.argtypes = [C.POINTER(SasNormRopeArgs), C.c_void_p]
+                L.sas_norm_rope_v1.restype = C.c_int
+                L.sas_norm_rope_bwd_plan.argtypes = [C.POINTER(SasNormRopeBwdArgs), C.POINTER(C.c_size_t)]
+                L.sas_norm_rope_bwd_plan.restype = C.c_int
+                L.sas_norm_rope_bwd_v1.argtypes = [C.POINTER(SasNormRopeBwdArgs), C.c_void_p]
+                L.sas_norm_rope_bwd_v1.restype = C.c_int
                 L.sas_bench_atomic_add_v1.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                                       C.c_void_p]
                 L.sas_bench_atomic_add_v1.restype = C.c_int

@@ -18,7 +18,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, rope
 
 _DT = {torch.bfloat16: _lib.SAS_DT_BF16, torch.float16: _lib.SAS_DT_FP16}
 FP8_ROW_BYTES = 656
@@ -134,3 +134,77 @@ def write_kv_cache(kv: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
     rc = _write_bytes()(_ARGS.pack(*args), torch.cuda.current_stream(dev).cuda_stream if _raw is None else _raw(dev.index))
     if rc:
         _lib.check(rc, "write_kv_cache")
+
+
+# what SasCacheAppendArgs puts behind its rope arguments
+_APPEND = struct.Struct("@8Q7q6ifi4Q4q2i")
+assert _APPEND.size == C.sizeof(_lib.SasCacheAppendArgs)
+
+
+def append_kv_cache(
+    kv: torch.Tensor,
+    cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    seqused_kv: torch.Tensor,
+    *,
+    table: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    norm_dim: Optional[int] = None,
+    weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    interleaved: bool = True,
+    q: Optional[torch.Tensor] = None,
+    q_norm_dim: Optional[int] = None,
+    q_weight: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """Append a step's KV rows ``kv [T, D]`` to the paged ``cache``, normed and
+    rotated on the way as :func:`dsv4_amd.rope.norm_rope` does it, and, where ``q``
+    ``[T, H, D]`` is given, the step's queries in the same launch; returns the queries.
+
+    Rows are packed as the attention's queries are: tokens ``cu_seqlens_q[b] ..
+    cu_seqlens_q[b + 1]`` are the last ones of sequence ``b``, whose ``seqused_kv[b]``
+    counts them already, so token ``i`` of its ``n`` is written at position
+    ``seqused_kv[b] - n + i`` through ``block_table`` and
+    :func:`~dsv4_amd.api.sparse_attn_sharedkv` takes the same two tensors next. The
+    angles are those of that position, or of ``positions [T]`` (the depths of a
+    draft tree's nodes). ``table``, ``norm_dim``, ``weight``, ``eps`` and
+    ``interleaved`` are ``norm_rope``'s; so are ``q_norm_dim`` and ``q_weight``.
+
+    ``cache`` is ``[num_blocks, block_size, 1, D]`` in ``kv``'s dtype, or uint8
+    ``[num_blocks, block_size, 1, 656]`` (bf16 ``kv`` with D = 576), quantised from
+    the fp32 values. Tokens behind the last sequence, at a negative position or at
+    one outside ``table`` are padding: nothing of the cache is written for them and
+    their queries come back as zeros; rows without a block are skipped, as by
+    :func:`write_kv_cache`. The rows of one call must go to distinct cache rows. No
+    host sync.
+    """
+    if kv.dim() != 2 or (q is not None and (q.dim() != 3 or q.shape[0] != kv.shape[0] or q.shape[2] != kv.shape[1])):
+        raise ValueError(f"kv must be [T, D] and q [T, H, D], got {tuple(kv.shape)}"
+                         + ("" if q is None else f" and {tuple(q.shape)}"))
+    b = rope._bind(q, kv, positions, table, q_norm_dim, q_weight, norm_dim, weight, eps, interleaved, False, False)
+    dev, D = b.dev, kv.shape[1]
+    fp8 = cache.dtype == torch.uint8
+    if cache.dim() != 4 or cache.shape[2] != 1:
+        raise ValueError(f"cache must be [num_blocks, block_size, 1, row], got {tuple(cache.shape)}")
+    if fp8:
+        if cache.shape[-1] != FP8_ROW_BYTES or kv.dtype != torch.bfloat16 or D != 576:
+            raise ValueError("fp8 cache rows need uint8 [..., 656] and bf16 kv with D = 576")
+    elif cache.dtype != kv.dtype or cache.shape[-1] != D:
+        raise ValueError("cache must hold rows of kv's dtype and width, or uint8 fp8 rows")
+    if not cache.is_contiguous():
+        raise ValueError("cache must be contiguous")
+    B = seqused_kv.numel()
+    if seqused_kv.dim() != 1 or cu_seqlens_q.shape != (B + 1,) or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"cu_seqlens_q [B + 1], seqused_kv [B] and block_table [B, max_blocks] must agree, got "
+                         f"{tuple(cu_seqlens_q.shape)}, {tuple(seqused_kv.shape)}, {tuple(block_table.shape)}")
+    for t in (cache, block_table, cu_seqlens_q, seqused_kv):
+        if t.device != dev:
+            raise ValueError("all tensors must be on kv's device")
+    bt, cu, used = _i32(block_table), _i32(cu_seqlens_q), _i32(seqused_kv)
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    rope._launch("sas_cache_append_v1", _APPEND.pack(
+        *b.pack(0 if out is None else out.data_ptr(), 0), cu.data_ptr(), used.data_ptr(), bt.data_ptr(), cache.data_ptr(),
+        B, bt.shape[1], cache.shape[1], cache.shape[0],
+        _lib.SAS_DT_FP8_E4M3_ROW656 if fp8 else _DT[kv.dtype], 0), dev, "append_kv_cache")
+    return out

@@ -40,7 +40,8 @@ enum {
   /* 656-byte fp8 cache row: 512 e4m3fn latent | 4 fp32 scales (one per 128
      latent channels) | 64 bf16 rope channels. Dequantised value =
      e4m3(byte) * scale[channel / 128]. */
-  SAS_DT_FP8_E4M3_ROW656 = 2
+  SAS_DT_FP8_E4M3_ROW656 = 2,
+  SAS_DT_FP32 = 3 /* norm weights */
 };
 
 /* Index-source scenario, sparse_attn_sharedkv_tilelang/api.py:196-202. */
@@ -298,6 +299,102 @@ typedef struct SasCacheWriteArgs {
 } SasCacheWriteArgs;
 
 int sas_cache_write_v1(const SasCacheWriteArgs* a, void* stream);
+
+/*
+ * Norms of queries and KV rows for each head, and the rotation by position, in
+ * one pass (no counterpart in the reference, whose operator starts from rotated
+ * rows). A row x is one head of q, or one token's kv row, of D channels; its
+ * first n = q_norm_dim (kv_norm_dim) channels are normed, its last rope_dim
+ * rotated:
+ *   y = x;  y[:n] = x[:n] * w / sqrt(mean(x[:n]^2) + eps)
+ *   (a, b) -> (a cos - b sin, a sin + b cos)
+ * on the pairs (2 i, 2 i + 1) of the rotated channels, or (i, i + rope_dim / 2)
+ * with SAS_ROPE_HALF; by the negative angle with SAS_ROPE_INVERSE. The pair i of
+ * a token at position p takes (cos, sin) = table[p][i]. Sums and products are
+ * fp32, rounded once at the end. A token whose position lies outside
+ * [0, table_rows) is padding: its output rows are zeros.
+ * D a multiple of 8 in [8, 1024], rope_dim a multiple of 8 (SAS_ROPE_HALF: 16)
+ * in [0, D], norm dims multiples of 8 in [0, D] (0: no norm); strides multiples
+ * of 8 elements, every tensor 16-byte aligned. Outputs must not overlap inputs.
+ */
+typedef struct SasNormRopeArgs {
+  const void* q;                 /* [T, H, D], or NULL with H = 0 */
+  const void* kv;                /* [T, D], or NULL */
+  const void* q_weight;          /* [q_norm_dim] weight_dtype, or NULL: ones */
+  const void* kv_weight;         /* [kv_norm_dim] weight_dtype, or NULL: ones */
+  const int32_t* positions;      /* [T]; NULL with rope_dim 0 */
+  const float* table;            /* [table_rows, rope_dim / 2, 2]; NULL with rope_dim 0 */
+  void* q_out;                   /* [T, H, D] contiguous */
+  void* kv_out;                  /* [T, D] contiguous */
+  int64_t T, H, D;
+  int64_t q_stride_t, q_stride_h, kv_stride_t;   /* elements */
+  int64_t table_rows;
+  int32_t rope_dim, q_norm_dim, kv_norm_dim;
+  int32_t dtype;                 /* SAS_DT_BF16 or SAS_DT_FP16: q, kv and outputs */
+  int32_t weight_dtype;          /* SAS_DT_FP32 or dtype */
+  int32_t flags;                 /* SAS_ROPE_* bits */
+  float eps;
+  int32_t reserved;              /* 0 */
+} SasNormRopeArgs;
+
+#define SAS_ROPE_HALF 1
+#define SAS_ROPE_INVERSE 2
+
+int sas_norm_rope_v1(const SasNormRopeArgs* a, void* stream);
+
+/*
+ * Backward of sas_norm_rope_v1: fwd holds its arguments (the outputs are
+ * ignored). With u = dy rotated back, g = u w and r = 1/sqrt(mean(x[:n]^2) + eps):
+ *   dx[:n] = r (g - x r^2 mean(g x)),  dx[n:] = u,  dw = sum over rows of u x r.
+ * All outputs are written whole. Padding tokens give zeros and add nothing to
+ * the weights' gradients, which are summed in fp32 in an order that depends on
+ * the sizes and the device alone. dq_weight / dkv_weight NULL: not computed.
+ */
+typedef struct SasNormRopeBwdArgs {
+  SasNormRopeArgs fwd;
+  const void* dq_out;            /* [T, H, D] strided, 16-byte aligned */
+  const void* dkv_out;           /* [T, D] strided */
+  void* dq;                      /* [T, H, D] contiguous */
+  void* dkv;                     /* [T, D] contiguous */
+  float* dq_weight;              /* [q_norm_dim] or NULL */
+  float* dkv_weight;             /* [kv_norm_dim] or NULL */
+  void* workspace;               /* size from sas_norm_rope_bwd_plan */
+  size_t workspace_bytes;
+  int64_t dq_out_stride_t, dq_out_stride_h, dkv_out_stride_t;
+} SasNormRopeBwdArgs;
+
+/* Workspace bytes of the backward (0 without weight gradients). Reads dims,
+   which of q and kv are given, and which weight gradients are asked for. */
+int sas_norm_rope_bwd_plan(const SasNormRopeBwdArgs* a, size_t* workspace_bytes);
+int sas_norm_rope_bwd_v1(const SasNormRopeBwdArgs* a, void* stream);
+
+/*
+ * The KV rows of a step, normed and rotated as by sas_norm_rope_v1, into the paged
+ * cache that the forward reads, and the step's queries with them in the same
+ * launch. Rows are packed as the forward's queries are: tokens
+ * [cu_seqlens_q[b], cu_seqlens_q[b + 1]) are the last ones of sequence b, whose
+ * act_kv[b] counts them already: token i of its n goes to position
+ * act_kv[b] - n + i (as sas_cache_write_v1 places it), which is its angle's
+ * position too unless rope.positions gives another. cache_dtype == rope.dtype:
+ * the D channels; SAS_DT_FP8_E4M3_ROW656 (bf16 kv, D = 576): the fp8 rows of
+ * sas_cache_write_v1, quantised from the fp32 values, rope channels (the last
+ * 64) as bf16. Tokens past cu_seqlens_q[B], at a negative position or at one
+ * outside the table are padding: no cache row is written, query rows are zeros.
+ * Rows whose block-table entry is missing or out of range are skipped. Rows
+ * written by one call must be distinct. rope.kv_out is ignored.
+ */
+typedef struct SasCacheAppendArgs {
+  SasNormRopeArgs rope;
+  const int32_t* cu_seqlens_q;   /* [B + 1] */
+  const int32_t* act_kv;         /* [B] */
+  const int32_t* block_table;    /* [B, bt_stride] */
+  void* cache;                   /* [num_blocks, block_size, 1, row] */
+  int64_t B, bt_stride, block_size, num_blocks;
+  int32_t cache_dtype;           /* rope.dtype, or SAS_DT_FP8_E4M3_ROW656 */
+  int32_t reserved;              /* 0 */
+} SasCacheAppendArgs;
+
+int sas_cache_append_v1(const SasCacheAppendArgs* a, void* stream);
 
 /* Thread-local message of the last failed call on this thread ("" if none). */
 const char* sas_last_error(void);
