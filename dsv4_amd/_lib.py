@@ -25,7 +25,7 @@ SAS_BWD_DQ_DTYPE = 16       # backward: dq in the query dtype, written whole
 SAS_ROPE_HALF = 1           # rotated pairs (i, i + rope_dim / 2)
 SAS_ROPE_INVERSE = 2        # rotation by the negative angle
 
-EXPORTED = ("sas_metadata_v1", "sas_metadata_device_v1", "sas_fwd_plan", "sas_fwd_v1", "sas_fwd_noalloc_v1", "sas_combine_v1",
+EXPORTED = ("sas_metadata_v1", "sas_metadata_device_v1", "sas_fwd_plan", "sas_fwd_v1", "sas_fwd_tree_v1", "sas_fwd_noalloc_v1", "sas_combine_v1",
             "sas_cache_write_v1", "sas_cache_append_v1", "sas_norm_rope_v1", "sas_norm_rope_bwd_plan", "sas_norm_rope_bwd_v1", "sas_bwd_v1", "sas_bwd_plan", "sas_last_error", "sas_version",
             "sas_bench_atomic_add_v1")
 
@@ -69,6 +69,10 @@ class SasFwdArgs(C.Structure):
         ("flags", C.c_int32),
         ("waves", C.c_int32),
     ]
+
+
+class SasFwdTreeArgs(C.Structure):
+    _fields_ = [("fwd", SasFwdArgs), ("tree_mask", C.c_void_p), ("tree_words", C.c_int64)]
 
 
 class SasCombineArgs(C.Structure):
@@ -148,6 +152,8 @@ def lib() -> C.CDLL:
                 L.sas_fwd_plan.restype = C.c_int
                 L.sas_fwd_v1.argtypes = [C.POINTER(SasFwdArgs), C.c_void_p]
                 L.sas_fwd_v1.restype = C.c_int
+                L.sas_fwd_tree_v1.argtypes = [C.POINTER(SasFwdTreeArgs), C.c_void_p]
+                L.sas_fwd_tree_v1.restype = C.c_int
                 L.sas_fwd_noalloc_v1.argtypes = [C.POINTER(SasFwdArgs), C.c_void_p]
                 L.sas_fwd_noalloc_v1.restype = C.c_int
                 L.sas_combine_v1.argtypes = [C.POINTER(SasCombineArgs), C.c_void_p]

@@ -631,7 +631,11 @@ _cache_lock = threading.Lock()
 # the plan) follows from its signature and is kept as bytes behind them.
 _PTRS = struct.Struct("@14Q")
 assert _lib.SasFwdArgs.T.offset == _PTRS.size
+# what SasFwdTreeArgs puts behind them: the mask and its words a token
+_TREE = struct.Struct("@Qq")
+assert C.sizeof(_lib.SasFwdTreeArgs) == C.sizeof(_lib.SasFwdArgs) + _TREE.size
 _fwd_raw = None
+_tree_raw = None
 
 
 def _fwd_bytes():
@@ -643,6 +647,17 @@ def _fwd_bytes():
         f.restype = C.c_int
         _fwd_raw = f
     return _fwd_raw
+
+
+def _tree_bytes():
+    """sas_fwd_tree_v1 taking its arguments as packed bytes."""
+    global _tree_raw
+    if _tree_raw is None:
+        f = _lib.lib()["sas_fwd_tree_v1"]
+        f.argtypes = [C.c_char_p, C.c_void_p]
+        f.restype = C.c_int
+        _tree_raw = f
+    return _tree_raw
 
 
 def sparse_attn_sharedkv(
@@ -717,6 +732,11 @@ def sparse_attn_sharedkv(
                  ori_mask_mode=ori_mask_mode, cmp_mask_mode=cmp_mask_mode, ori_win_left=ori_win_left,
                  ori_win_right=ori_win_right, layout_q=layout_q, layout_kv=layout_kv,
                  core_num=core_num, topk_cmp=topk_cmp, num_splits=0, head_waves=0, waves=0)
+    return _run_first(r, key, stream, dev, return_softmax_lse)
+
+
+def _run_first(r: _Resolved, key, stream, dev, return_softmax_lse, tree_mask=None):
+    """Run a call from its resolution, kept for the signature's later calls where it holds for them."""
     if r.cacheable:
         kept = _Cached(r)
         with _cache_lock:
@@ -741,7 +761,11 @@ def sparse_attn_sharedkv(
         if r.ws_bytes:
             ws = _workspace(dev, stream, r.ws_bytes)
             a.workspace, a.workspace_bytes = ws.data_ptr(), r.ws_bytes
-        _lib.check(_lib.lib().sas_fwd_v1(C.byref(a), C.c_void_p(stream)), "sparse_attn_sharedkv")
+        if tree_mask is None:
+            _lib.check(_lib.lib().sas_fwd_v1(C.byref(a), C.c_void_p(stream)), "sparse_attn_sharedkv")
+        else:
+            ta = _lib.SasFwdTreeArgs(fwd=a, tree_mask=tree_mask.data_ptr(), tree_words=tree_mask.shape[-1])
+            _lib.check(_lib.lib().sas_fwd_tree_v1(C.byref(ta), C.c_void_p(stream)), "sparse_attn_sharedkv_tree")
     finally:
         if staged is not None:
             ring.release(staged[1], stream)
@@ -764,7 +788,7 @@ class _Cached:
 
 
 def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table,
-                cu_seqlens_q, seqused_kv, sinks, return_softmax_lse):
+                cu_seqlens_q, seqused_kv, sinks, return_softmax_lse, tree_mask=None):
     out = q.new_empty(r.out_shape)
     lse = sinks.new_empty(r.lse_shape)   # fp32 on the device, or the call would not be cached
     cu, kv = cu_seqlens_q.data_ptr(), seqused_kv.data_ptr()
@@ -791,18 +815,105 @@ def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, 
         # capture), or another thread may outgrow and replace the shared one
         ws = _workspace(dev, stream, r.ws_bytes) if r.ws_bytes else None
         cmp_ = cmp_kv is not None
-        rc = _fwd_bytes()(
-            _PTRS.pack(q.data_ptr(), ori_kv.data_ptr(), ori_block_table.data_ptr(), cmp_kv.data_ptr() if cmp_ else 0,
-                       cmp_block_table.data_ptr() if cmp_ else 0,
-                       cmp_sparse_indices.data_ptr() if cmp_ and cmp_sparse_indices is not None else 0,
-                       cu, 0, kv, sinks.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                       0 if ws is None else ws.data_ptr(), r.ws_bytes) + r.tail, stream)
+        packed = _PTRS.pack(q.data_ptr(), ori_kv.data_ptr(), ori_block_table.data_ptr(), cmp_kv.data_ptr() if cmp_ else 0,
+                            cmp_block_table.data_ptr() if cmp_ else 0,
+                            cmp_sparse_indices.data_ptr() if cmp_ and cmp_sparse_indices is not None else 0,
+                            cu, 0, kv, sinks.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                            0 if ws is None else ws.data_ptr(), r.ws_bytes) + r.tail
+        if tree_mask is None:
+            rc = _fwd_bytes()(packed, stream)
+        else:
+            rc = _tree_bytes()(packed + _TREE.pack(tree_mask.data_ptr(), tree_mask.shape[-1]), stream)
         if rc:
             _lib.check(rc, "sparse_attn_sharedkv")
     finally:
         if staged is not None:
             ring.release(staged[1], stream)
     return (out, lse) if return_softmax_lse else out
+
+
+def _geometry(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.dtype, t.get_device(), t.is_contiguous())
+
+
+TREE_WORDS_MAX = 64
+
+
+def sparse_attn_sharedkv_tree(
+    q: torch.Tensor,
+    *,
+    tree_mask: torch.Tensor,
+    ori_kv: torch.Tensor,
+    cmp_kv: Optional[torch.Tensor] = None,
+    cmp_sparse_indices: Optional[torch.Tensor] = None,
+    ori_block_table: torch.Tensor,
+    cmp_block_table: Optional[torch.Tensor] = None,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    seqused_kv: torch.Tensor,
+    sinks: torch.Tensor,
+    softmax_scale: float,
+    cmp_ratio: Optional[int] = None,
+    ori_win_left: int = 127,
+    layout_q: str = "TND",
+    return_softmax_lse: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """:func:`sparse_attn_sharedkv` for trees of drafted tokens (the reference
+    takes chains only, api.py:129-397).
+
+    A sequence's query tokens are a tree's nodes, parents before children, each
+    with its row in the cache: behind the ``n = seqused_kv[b] - nodes`` committed rows,
+    node ``i``'s at position ``n + i`` (:func:`dsv4_amd.cache.append_kv_cache` puts them
+    there, rotated by the nodes' depths). ``tree_mask`` int64 ``[T, W]`` (BSND: ``[B, S,
+    W]``), W at most 64: bit ``j % 64`` of word ``j // 64`` says that a token attends
+    node ``j`` of its sequence, one bit for each of its ancestors and one for itself.
+    With ``c`` bits set the token stands at position ``n + c - 1``: its window is the last
+    ``ori_win_left + 1`` of the committed rows and its attended nodes, and compressed
+    rows count from that position as ever (indices below ``(n + c) // cmp_ratio``;
+    pass -1 for rows that hold tokens of another branch). Bits past a sequence's
+    nodes, and of rows before position 0, are ignored; a token without any attends
+    the committed and compressed rows alone.
+
+    The other arguments and the result are :func:`sparse_attn_sharedkv`'s; a chain
+    (bits ``0 .. i`` of node ``i``) gives what that function gives.
+    """
+    lead = tuple(q.shape[:-2])
+    if tree_mask.dtype is not torch.int64 or tree_mask.dim() != len(lead) + 1 or tuple(tree_mask.shape[:-1]) != lead or \
+            not 1 <= tree_mask.shape[-1] <= TREE_WORDS_MAX:
+        raise ValueError(f"tree_mask must be int64 {[*lead, 'W']}, W from 1 to {TREE_WORDS_MAX}, got {tree_mask.dtype} "
+                         f"{tuple(tree_mask.shape)}")
+    if tree_mask.device != q.device:
+        raise ValueError("tree_mask must be on q's device")
+    mask = tree_mask.contiguous()
+    cfa_k = None
+    if cmp_kv is not None and cmp_sparse_indices is None and seqused_kv.numel():
+        cfa_k = int(seqused_kv.max().item())
+    # resolutions are kept as sparse_attn_sharedkv's are; they hold nothing of the mask
+    key = ("tree", _geometry(q), _geometry(ori_kv), _geometry(ori_block_table), _geometry(seqused_kv), _geometry(sinks),
+           _geometry(cu_seqlens_q), _geometry(cmp_kv), _geometry(cmp_block_table), _geometry(cmp_sparse_indices),
+           float(softmax_scale), cmp_ratio, ori_win_left, layout_q, cfa_k)
+    dev = q.device
+    if q.is_cuda and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return sparse_attn_sharedkv_tree(
+                q, tree_mask=mask, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices,
+                ori_block_table=ori_block_table, cmp_block_table=cmp_block_table, cu_seqlens_q=cu_seqlens_q,
+                seqused_kv=seqused_kv, sinks=sinks, softmax_scale=softmax_scale, cmp_ratio=cmp_ratio,
+                ori_win_left=ori_win_left, layout_q=layout_q, return_softmax_lse=return_softmax_lse)
+    stream = _raw_stream(dev) if q.is_cuda else None
+    r = _cache.get(key)
+    if r is not None:
+        r.used = next(_uses)
+        return _run_cached(r, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table,
+                           cu_seqlens_q, seqused_kv, sinks, return_softmax_lse, mask)
+    r = _resolve(q, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices, ori_block_table=ori_block_table,
+                 cmp_block_table=cmp_block_table, cu_seqlens_q=cu_seqlens_q, seqused_kv=seqused_kv, sinks=sinks,
+                 softmax_scale=softmax_scale, **dict(_TREE_DEFAULTS, cmp_ratio=cmp_ratio, ori_win_left=ori_win_left,
+                                                     layout_q=layout_q))
+    return _run_first(r, key, stream, dev, return_softmax_lse, mask)
+
+
+_TREE_DEFAULTS = {k: v for k, v in _FWD_DEFAULTS.items() if k not in (
+    "cmp_kv", "cmp_sparse_indices", "cmp_block_table", "cu_seqlens_q")}
 
 
 class PreparedBackward:

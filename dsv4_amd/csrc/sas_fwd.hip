@@ -2226,8 +2226,10 @@ extern "C" int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* wo
   return SAS_OK;
 }
 
-extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
-  sas::clear_error();
+namespace {
+
+// sas_fwd_v1, or with tree_mask sas_fwd_tree_v1
+int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, void* stream) {
   Plan pl;
   int rc = make_plan(a, &pl);
   if (rc) return rc;
@@ -2295,10 +2297,13 @@ extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
   // An output far beyond the L2s (4K prefill: 268 MB) streams out instead of
   // evicting the cache rows the next tokens gather (C3: 586 -> 571 µs).
   fp.out_nt = pl.nsplit == 1 && (size_t)a->T * a->H * kDV * 2 >= (size_t(16) << 20);
+  fp.tree = tree_mask;
+  fp.tree_words = tree_words;
   hipStream_t st = (hipStream_t)stream;
 
-  if (const int run = win_run(a, pl)) return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
-  if (const int run = dense_run(a, pl)) {
+  // (runs of tokens are chains)
+  if (const int run = tree_mask ? 0 : win_run(a, pl)) return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
+  if (const int run = tree_mask ? 0 : dense_run(a, pl)) {
     fp.nhg = (int)a->H / 64;
     return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
   }
@@ -2311,6 +2316,23 @@ extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
                      : dispatch_hw<512, _Float16, 0>(pl.hw, pl.nw, pl.exact, fp, nblocks, st);
   if (rc || pl.nsplit == 1 || (a->flags & SAS_FWD_NO_COMBINE)) return rc;
   return launch_combine(fp, a->q_dtype, st);
+}
+
+}  // namespace
+
+extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
+  sas::clear_error();
+  return fwd_impl(a, nullptr, 0, stream);
+}
+
+extern "C" int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream) {
+  sas::clear_error();
+  if (!a) return sas::set_error(SAS_EINVAL, "null args");
+  if (a->tree_words < 1 || a->tree_words > 64)
+    return sas::set_error(SAS_EINVAL, "tree_words must be 1 to 64 (got %lld)", (long long)a->tree_words);
+  if (a->fwd.T > 0 && (!a->tree_mask || (uintptr_t)a->tree_mask % 8))
+    return sas::set_error(SAS_EINVAL, "tree_mask must be an 8-byte aligned device pointer");
+  return fwd_impl(&a->fwd, a->tree_mask, (int)a->tree_words, stream);
 }
 
 // ---------------------------------------------------------------------------

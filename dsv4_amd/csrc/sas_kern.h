@@ -130,6 +130,8 @@ struct FwdParams {
   int nxcd;      // XCDs the grid is dealt over (device_xcds())
   int part_nt;   // 1: split partials go out with non-temporal stores
   int out_nt;    // 1: the output (one split) goes out with non-temporal stores
+  const uint64_t* tree;   // draft trees: [T, tree_words] attended slots of the token's sequence, or NULL
+  int tree_words;         // 64-slot words a token, at most 64
 };
 
 // ---------------------------------------------------------------------------
@@ -404,6 +406,53 @@ __device__ __forceinline__ Tok item_of(const FwdParams& p, int item) {
   return k;
 }
 
+// Position of the k-th (from 0) set bit of m, which has more than k: halves by
+// their counts.
+__device__ __forceinline__ int nth_bit(uint64_t m, int k) {
+  uint32_t x = (uint32_t)m;
+  int at = 0, c = __popc(x);
+  if (k >= c) { k -= c; at = 32; x = (uint32_t)(m >> 32); }
+#pragma unroll
+  for (int w = 16; w >= 1; w >>= 1) {
+    c = __popc(x & ((1u << w) - 1u));
+    if (k >= c) { k -= c; at += w; x >>= w; }
+  }
+  return at;
+}
+
+// A token's row of a draft tree's mask. Lane w holds word w (at most 64 words):
+// the draft slots of its sequence that the token attends, its ancestors and
+// itself. Slots past the sequence's drafts, or before position 0, drop out.
+struct Tree {
+  uint64_t word;   // this lane's
+  int count;       // set bits of all words
+  __device__ __forceinline__ Tree(uint64_t w, int lane, int first, int end) : word(w) {
+    const int lo = first - 64 * lane, hi = end - 64 * lane;   // this word's valid bits: [lo, hi)
+    if (lo > 0) word = lo < 64 ? word >> lo << lo : 0;
+    if (hi < 64) word = hi > 0 ? word & ((1ull << hi) - 1ull) : 0;
+    count = 0;
+    const uint64_t any = __ballot(word != 0);
+    for (uint64_t a = any; a; a &= a - 1) count += __popcll(at(__ffsll((unsigned long long)a) - 1));
+  }
+  // word w, in scalar registers
+  __device__ __forceinline__ uint64_t at(int w) const {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(word >> 32), w) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)word, w);
+  }
+  // slot of the set bit of rank k, per lane (k in [0, count), else any slot)
+  __device__ __forceinline__ int slot(int k) const {
+    int s = 0, pre = 0;
+    for (uint64_t a = __ballot(word != 0); a; a &= a - 1) {
+      const int w = __ffsll((unsigned long long)a) - 1;
+      const uint64_t m = at(w);
+      const int n = __popcll(m);
+      if (k >= pre && k < pre + n) s = 64 * w + nth_bit(m, k - pre);
+      pre += n;
+    }
+    return s;
+  }
+};
+
 // Resolve the item's slot range to cache rows and compact the valid ones, in
 // slot order, into lds_rows[0, nvalid) as row byte addresses (ROWB bytes per
 // row), so the streaming loops only add a chunk offset. The first NT threads
@@ -444,6 +493,8 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
     // act_q == NULL: q_prefix is cu_seqlens_q [B + 1] and a query length is
     // the difference of two entries (loaded in the same round trip)
     const bool cu = p.act_q == nullptr;
+    uint64_t tree_word = 0;
+    if (p.tree && lane < p.tree_words) tree_word = p.tree[(size_t)t * p.tree_words + lane];
     int qp0 = INT_MAX, aq0 = 0, akv0 = 0;
     if (lane < p.B) { qp0 = p.q_prefix[lane]; aq0 = cu ? p.q_prefix[lane + 1] : p.act_q[lane]; akv0 = p.act_kv[lane]; }
     // token -> (batch, position): largest b with q_prefix[b] <= t (q_prefix is
@@ -465,10 +516,15 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
     if (cu) aq -= qpb;   // end of the batch's tokens -> its query length
     const int spos = t - qpb;
     const bool padded = spos < 0 || spos >= aq;
-    const int sg = akv - aq + spos;                              // causal position
+    // causal position. Of a draft tree's node: its depth below the rows before
+    // the drafts (its set bits, itself among them, come last), and the window
+    // takes its `path` nearest drafts, then the rows before the drafts.
+    const Tree tree(tree_word, lane, aq - akv, p.tree ? aq : 0);
+    const int sg = p.tree ? max(akv - aq, 0) + tree.count - 1 : akv - aq + spos;
     const int nwin = (padded || sg < 0) ? 0 : min(sg, p.win_left) + 1;
     const int wlo = sg - nwin + 1;                               // = max(sg - win_left, 0)
     const int thr = (padded || sg + 1 <= 0) ? 0 : (sg + 1) / p.cmp_ratio;
+    const int path = min(tree.count, nwin);
     if (tid == 0) { lds_tok[0] = b; lds_tok[1] = padded; lds_tok[2] = thr; }
 
     // ---- round trip 2: block tables -----------------------------------------
@@ -485,9 +541,11 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
       if (r >= nr) continue;   // uniform
       const int j = s0 + r * NT + tid;
       const bool live = j < s1 && !padded;
+      int draft = 0;   // its slot, for window slots from nwin - path on
+      if (p.tree && s0 + r * NT < wincap) draft = tree.slot(tree.count - nwin + j);   // wave-uniform
       int blk;
       if (j < wincap) {
-        const int pos = wlo + j;
+        const int pos = p.tree && j >= nwin - path ? max(akv - aq + draft, 0) : wlo + j;
         blk = pos / p.ori_bs;
         off[r] = pos - blk * p.ori_bs;
         ok[r] = live && j < nwin && blk < p.ori_bt_stride;

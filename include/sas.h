@@ -195,6 +195,29 @@ int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* workspace_byt
 int sas_fwd_v1(const SasFwdArgs* a, void* stream);
 
 /*
+ * The forward for trees of drafted tokens (no counterpart in the reference): the
+ * tokens of sequence b are a tree's nodes, one cache row each in query order
+ * behind its n = act_kv[b] - act_q[b] committed rows, so node i's row lies at
+ * position n + i. Bit j (of word j / 64) of tree_mask[t] says that token t
+ * attends node j of its sequence: its ancestors and itself. With c such nodes,
+ * token t stands at position n + c - 1; its window is the last win_left + 1 of
+ * (committed rows, attended nodes in query order), and compressed rows are
+ * attended as by sas_fwd_v1 from that position (below (n + c) / cmp_ratio). A
+ * chain (bits 0 .. i for node i) is sas_fwd_v1's own mask. Bits past the
+ * sequence's tokens, or of rows before position 0 (act_kv < act_q; n counts as 0
+ * then), are ignored; a row without bits attends committed and compressed rows
+ * alone, and with none of them the sink (out 0, lse the sink). fwd's plan and workspace are
+ * sas_fwd_plan's.
+ */
+typedef struct SasFwdTreeArgs {
+  SasFwdArgs fwd;
+  const uint64_t* tree_mask;     /* [T, tree_words] */
+  int64_t tree_words;            /* 1 .. 64 */
+} SasFwdTreeArgs;
+
+int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream);
+
+/*
  * sas_fwd_v1 without any allocation by caller or library, for callers that
  * cannot allocate device memory (code under HIP graph capture, tight serving
  * loops, harnesses that forbid hipMalloc). No counterpart in the reference.
