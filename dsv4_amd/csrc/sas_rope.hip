@@ -10,21 +10,21 @@
 //   dx[:n] = r (g - x r^2 (sum g x) / n),  dx[n:] = u,  dw = sum_rows u x r.
 //
 // All of it is HBM-bound: a row is read once and written once (backward: two
-// reads), 2 D bytes each way, against some 5 VALU operations a channel. Eight
-// lanes share a row and a wave takes eight rows: channel chunk (8 channels, 16
-// bytes) 8 i + l of its row belongs to lane l of the eight, so a load
-// instruction covers whole 128-byte lines, 512 and 576 channels come out even (8 or
-// 9 loads a lane, all in flight at once; a wave a row leaves 56 of 64 lanes
-// idle in the second load of 576), and a row's sums take three DPP steps. The 64
-// rotated channels are then the last chunk of every lane. Nothing passes
-// through LDS but the backward's weight sums.
+// reads), 2 D bytes each way, against some 5 (15) VALU operations a channel. Sixteen
+// lanes share a row and a wave takes four: channel chunk (8 channels, 16
+// bytes) 16 i + l of its row belongs to lane l of the sixteen, so a load
+// instruction covers whole 256-byte pieces of four rows, all of a lane's loads are
+// in flight at once, and a row's sums are four DPP steps inside the sixteen lanes.
+// Nothing passes through LDS but the weights and the backward's sums of theirs.
 
 #include "sas_kern.h"
 
 namespace sas {
 namespace {
 
-constexpr int kRopeThreads = 256, kRopeRows = kRopeThreads / 8;   // rows a workgroup takes at a time
+constexpr int kLanes = 16;                                            // of a row
+constexpr int kRopeThreads = 256, kRopeRows = kRopeThreads / kLanes;   // rows a workgroup takes at a time
+constexpr int kWaveRows = 64 / kLanes;
 constexpr int kFp8ScaleOff = 512, kFp8RopeOff = 528;
 constexpr float kFp8Max = 448.f;
 
@@ -60,17 +60,25 @@ template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-// over the eight lanes of a row: pairs, quads, then the other quad (half-row mirror)
-__device__ __forceinline__ float sum8(float x) {
+// over a row's sixteen lanes: pairs, quads, eights (mirrored halves), all (mirrored)
+__device__ __forceinline__ float sum16(float x) {
   x += dpp<0xB1>(x);
   x += dpp<0x4E>(x);
-  return x + dpp<0x141>(x);
+  x += dpp<0x141>(x);
+  return x + dpp<0x140>(x);
 }
-__device__ __forceinline__ float max8(float x) {
+__device__ __forceinline__ float max16(float x) {
   x = fmaxf(x, dpp<0xB1>(x));
   x = fmaxf(x, dpp<0x4E>(x));
-  return fmaxf(x, dpp<0x141>(x));
+  x = fmaxf(x, dpp<0x141>(x));
+  return fmaxf(x, dpp<0x140>(x));
 }
+
+// v as a value of its own: what was computed from it before is not kept for later
+// (and what it is computed from is not sunk into a branch that alone reads it)
+__device__ __forceinline__ void opaque(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+__device__ __forceinline__ void opaque(float4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+__device__ __forceinline__ void opaque(float& v) { asm volatile("" : "+v"(v)); }
 
 template <typename QT>
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -83,15 +91,39 @@ template <typename QT>
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack2<QT>(f[0], f[1]), pack2<QT>(f[2], f[3]), pack2<QT>(f[4], f[5]), pack2<QT>(f[6], f[7]));
 }
-// weights of channels 8 c .. 8 c + 7
-template <typename QT>
-__device__ __forceinline__ void weights8(const RopeParams& p, const uint8_t* w, int c, float (&f)[8]) {
-  if (p.wf32) {
-    const float4 a = reinterpret_cast<const float4*>(w)[2 * c], b = reinterpret_cast<const float4*>(w)[2 * c + 1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    unpack8<QT>(reinterpret_cast<const uint4*>(w)[c], f);
+// The part's weights as fp32 in LDS, ones past them (and where there are none, if
+// the caller asks for a part without): a workgroup's rows share them, in global
+// memory each wave would fetch its chunks' anew, in two types. `get` issues the
+// loads, `put` writes them behind the caller's own loads.
+template <typename QT, int NI>
+struct Weights {
+  static constexpr int kAll = NI * kLanes * 8, N = (kAll + kRopeThreads - 1) / kRopeThreads;
+  float w[N];
+  __device__ __forceinline__ void get(const RopeParams& p, const RopePart& a, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = tid + k * kRopeThreads;
+      w[k] = 1.f;
+      if (a.w && j < a.n) w[k] = p.wf32 ? reinterpret_cast<const float*>(a.w)[j] : (float)reinterpret_cast<const QT*>(a.w)[j];
+    }
   }
+  __device__ __forceinline__ void put(float* lds, int tid) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int j = tid + k * kRopeThreads;
+      if (kAll % kRopeThreads == 0 || j < kAll) lds[j] = w[k];
+    }
+    asm volatile("" ::: "memory");
+    lds_barrier();
+    asm volatile("" ::: "memory");
+  }
+};
+// weights of channels 8 c .. 8 c + 7
+__device__ __forceinline__ void weights8(uint32_t lds, int c, float (&f)[8]) {
+  const LDS_AS f32x4* w = reinterpret_cast<const LDS_AS f32x4*>((size_t)(lds + 32 * c));
+  const f32x4 a = w[0], b = w[1];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) { f[k] = a[k]; f[4 + k] = b[k]; }
 }
 
 // Token -> (sequence, place): the largest b with cu[b] <= t, one ballot per row and 64
@@ -106,9 +138,9 @@ __device__ __forceinline__ Place place_of(const RopeParams& p, int t, int lane) 
     if (i < p.B) { q0 = p.cu[i]; q1 = p.cu[i + 1]; kv = p.used[i]; }
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int m = __popcll(__ballot(q0 <= __builtin_amdgcn_readlane(t, 8 * j)));
-      n = (lane >> 3) == j ? m : n;
+    for (int j = 0; j < kWaveRows; ++j) {
+      const int m = __popcll(__ballot(q0 <= __builtin_amdgcn_readlane(t, kLanes * j)));
+      n = lane / kLanes == j ? m : n;
     }
     const int at = max(n - 1, 0);
     const int s = __shfl(q0, at), e = __shfl(q1, at), u = __shfl(kv, at);
@@ -119,55 +151,82 @@ __device__ __forceinline__ Place place_of(const RopeParams& p, int t, int lane) 
   return o;
 }
 
-// A lane's share of one row. LAST: D = 64 NI and R = 64, so the rotated
-// channels are exactly the lanes' last chunks (the branch and its late loads go).
+// Token and head of the lane's row, the wave's first row being r0: one division for
+// the wave, the rows after it step on. A lane without a row takes r0's.
+struct Head { uint32_t t, h; };
+__device__ __forceinline__ Head head_of(uint32_t r0, uint32_t H, int lane, bool live) {
+  const uint32_t t0 = r0 / H, h0 = r0 - t0 * H;
+  uint32_t t = t0, h = h0 + lane / kLanes;
+  if (H >= (uint32_t)kWaveRows) {
+    if (h >= H) { h -= H; ++t; }
+  } else {
+    const uint32_t k = h / H;
+    t += k;
+    h -= k * H;
+  }
+  return live ? Head{t, h} : Head{t0, h0};
+}
+
+// A lane's share of one row of up to 128 NI channels. LAST: more than 128 (NI - 1), and the
+// rotated channels are the row's last 64 (or none), which lie in iteration NI - 1.
 template <typename QT, int NI, bool LAST, bool HALF>
 struct Row {
-  int sub, nch, nn, rc0, hc;   // lane of eight; chunks: row's, normed, first rotated, half the rotated ones
+  int sub, nch, nn, rc0, hc;   // lane of sixteen; chunks: row's, normed, first rotated, half the rotated ones
   uint4 v[NI];
 
   __device__ Row(const RopeParams& p, int n, int lane)
-      : sub(lane & 7), nch(LAST ? 8 * NI : p.D / 8), nn(n / 8), rc0(LAST ? 8 * (NI - 1) : (p.D - p.R) / 8),
-        hc(LAST ? 4 : p.R / 16) {}
-  __device__ __forceinline__ int chunk(int i) const { return 8 * i + sub; }
-  __device__ __forceinline__ bool has(int i) const { return LAST || chunk(i) < nch; }
-  // wave-uniform: chunks of iteration i are rotated
-  __device__ __forceinline__ bool turns(int i) const { return LAST ? i == NI - 1 : 8 * i + 7 >= rc0 && 8 * i < nch; }
+      : sub(lane & (kLanes - 1)), nch(p.D / 8), nn(n / 8), rc0((p.D - p.R) / 8), hc(p.R / 16) {}
+  __device__ __forceinline__ int chunk(int i) const { return kLanes * i + sub; }
+  __device__ __forceinline__ bool has(int i) const { return (LAST && i < NI - 1) || chunk(i) < nch; }
+  // wave-uniform: iteration i has rotated chunks
+  __device__ __forceinline__ bool turns(int i) const {
+    return LAST ? i == NI - 1 : kLanes * (i + 1) > rc0 && kLanes * i < nch;
+  }
   __device__ __forceinline__ int partner(int c) const { return c - rc0 < hc ? c + hc : c - hc; }
 
   __device__ __forceinline__ static uint4 ld(const uint8_t* x, int c) {
-    return gld16(reinterpret_cast<uint64_t>(x) + 16 * c);
+    return gld16(reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)c);
   }
-  // every lane loads (a clamped chunk)
+  // every lane loads; chunks past the first `most` are clamped to the last of them
+  // (a line that is fetched anyway)
   __device__ __forceinline__ void load(const uint8_t* x) {
+    const uint64_t b = reinterpret_cast<uint64_t>(x) + 16 * sub;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) v[i] = ld(x, LAST ? chunk(i) : min(chunk(i), nch - 1));
+    for (int i = 0; i < NI; ++i) v[i] = LAST && i < NI - 1 ? gld16(b + 16 * kLanes * i) : ld(x, min(chunk(i), nch - 1));
+  }
+  __device__ __forceinline__ void load_normed(const uint8_t* x) {
+    const int last = max(nn - 1, 0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) v[i] = ld(x, min(chunk(i), last));
   }
   // y (channels of chunk c) rotated by the position's angles; `other` holds the
   // partner chunk's channels (HALF)
   __device__ __forceinline__ void rotate(const RopeParams& p, const float* cs, int c, const float (&y)[8],
                                          const float (&other)[8], float sign, float (&o)[8]) const {
+    constexpr int NE = HALF ? 4 : 2;   // (cos, sin, cos, sin) of two pairs each
+    const int j = c - rc0;
+    const bool first = j < hc;
+    const uint64_t at = reinterpret_cast<uint64_t>(cs) + (HALF ? 64 * (first ? j : j - hc) : 32 * j);
+    float4 e[NE];
+#pragma unroll
+    for (int k = 0; k < NE; ++k) e[k] = __builtin_bit_cast(float4, gld16(at + 16 * k));
+#pragma unroll
+    for (int k = 0; k < NE; ++k) opaque(e[k]);
     if constexpr (HALF) {
-      const int j = c - rc0;
-      const bool first = j < hc;
-      const float4* e = reinterpret_cast<const float4*>(cs + 16 * (first ? j : j - hc));
+      const float s = first ? -sign : sign;   // first half: a c - b s; second: b c + a s, the pair's other in `other`
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float4 a = e[k];
-        // first half: a c - b s; second: b c + a s, `other` being the pair's other channel
-        const float s0 = first ? -sign * a.y : sign * a.y, s1 = first ? -sign * a.w : sign * a.w;
-        o[2 * k] = fmaf(y[2 * k], a.x, other[2 * k] * s0);
-        o[2 * k + 1] = fmaf(y[2 * k + 1], a.z, other[2 * k + 1] * s1);
+        o[2 * k] = fmaf(y[2 * k], e[k].x, other[2 * k] * (s * e[k].y));
+        o[2 * k + 1] = fmaf(y[2 * k + 1], e[k].z, other[2 * k + 1] * (s * e[k].w));
       }
     } else {
-      const float4* e = reinterpret_cast<const float4*>(cs + 8 * (c - rc0));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float4 a = e[k];
-        o[4 * k] = fmaf(y[4 * k], a.x, -sign * a.y * y[4 * k + 1]);
-        o[4 * k + 1] = fmaf(y[4 * k + 1], a.x, sign * a.y * y[4 * k]);
-        o[4 * k + 2] = fmaf(y[4 * k + 2], a.z, -sign * a.w * y[4 * k + 3]);
-        o[4 * k + 3] = fmaf(y[4 * k + 3], a.z, sign * a.w * y[4 * k + 2]);
+        const float s0 = sign * e[k].y, s1 = sign * e[k].w;
+        o[4 * k] = fmaf(y[4 * k], e[k].x, -s0 * y[4 * k + 1]);
+        o[4 * k + 1] = fmaf(y[4 * k + 1], e[k].x, s0 * y[4 * k]);
+        o[4 * k + 2] = fmaf(y[4 * k + 2], e[k].z, -s1 * y[4 * k + 3]);
+        o[4 * k + 3] = fmaf(y[4 * k + 3], e[k].z, s1 * y[4 * k + 2]);
       }
     }
   }
@@ -177,54 +236,50 @@ struct Row {
 // type, 656-byte fp8 rows of the paged cache.
 enum { kToRows = 0, kToCache = 1, kToFp8 = 2 };
 
-// latent channels of iterations 2 g and 2 g + 1 are one 128-channel scale group
-__device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, const float (&a)[8], const float (&b)[8],
-                                              bool write) {
+// 128 latent channels, one iteration of the row's lanes, share a scale
+__device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, const float (&x)[8], bool write) {
   float amax = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fmaxf(fabsf(a[k]), fabsf(b[k])));
-  amax = max8(amax);
+  for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
+  amax = max16(amax);
   const float scale = amax > 0.f ? amax / kFp8Max : 1.f;
   // (at most the largest float: zeros beside channels below 1e-36 stay zeros)
   const float inv = amax > 0.f ? fminf(kFp8Max / amax, 3.402823466e38f) : 1.f;
+  uint32_t q[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float (&x)[8] = h ? b : a;
-    uint32_t q[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      auto cl = [&](float f) { return __builtin_amdgcn_fmed3f(f * inv, -kFp8Max, kFp8Max); };
-      int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j]), cl(x[4 * j + 1]), 0, false);
-      t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j + 2]), cl(x[4 * j + 3]), t, true);
-      q[j] = (uint32_t)t;
-    }
-    if (write) *reinterpret_cast<uint2*>(dst + 128 * g + 64 * h + 8 * sub) = make_uint2(q[0], q[1]);
+  for (int j = 0; j < 2; ++j) {
+    auto cl = [&](float f) { return __builtin_amdgcn_fmed3f(f * inv, -kFp8Max, kFp8Max); };
+    int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j]), cl(x[4 * j + 1]), 0, false);
+    t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j + 2]), cl(x[4 * j + 3]), t, true);
+    q[j] = (uint32_t)t;
   }
-  if (write && sub == 0) *reinterpret_cast<float*>(dst + kFp8ScaleOff + 4 * g) = scale;
+  if (!write) return;
+  *reinterpret_cast<uint2*>(dst + 128 * g + 8 * sub) = make_uint2(q[0], q[1]);
+  if (sub == 0) *reinterpret_cast<float*>(dst + kFp8ScaleOff + 4 * g) = scale;
 }
 
-// Rows of one part: workgroup `blk` of its grid.
+// Rows of one part: workgroup `blk` of its grid. `cached`: they go to the cache
+// (workgroup-uniform; DST says how).
 template <typename QT, int NI, bool LAST, bool HALF, int DST, bool APPEND>
-__device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a, uint32_t blk, int tid) {
+__device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a, uint32_t blk, int tid, float* lds,
+                                          bool cached) {
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t r0 = blk * kRopeRows + wave * 8;   // the wave's first row
-  if (r0 >= a.rows) return;
-  const uint32_t row = r0 + (lane >> 3);
-  const bool live = row < a.rows;
-  // its token and head: one division for the wave, the rows after it step on
-  uint32_t t = r0 / a.H, h = r0 - t * a.H + (lane >> 3);
-  if (a.H >= 8) {
-    if (h >= a.H) { h -= a.H; ++t; }
-  } else {
-    const uint32_t k = h / a.H;
-    t += k;
-    h -= k * a.H;
-  }
-  if (!live) { t = r0 / a.H; h = r0 - t * a.H; }   // a row to load; nothing of it is stored
-
+  const uint32_t w0 = blk * kRopeRows + wave * kWaveRows;   // the wave's first row
+  const uint32_t r0 = w0 < a.rows ? w0 : 0;                 // (a wave without rows stays for the barrier)
+  const uint32_t row = r0 + lane / kLanes;
+  const bool live = row < a.rows && w0 < a.rows;
+  const auto [t, h] = head_of(r0, a.H, lane, live);
   Row<QT, NI, LAST, HALF> r(p, a.n, lane);
   const uint8_t* x = a.x + (long long)t * a.st + (long long)h * a.sh;
-  r.load(x);
+  if (a.w) {   // workgroup-uniform
+    Weights<QT, NI> w;
+    w.get(p, a, tid);
+    r.load(x);
+    w.put(lds, tid);
+  } else {
+    r.load(x);
+  }
+  if (w0 >= a.rows) return;
 
   Place at{0, 0, false};
   if constexpr (APPEND) at = place_of(p, (int)t, lane);
@@ -233,8 +288,8 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
   const bool in = (!p.R || (pos >= 0 && pos < p.table_rows)) && !at.padded;
   const float* cs = p.table + (size_t)(in ? pos : 0) * p.R;
   uint8_t* dst = nullptr;
-  if constexpr (DST == kToRows) {
-    dst = a.y + (size_t)row * p.D * 2;
+  if (!cached) {
+    if (live) dst = a.y + (size_t)row * p.D * 2;
   } else {
     const int blkno = in ? at.slot / p.bs : 0;
     const bool okt = in && blkno < p.bt_stride;
@@ -242,7 +297,7 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
     if (live && okt && phys >= 0 && phys < p.nblocks)
       dst = p.cache + ((size_t)phys * p.bs + (at.slot - blkno * p.bs)) * (DST == kToFp8 ? kRow656 : p.D * 2);
   }
-  const bool write = DST == kToRows ? live : dst != nullptr;
+  const bool write = dst != nullptr;
 
   // the norm
   float rinv = 1.f;
@@ -256,25 +311,28 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
       for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
       ss += r.chunk(i) < r.nn ? s : 0.f;
     }
-    rinv = rsqrtf(sum8(ss) / (float)a.n + p.eps);
+    rinv = rsqrtf(sum16(ss) / (float)a.n + p.eps);
   }
   auto normed = [&](const uint4& v, int c, float (&f)[8]) {
     unpack8<QT>(v, f);
-    if (c < r.nn) {
+    const float s = c < r.nn ? rinv : 1.f;
+    if (a.w) {
       float w[8];
-      if (a.w) weights8<QT>(p, a.w, c, w);
+      weights8(lds_addr_of(lds), c, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= a.w ? rinv * w[k] : rinv;
+      for (int k = 0; k < 8; ++k) f[k] *= s * w[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= s;
     }
   };
-  float keep[8];   // fp8: the first chunk of a scale group's two
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = r.chunk(i);
     float f[8];
     normed(r.v[i], c, f);
     if (p.R && r.turns(i)) {
-      const bool turn = LAST || (c >= r.rc0 && c < r.nch);
+      const bool turn = c >= r.rc0 && c < r.nch;
       const int ct = turn ? c : r.rc0;
       float other[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
       if constexpr (HALF) {
@@ -286,18 +344,11 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
       for (int k = 0; k < 8; ++k) f[k] = turn ? o[k] : f[k];
     }
     if constexpr (DST == kToFp8) {
-      if (i < 8) {
-        if (i & 1) put_fp8_group(dst, i >> 1, r.sub, keep, f, write);
-        else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) keep[k] = f[k];
-        }
-      } else if (write) {
-        *reinterpret_cast<uint4*>(dst + kFp8RopeOff + 16 * r.sub) = pack8<__bf16>(f);
-      }
+      if (i < 4) put_fp8_group(dst, i, r.sub, f, write);
+      else if (write && r.sub < 8) *reinterpret_cast<uint4*>(dst + kFp8RopeOff + 16 * r.sub) = pack8<__bf16>(f);
     } else if (write && r.has(i)) {
       uint4 o = pack8<QT>(f);
-      if (DST == kToRows && !in) o = make_uint4(0, 0, 0, 0);   // a padded row
+      if (!in) o = make_uint4(0, 0, 0, 0);   // a padded row (of the queries: none goes to the cache)
       *reinterpret_cast<uint4*>(dst + 16 * c) = o;
     }
   }
@@ -308,9 +359,17 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
 template <typename QT, int NI, bool LAST, bool HALF, int DST>
 __global__ void __launch_bounds__(kRopeThreads) sas_rope_kernel(const RopeParams p) {
   constexpr bool kAppend = DST != kToRows;
+  __shared__ __attribute__((aligned(16))) float lds[Weights<QT, NI>::kAll];
   const uint32_t b = blockIdx.x, nkv = (uint32_t)p.part[0].blocks;
-  if (b < nkv) rope_rows<QT, NI, LAST, HALF, DST, kAppend>(p, p.part[0], b, threadIdx.x);
-  else rope_rows<QT, NI, LAST, HALF, kToRows, kAppend>(p, p.part[1], b - nkv, threadIdx.x);
+  // one copy of the code where it can be: its first fetch is much of a small call
+  const RopePart& a = p.part[b < nkv ? 0 : 1];
+  const uint32_t blk = b < nkv ? b : b - nkv;
+  if constexpr (DST == kToFp8) {
+    if (b < nkv) rope_rows<QT, NI, LAST, HALF, kToFp8, true>(p, a, blk, threadIdx.x, lds, true);
+    else rope_rows<QT, NI, LAST, HALF, kToCache, true>(p, a, blk, threadIdx.x, lds, false);
+  } else {
+    rope_rows<QT, NI, LAST, HALF, DST, kAppend>(p, a, blk, threadIdx.x, lds, kAppend && b < nkv);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -320,152 +379,171 @@ __global__ void __launch_bounds__(kRopeThreads) sas_rope_kernel(const RopeParams
 // A workgroup walks its part's rows; with weights every lane sums its channels'
 // weight gradients in registers, the workgroup adds them up through LDS once
 // at its end and leaves one partial row: no atomics, the same order every time.
+// W: weight gradients are wanted of a part at least (else none has weights in
+// need of sums; weights themselves may be there).
 template <typename QT, int NI, bool LAST, bool HALF, bool W>
-__device__ __forceinline__ void rope_grad_rows(const RopeParams& p, const RopePart& a, uint32_t blk, int tid,
-                                               float* lds) {
-  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+__global__ void __launch_bounds__(kRopeThreads, NI <= 5 ? 3 : 2) sas_rope_grad_kernel(const RopeParams p) {
+  constexpr int kWaves = kRopeThreads / 64;
+  constexpr int kAll = Weights<QT, NI>::kAll;
+  __shared__ __attribute__((aligned(16))) float lds[W ? kWaves * kAll : kAll];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t nkv = (uint32_t)p.part[0].blocks;
+  const RopePart& a = p.part[blockIdx.x < nkv ? 0 : 1];
+  const uint32_t blk = blockIdx.x < nkv ? blockIdx.x : blockIdx.x - nkv;
+  {
+    Weights<QT, NI> w;   // ones where there are none
+    w.get(p, a, tid);
+    w.put(lds, tid);
+  }
   float dw[W ? NI : 1][8];
 #pragma unroll
   for (int i = 0; i < (W ? NI : 1); ++i)
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = 0.f;
   Row<QT, NI, LAST, HALF> r(p, a.n, lane), g(p, a.n, lane);
-  for (uint32_t r0 = blk * kRopeRows + wave * 8; r0 < a.rows; r0 += (uint32_t)a.blocks * kRopeRows) {
-    const uint32_t row = r0 + (lane >> 3);
+  for (uint32_t r0 = blk * kRopeRows + wave * kWaveRows; r0 < a.rows; r0 += (uint32_t)a.blocks * kRopeRows) {
+    const uint32_t row = r0 + lane / kLanes;
     const bool live = row < a.rows;
-    uint32_t t = r0 / a.H, h = r0 - t * a.H + (lane >> 3);
-    if (a.H >= 8) {
-      if (h >= a.H) { h -= a.H; ++t; }
-    } else {
-      const uint32_t k = h / a.H;
-      t += k;
-      h -= k * a.H;
-    }
-    if (!live) { t = r0 / a.H; h = r0 - t * a.H; }
-    r.load(a.x + (long long)t * a.st + (long long)h * a.sh);
+    const auto [t, h] = head_of(r0, a.H, lane, live);
+    const int pos = p.R ? p.pos[t] : 0;
+    // (kept out of registers: hoisted out of the loop the weights cost a wave a SIMD)
+    uint32_t wl = lds_addr_of(lds);
+    asm volatile("" : "+v"(wl));
+    // x of normed channels alone is needed: the others' lines are not fetched
+    r.load_normed(a.x + (long long)t * a.st + (long long)h * a.sh);
     const uint8_t* dy = a.dy + (long long)t * a.dst + (long long)h * a.dsh;
     g.load(dy);
-    const int pos = p.R ? p.pos[t] : 0;
     const bool in = live && (!p.R || (pos >= 0 && pos < p.table_rows));
     const float* cs = p.table + (size_t)(in ? pos : 0) * p.R;
-    // dy rotated back, in place (HALF: partners come from memory again, which is still dy)
-    float ut[LAST ? 1 : NI][8];   // rotated chunks, in 32 bits
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      if (!(p.R && r.turns(i))) continue;
-      const int c = r.chunk(i);
-      const bool turn = LAST || (c >= r.rc0 && c < r.nch);
-      const int ct = turn ? c : r.rc0;
-      float f[8], other[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
-      unpack8<QT>(g.v[i], f);
-      if constexpr (HALF) unpack8<QT>(r.ld(dy, r.partner(ct)), other);
-      r.rotate(p, cs, ct, f, other, -p.sign, o);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) ut[LAST ? 0 : i][k] = turn ? o[k] : f[k];
-    }
+    // u = dy rotated back, of iteration i
     auto grad = [&](int i, float (&u)[8]) {
+      unpack8<QT>(g.v[i], u);
       if (p.R && r.turns(i)) {
+        const int c = r.chunk(i);
+        const bool turn = c >= r.rc0 && c < r.nch;
+        const int ct = turn ? c : r.rc0;
+        float other[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
+        if constexpr (HALF) unpack8<QT>(r.ld(dy, r.partner(ct)), other);
+        r.rotate(p, cs, ct, u, other, -p.sign, o);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) u[k] = ut[LAST ? 0 : i][k];
-      } else {
-        unpack8<QT>(g.v[i], u);
+        for (int k = 0; k < 8; ++k) u[k] = turn ? (in ? o[k] : 0.f) : u[k];
       }
     };
-    float rinv = 1.f, m = 0.f;
-    if (a.n) {
-      float ss = 0.f, sg = 0.f;
+    // the rotated channels of the builds with one such iteration are kept, the
+    // others' made twice
+    float last[8];
+    if constexpr (LAST) grad(NI - 1, last);
+    auto get = [&](int i, float (&u)[8]) {
+      if (LAST && i == NI - 1) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c = r.chunk(i);
-        if (!(c < r.nn)) continue;
-        float f[8], u[8], w[8];
-        unpack8<QT>(r.v[i], f);
+        for (int k = 0; k < 8; ++k) u[k] = last[k];
+      } else {
         grad(i, u);
-        if (a.w) weights8<QT>(p, a.w, c, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          ss = fmaf(f[k], f[k], ss);
-          sg = fmaf(a.w ? u[k] * w[k] : u[k], f[k], sg);
-        }
       }
-      rinv = rsqrtf(sum8(ss) / (float)a.n + p.eps);
-      m = sum8(sg) / (float)a.n * rinv * rinv;
+    };
+    // x of the other channels, and rows that are padding or past the last one,
+    // count as zeros whatever they hold
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if (!in || r.chunk(i) >= r.nn) r.v[i] = make_uint4(0, 0, 0, 0);
+      if (!in) g.v[i] = make_uint4(0, 0, 0, 0);
+      opaque(r.v[i]);
+      opaque(g.v[i]);
     }
-    uint8_t* dst = a.y + (size_t)row * p.D * 2;
+    if constexpr (LAST) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) last[k] = in ? last[k] : 0.f;
+    }
+    float ss = 0.f, sg = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = r.chunk(i);
-      float u[8], o[8];
-      grad(i, u);
-      if (c < r.nn) {
-        float f[8], w[8];
-        unpack8<QT>(r.v[i], f);
-        if (a.w) weights8<QT>(p, a.w, c, w);
+      float f[8], u[8], w[8], s2 = 0.f;
+      unpack8<QT>(r.v[i], f);
+      get(i, u);
+      weights8(wl, c, w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          o[k] = rinv * ((a.w ? u[k] * w[k] : u[k]) - f[k] * m);
-          if constexpr (W) dw[i][k] += in ? u[k] * (f[k] * rinv) : 0.f;
-        }
-      } else {
+      for (int k = 0; k < 8; ++k) {
+        ss = fmaf(f[k], f[k], ss);
+        s2 = fmaf(u[k] * w[k], f[k], s2);
+      }
+      sg += c < r.nn ? s2 : 0.f;   // (an infinite gradient of the other channels stays out)
+      __builtin_amdgcn_sched_barrier(0);   // chunk by chunk: their 32-bit values all at once spill
+    }
+    const float n = (float)max(a.n, 1);
+    float rinv = rsqrtf(sum16(ss) / n + p.eps);
+    opaque(rinv);
+    rinv = in ? rinv : 0.f;   // (eps 0: no infinity in a padded row)
+    const float m = sum16(sg) / n * rinv * rinv * rinv;
+    uint8_t* dst = a.y + (size_t)row * p.D * 2 + 16 * r.sub;
+    // the second pass unpacks anew: kept from the first, the values in 32 bits spill
+    asm volatile("" : "+v"(wl));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = u[k];
+    for (int i = 0; i < NI; ++i) {
+      opaque(r.v[i]);
+      opaque(g.v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = r.chunk(i);
+      float f[8], u[8], w[8], o[8];
+      unpack8<QT>(r.v[i], f);
+      get(i, u);
+      weights8(wl, c, w);
+      // past the normed channels: u 1 - 0 0
+      const float ri = c < r.nn ? rinv : 1.f, mi = c < r.nn ? m : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        o[k] = fmaf(u[k] * w[k], ri, -(f[k] * mi));
+        if constexpr (W) dw[i][k] = fmaf(u[k], f[k] * rinv, dw[i][k]);   // (past n: never read)
       }
-      if (live && r.has(i)) {
-        uint4 v = pack8<QT>(o);
-        if (!in) v = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + 16 * c) = v;
-      }
+      const uint4 v = pack8<QT>(o);
+      if (live && r.has(i)) *reinterpret_cast<uint4*>(dst + 16 * kLanes * i) = v;
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   if constexpr (W) {
     if (!a.dw) return;   // workgroup-uniform
-    // the wave's eight rows, then its four waves
+    lds_barrier();       // every wave has done with the weights
+    asm volatile("" ::: "memory");
+    // the wave's four rows, then its four waves
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float s = dw[i][k];
-        s += dpp<0x128>(s);   // the other row of the 16 lanes
-        s = rows_sum(s);
-        if (lane < 8) lds[wave * (NI * 64) + r.chunk(i) * 8 + k] = s;
+        const float s = rows_sum(dw[i][k]);
+        if (lane < kLanes) lds[wave * kAll + r.chunk(i) * 8 + k] = s;
       }
     }
     __syncthreads();
     for (int j = tid; j < a.n; j += kRopeThreads) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRopeThreads / 64; ++w) s += lds[w * (NI * 64) + j];
+      for (int w = 0; w < kWaves; ++w) s += lds[w * kAll + j];
       a.dw[(size_t)blk * p.D + j] = s;
     }
   }
 }
 
-template <typename QT, int NI, bool LAST, bool HALF, bool W>
-__global__ void __launch_bounds__(kRopeThreads) sas_rope_grad_kernel(const RopeParams p) {
-  __shared__ float lds[W ? (kRopeThreads / 64) * NI * 64 : 1];
-  const uint32_t b = blockIdx.x, nkv = (uint32_t)p.part[0].blocks;
-  if (b < nkv) rope_grad_rows<QT, NI, LAST, HALF, W>(p, p.part[0], b, threadIdx.x, lds);
-  else rope_grad_rows<QT, NI, LAST, HALF, W>(p, p.part[1], b - nkv, threadIdx.x, lds);
-}
-
-// Weight gradients from the workgroups' partial rows: 16 channels a workgroup, 16
-// threads a channel, in a fixed order.
+// Weight gradients from the workgroups' partial rows: 16 channels a workgroup, 64
+// threads a channel (16: 4.2 us for 512 rows, a load after the other), in a fixed order.
 struct RopeSum { const float* part[2]; float* dw[2]; int rows[2], n[2], D; };
-__global__ void __launch_bounds__(256) sas_rope_dw_kernel(const RopeSum s) {
-  __shared__ float lds[16][17];
+constexpr int kSumThreads = 1024, kSumRows = kSumThreads / 16;
+__global__ void __launch_bounds__(kSumThreads) sas_rope_dw_kernel(const RopeSum s) {
+  __shared__ float lds[kSumRows][17];
   const int w = blockIdx.y, c = threadIdx.x & 15, k = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
-  if (!s.dw[w]) return;
+  if (!s.dw[w]) return;   // workgroup-uniform
   float v = 0.f;
   if (j < s.n[w]) {
 #pragma unroll 8
-    for (int i = k; i < s.rows[w]; i += 16) v += s.part[w][(size_t)i * s.D + j];
+    for (int i = k; i < s.rows[w]; i += kSumRows) v += s.part[w][(size_t)i * s.D + j];
   }
   lds[k][c] = v;
   __syncthreads();
   if (k == 0 && j < s.n[w]) {
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += lds[i][c];
+    for (int i = 0; i < kSumRows; ++i) v += lds[i][c];
     s.dw[w][j] = v;
   }
 }
@@ -533,17 +611,17 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
 }
 
 // The kernel for a row width: 128, 512 or 576 channels with 64 rotated ones (or none) in
-// their own builds, any other in one of up to 16 chunks a lane.
+// their own builds, any other in one of up to eight chunks a lane.
 template <typename F>
 int by_width(const SasNormRopeArgs* a, F&& f) {
   const bool last = a->rope_dim == 64 || a->rope_dim == 0;
   auto half = [&](auto ni, auto l) {
     return a->flags & SAS_ROPE_HALF ? f(ni, l, std::true_type{}) : f(ni, l, std::false_type{});
   };
-  if (last && a->D == 576) return half(std::integral_constant<int, 9>{}, std::true_type{});
-  if (last && a->D == 512) return half(std::integral_constant<int, 8>{}, std::true_type{});
-  if (last && a->D == 128) return half(std::integral_constant<int, 2>{}, std::true_type{});
-  return half(std::integral_constant<int, 16>{}, std::false_type{});
+  if (last && a->D == 576) return half(std::integral_constant<int, 5>{}, std::true_type{});
+  if (last && a->D == 512) return half(std::integral_constant<int, 4>{}, std::true_type{});
+  if (last && a->D == 128) return half(std::integral_constant<int, 1>{}, std::true_type{});
+  return half(std::integral_constant<int, 8>{}, std::false_type{});
 }
 
 int launched(const char* what) {
@@ -565,11 +643,11 @@ int launch_rope(const SasNormRopeArgs* a, const RopeParams& p, hipStream_t st, c
   });
 }
 
-// Workgroups of the backward's two parts: two a CU (a build holds 2 to 3 waves a
+// Workgroups of the backward's two parts: three a CU (what the builds with weights hold, 3 waves a
 // SIMD), shared out by rows, none without rows of its own.
 void grad_blocks(RopeParams* p) {
   const double all = (double)p->part[0].rows + p->part[1].rows;
-  const long long most = 2LL * device_cus();
+  const long long most = 3LL * device_cus();
   for (RopePart& x : p->part) {
     const long long full = ((long long)x.rows + kRopeRows - 1) / kRopeRows;
     const long long share = std::max<long long>(1, (long long)(most * (double)x.rows / std::max(all, 1.0) + 0.5));
@@ -677,7 +755,7 @@ extern "C" int sas_norm_rope_bwd_v1(const SasNormRopeBwdArgs* a, void* stream) {
     if (e) return e;
   }
   if (dw[0] || dw[1]) {
-    hipLaunchKernelGGL(sas_rope_dw_kernel, dim3((unsigned)((f->D + 15) / 16), 2), dim3(256), 0, st, s);
+    hipLaunchKernelGGL(sas_rope_dw_kernel, dim3((unsigned)((f->D + 15) / 16), 2), dim3(kSumThreads), 0, st, s);
     return launched("norm_rope_bwd");
   }
   return SAS_OK;
@@ -713,11 +791,11 @@ extern "C" int sas_cache_append_v1(const SasCacheAppendArgs* a, void* stream) {
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   const bool half = r->flags & SAS_ROPE_HALF;
   if (r->rope_dim == 64 || r->rope_dim == 0) {
-    if (half) go(sas_rope_kernel<__bf16, 9, true, true, kToFp8>);
-    else go(sas_rope_kernel<__bf16, 9, true, false, kToFp8>);
+    if (half) go(sas_rope_kernel<__bf16, 5, true, true, kToFp8>);
+    else go(sas_rope_kernel<__bf16, 5, true, false, kToFp8>);
   } else {
-    if (half) go(sas_rope_kernel<__bf16, 9, false, true, kToFp8>);
-    else go(sas_rope_kernel<__bf16, 9, false, false, kToFp8>);
+    if (half) go(sas_rope_kernel<__bf16, 5, false, true, kToFp8>);
+    else go(sas_rope_kernel<__bf16, 5, false, false, kToFp8>);
   }
   return launched("cache_append");
 }
