@@ -48,6 +48,7 @@ struct RopeParams {
   int table_rows, D, R, T;
   int wf32;                    // weights are fp32 (else the rows' type)
   float eps, sign;             // sign of the rotation
+  int nt_load, nt_store;       // rows are read / written non-temporally
   // append
   const int32_t* cu;           // [B + 1]
   const int32_t* used;         // [B]
@@ -79,6 +80,32 @@ __device__ __forceinline__ float max16(float x) {
 __device__ __forceinline__ void opaque(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 __device__ __forceinline__ void opaque(float4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
 __device__ __forceinline__ void opaque(float& v) { asm volatile("" : "+v"(v)); }
+
+// 16 bytes of a row, past the caches with NT
+template <bool NT>
+__device__ __forceinline__ uint4 ld16(uint64_t a) {
+  const SAS_GLOBAL u32x4g* p = reinterpret_cast<const SAS_GLOBAL u32x4g*>(a);
+  return __builtin_bit_cast(uint4, NT ? __builtin_nontemporal_load(p) : *p);
+}
+// One of two branches that differ in nothing but NT: the compiler would merge
+// them and drop it.
+template <typename F, typename G>
+__device__ __forceinline__ void either(int nt, F&& yes, G&& no) {
+  if (nt) {
+    asm volatile("; nt" ::: "memory");
+    yes();
+    asm volatile("; nt end" ::: "memory");
+  } else {
+    asm volatile("; cached" ::: "memory");
+    no();
+    asm volatile("; cached end" ::: "memory");
+  }
+}
+__device__ __forceinline__ void st16(uint8_t* p, const uint4& v, int nt) {
+  u32x4g* d = reinterpret_cast<u32x4g*>(p);
+  const u32x4g w = __builtin_bit_cast(u32x4g, v);
+  either(nt, [&] { __builtin_nontemporal_store(w, d); }, [&] { *d = w; });
+}
 
 template <typename QT>
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -128,24 +155,28 @@ __device__ __forceinline__ void weights8(uint32_t lds, int c, float (&f)[8]) {
 
 // Token -> (sequence, place): the largest b with cu[b] <= t, one ballot per row and 64
 // sequences. Every lane of the wave takes part; `t` is the token of the lane's row.
+// `seq` holds the lane's own sequence of the first 64, loaded ahead of the row.
+struct Seq { int q0, q1, kv; };
+__device__ __forceinline__ Seq seq_of(const RopeParams& p, int i) {
+  return i < p.B ? Seq{p.cu[i], p.cu[i + 1], p.used[i]} : Seq{INT_MAX, 0, 0};
+}
 struct Place { int slot, b; bool padded; };
-__device__ __forceinline__ Place place_of(const RopeParams& p, int t, int lane) {
+__device__ __forceinline__ Place place_of(const RopeParams& p, Seq seq, int t, int lane) {
   Place o{0, 0, true};
   int len = 0, start = 0;
-  for (int c0 = 0; c0 < p.B; c0 += 64) {
-    const int i = c0 + lane;
-    int q0 = INT_MAX, q1 = 0, kv = 0;
-    if (i < p.B) { q0 = p.cu[i]; q1 = p.cu[i + 1]; kv = p.used[i]; }
+  for (int c0 = 0;;) {
     int n = 0;
 #pragma unroll
     for (int j = 0; j < kWaveRows; ++j) {
-      const int m = __popcll(__ballot(q0 <= __builtin_amdgcn_readlane(t, kLanes * j)));
+      const int m = __popcll(__ballot(seq.q0 <= __builtin_amdgcn_readlane(t, kLanes * j)));
       n = lane / kLanes == j ? m : n;
     }
     const int at = max(n - 1, 0);
-    const int s = __shfl(q0, at), e = __shfl(q1, at), u = __shfl(kv, at);
+    const int s = __shfl(seq.q0, at), e = __shfl(seq.q1, at), u = __shfl(seq.kv, at);
     if (n > 0) { o.b = c0 + at; start = s; len = e - s; o.slot = u - len + (t - s); o.padded = false; }
-    if (__ballot(n == 64) == 0) break;   // wave-uniform: no row's sequence lies further on
+    c0 += 64;
+    if (c0 >= p.B || __ballot(n == 64) == 0) break;   // wave-uniform: no row's sequence lies further on
+    seq = seq_of(p, c0 + lane);
   }
   o.padded = o.padded || t < start || t - start >= len || o.slot < 0;
   return o;
@@ -187,37 +218,55 @@ struct Row {
   __device__ __forceinline__ static uint4 ld(const uint8_t* x, int c) {
     return gld16(reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)c);
   }
-  // every lane loads; chunks past the first `most` are clamped to the last of them
-  // (a line that is fetched anyway)
+  // every lane loads; chunks past the row's (normed: past its normed ones, whose
+  // lines are then not fetched) are clamped to the last of them
+  template <bool NT>
   __device__ __forceinline__ void load(const uint8_t* x) {
     const uint64_t b = reinterpret_cast<uint64_t>(x) + 16 * sub;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) v[i] = LAST && i < NI - 1 ? gld16(b + 16 * kLanes * i) : ld(x, min(chunk(i), nch - 1));
+    for (int i = 0; i < NI; ++i)
+      v[i] = ld16<NT>(LAST && i < NI - 1 ? b + 16 * kLanes * i
+                                         : reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)min(chunk(i), nch - 1));
   }
+  template <bool NT>
   __device__ __forceinline__ void load_normed(const uint8_t* x) {
     const int last = max(nn - 1, 0);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) v[i] = ld(x, min(chunk(i), last));
+    for (int i = 0; i < NI; ++i) v[i] = ld16<NT>(reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)min(chunk(i), last));
   }
-  // y (channels of chunk c) rotated by the position's angles; `other` holds the
-  // partner chunk's channels (HALF)
-  __device__ __forceinline__ void rotate(const RopeParams& p, const float* cs, int c, const float (&y)[8],
-                                         const float (&other)[8], float sign, float (&o)[8]) const {
-    constexpr int NE = HALF ? 4 : 2;   // (cos, sin, cos, sin) of two pairs each
-    const int j = c - rc0;
-    const bool first = j < hc;
-    const uint64_t at = reinterpret_cast<uint64_t>(cs) + (HALF ? 64 * (first ? j : j - hc) : 32 * j);
-    float4 e[NE];
+};
+
+// The rotation of one chunk: the angles of its pairs and, where these lie apart
+// (HALF), the pairs' other channels, loaded as early as the position is known.
+template <typename QT, bool HALF>
+struct Turn {
+  static constexpr int NE = HALF ? 4 : 2;   // (cos, sin, cos, sin) of two pairs each
+  float4 e[NE];
+  uint4 other;
+  int j, hc;
+  // chunk c of the row x; a chunk that is not rotated loads the first rotated one's
+  template <typename R>
+  __device__ __forceinline__ void load(const R& r, const float* cs, const uint8_t* x, int c) {
+    hc = r.hc;
+    const bool turn = c >= r.rc0 && c < r.nch;
+    j = turn ? c - r.rc0 : 0;
+    const uint64_t at = reinterpret_cast<uint64_t>(cs) + (HALF ? 64 * (j < hc ? j : j - hc) : 32 * j);
 #pragma unroll
     for (int k = 0; k < NE; ++k) e[k] = __builtin_bit_cast(float4, gld16(at + 16 * k));
+    if constexpr (HALF) other = gld16(reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)r.partner(r.rc0 + j));
+  }
+  __device__ __forceinline__ void ready() {
 #pragma unroll
     for (int k = 0; k < NE; ++k) opaque(e[k]);
+  }
+  // y rotated, z being its pairs' other channels (HALF)
+  __device__ __forceinline__ void turn(const float (&y)[8], const float (&z)[8], float sign, float (&o)[8]) const {
     if constexpr (HALF) {
-      const float s = first ? -sign : sign;   // first half: a c - b s; second: b c + a s, the pair's other in `other`
+      const float s = j < hc ? -sign : sign;   // first half: a c - b s; second: b c + a s
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        o[2 * k] = fmaf(y[2 * k], e[k].x, other[2 * k] * (s * e[k].y));
-        o[2 * k + 1] = fmaf(y[2 * k + 1], e[k].z, other[2 * k + 1] * (s * e[k].w));
+        o[2 * k] = fmaf(y[2 * k], e[k].x, z[2 * k] * (s * e[k].y));
+        o[2 * k + 1] = fmaf(y[2 * k + 1], e[k].z, z[2 * k + 1] * (s * e[k].w));
       }
     } else {
 #pragma unroll
@@ -271,22 +320,29 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
   const auto [t, h] = head_of(r0, a.H, lane, live);
   Row<QT, NI, LAST, HALF> r(p, a.n, lane);
   const uint8_t* x = a.x + (long long)t * a.st + (long long)h * a.sh;
+  // what positions and places hang on goes first, the row behind it
+  Seq seq{};
+  if constexpr (APPEND) seq = seq_of(p, lane);
+  int pos = 0;
+  const bool own = !APPEND || p.pos;   // positions are given
+  if (p.R && own) pos = p.pos[t];
   if (a.w) {   // workgroup-uniform
     Weights<QT, NI> w;
     w.get(p, a, tid);
-    r.load(x);
+    either(p.nt_load, [&] { r.template load<true>(x); }, [&] { r.template load<false>(x); });
     w.put(lds, tid);
   } else {
-    r.load(x);
+    either(p.nt_load, [&] { r.template load<true>(x); }, [&] { r.template load<false>(x); });
   }
   if (w0 >= a.rows) return;
 
   Place at{0, 0, false};
-  if constexpr (APPEND) at = place_of(p, (int)t, lane);
-  int pos = 0;
-  if (p.R) pos = APPEND && !p.pos ? at.slot : p.pos[t];
+  if constexpr (APPEND) at = place_of(p, seq, (int)t, lane);
+  if (!own) pos = at.slot;
   const bool in = (!p.R || (pos >= 0 && pos < p.table_rows)) && !at.padded;
   const float* cs = p.table + (size_t)(in ? pos : 0) * p.R;
+  Turn<QT, HALF> last;   // of iteration NI - 1
+  if (LAST && p.R) last.load(r, cs, x, r.chunk(NI - 1));
   uint8_t* dst = nullptr;
   if (!cached) {
     if (live) dst = a.y + (size_t)row * p.D * 2;
@@ -332,16 +388,15 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
     float f[8];
     normed(r.v[i], c, f);
     if (p.R && r.turns(i)) {
-      const bool turn = c >= r.rc0 && c < r.nch;
-      const int ct = turn ? c : r.rc0;
+      Turn<QT, HALF> one;
+      if constexpr (!LAST) one.load(r, cs, x, c);
+      Turn<QT, HALF>& e = LAST ? last : one;
+      e.ready();
       float other[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
-      if constexpr (HALF) {
-        const int pc = r.partner(ct);
-        normed(r.ld(x, pc), pc, other);
-      }
-      r.rotate(p, cs, ct, f, other, p.sign, o);
+      if constexpr (HALF) normed(e.other, r.partner(r.rc0 + e.j), other);
+      e.turn(f, other, p.sign, o);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = turn ? o[k] : f[k];
+      for (int k = 0; k < 8; ++k) f[k] = c >= r.rc0 && c < r.nch ? o[k] : f[k];
     }
     if constexpr (DST == kToFp8) {
       if (i < 4) put_fp8_group(dst, i, r.sub, f, write);
@@ -349,7 +404,7 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
     } else if (write && r.has(i)) {
       uint4 o = pack8<QT>(f);
       if (!in) o = make_uint4(0, 0, 0, 0);   // a padded row (of the queries: none goes to the cache)
-      *reinterpret_cast<uint4*>(dst + 16 * c) = o;
+      st16(dst + 16 * c, o, p.nt_store);
     }
   }
 }
@@ -410,9 +465,10 @@ __global__ void __launch_bounds__(kRopeThreads, NI <= 5 ? 3 : 2) sas_rope_grad_k
     uint32_t wl = lds_addr_of(lds);
     asm volatile("" : "+v"(wl));
     // x of normed channels alone is needed: the others' lines are not fetched
-    r.load_normed(a.x + (long long)t * a.st + (long long)h * a.sh);
+    const uint8_t* x = a.x + (long long)t * a.st + (long long)h * a.sh;
     const uint8_t* dy = a.dy + (long long)t * a.dst + (long long)h * a.dsh;
-    g.load(dy);
+    either(p.nt_load, [&] { r.template load_normed<true>(x); g.template load<true>(dy); },
+           [&] { r.template load_normed<false>(x); g.template load<false>(dy); });
     const bool in = live && (!p.R || (pos >= 0 && pos < p.table_rows));
     const float* cs = p.table + (size_t)(in ? pos : 0) * p.R;
     // u = dy rotated back, of iteration i
@@ -420,13 +476,14 @@ __global__ void __launch_bounds__(kRopeThreads, NI <= 5 ? 3 : 2) sas_rope_grad_k
       unpack8<QT>(g.v[i], u);
       if (p.R && r.turns(i)) {
         const int c = r.chunk(i);
-        const bool turn = c >= r.rc0 && c < r.nch;
-        const int ct = turn ? c : r.rc0;
+        Turn<QT, HALF> e;
+        e.load(r, cs, dy, c);
+        e.ready();
         float other[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, o[8];
-        if constexpr (HALF) unpack8<QT>(r.ld(dy, r.partner(ct)), other);
-        r.rotate(p, cs, ct, u, other, -p.sign, o);
+        if constexpr (HALF) unpack8<QT>(e.other, other);
+        e.turn(u, other, -p.sign, o);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) u[k] = turn ? (in ? o[k] : 0.f) : u[k];
+        for (int k = 0; k < 8; ++k) u[k] = c >= r.rc0 && c < r.nch ? (in ? o[k] : 0.f) : u[k];
       }
     };
     // the rotated channels of the builds with one such iteration are kept, the
@@ -498,7 +555,7 @@ __global__ void __launch_bounds__(kRopeThreads, NI <= 5 ? 3 : 2) sas_rope_grad_k
         if constexpr (W) dw[i][k] = fmaf(u[k], f[k] * rinv, dw[i][k]);   // (past n: never read)
       }
       const uint4 v = pack8<QT>(o);
-      if (live && r.has(i)) *reinterpret_cast<uint4*>(dst + 16 * kLanes * i) = v;
+      if (live && r.has(i)) st16(dst + 16 * kLanes * i, v, p.nt_store);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -551,6 +608,8 @@ __global__ void __launch_bounds__(kSumThreads) sas_rope_dw_kernel(const RopeSum 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+
+constexpr double kInfinityCache = 256e6;
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -608,6 +667,16 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
     q.st = a->q_stride_t * 2; q.sh = a->q_stride_h * 2; q.rows = (uint32_t)(a->T * a->H);
   }
   for (RopePart& x : p->part) x.blocks = (int)((x.rows + kRopeRows - 1) / kRopeRows);
+  // Rows that with the output outgrow the 256 MB Infinity Cache are read past the
+  // caches, and an output of twice its size written so. us a call without, with
+  // the loads, with both, and of call and attention over its output, 64 heads of 512
+  // channels: 2048 tokens 42 / 43 / 45, 103 / 103 / 113; 4096 94 / 80 / 88, 217 / 206 /
+  // 215; 8192 187 / 181 / 173, 421 / 414 / 415. Smaller outputs are left for their
+  // reader: written past the caches, 43 -> 38 us alone for 5300 tokens of 16 heads, but
+  // call and attention of 2048 tokens 103 -> 115.
+  const double bytes = 2.0 * a->D * ((double)p->part[0].rows + p->part[1].rows);
+  p->nt_load = 2 * bytes >= kInfinityCache;
+  p->nt_store = bytes >= 2 * kInfinityCache;
 }
 
 // The kernel for a row width: 128, 512 or 576 channels with 64 rotated ones (or none) in
@@ -670,6 +739,10 @@ int check_grad(const SasNormRopeBwdArgs* a, RopeParams* p) {
     return set_error(SAS_EINVAL, "norm_rope_bwd: a weight gradient needs its weight");
   fill_rope(f, p);
   grad_blocks(p);
+  // us without, with loads, with both, 64 heads of 512 channels: 1024 tokens 37 / 38 /
+  // 36; 2048 80 / 68 / 67; 4096 153 / 148 / 129; 8192 304 / 294 / 285
+  const double bytes = 2.0 * f->D * ((double)p->part[0].rows + p->part[1].rows);
+  p->nt_load = p->nt_store = 3 * bytes >= kInfinityCache;
   return SAS_OK;
 }
 
