@@ -136,9 +136,11 @@ def write_kv_cache(kv: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
         _lib.check(rc, "write_kv_cache")
 
 
-# what SasCacheAppendArgs puts behind its rope arguments
-_APPEND = struct.Struct("@8Q7q6ifi4Q4q2i")
-assert _APPEND.size == C.sizeof(_lib.SasCacheAppendArgs)
+# what SasCacheAppendArgs puts behind its rope arguments: four pointers, then what
+# follows from the geometry
+_APPEND_PTRS = struct.Struct("@4Q")
+_APPEND_DIMS = struct.Struct("@4q2i")
+assert C.sizeof(_lib.SasNormRopeArgs) + _APPEND_PTRS.size + _APPEND_DIMS.size == C.sizeof(_lib.SasCacheAppendArgs)
 
 
 def append_kv_cache(
@@ -179,6 +181,19 @@ def append_kv_cache(
     :func:`write_kv_cache`. The rows of one call must go to distinct cache rows. No
     host sync.
     """
+    key = (rope._signature(2, q, kv, positions, table, q_norm_dim, q_weight, norm_dim, weight, eps, interleaved, False),
+           cache.shape, cache.dtype, cache.get_device(), cache.is_contiguous(),
+           block_table.shape, block_table.dtype, block_table.get_device(), block_table.is_contiguous(),
+           cu_seqlens_q.shape, cu_seqlens_q.dtype, cu_seqlens_q.get_device(), cu_seqlens_q.is_contiguous(),
+           seqused_kv.shape, seqused_kv.dtype, seqused_kv.get_device(), seqused_kv.is_contiguous())
+    b = rope._sigs.get(key)
+    if b is not None and rope._aligned(q, kv, table, q_weight, weight):
+        out = None if q is None else rope._out(q, b.q_like)
+        packed = rope._pack_ptrs(q, kv, q_weight, weight, positions, table, out, None)
+        rope._launch("sas_cache_append_v1", packed + b.dims + _APPEND_PTRS.pack(
+            cu_seqlens_q.data_ptr(), seqused_kv.data_ptr(), block_table.data_ptr(), cache.data_ptr()) + b.extra, b.dev,
+            "append_kv_cache")
+        return out
     if kv.dim() != 2 or (q is not None and (q.dim() != 3 or q.shape[0] != kv.shape[0] or q.shape[2] != kv.shape[1])):
         raise ValueError(f"kv must be [T, D] and q [T, H, D], got {tuple(kv.shape)}"
                          + ("" if q is None else f" and {tuple(q.shape)}"))
@@ -202,9 +217,11 @@ def append_kv_cache(
         if t.device != dev:
             raise ValueError("all tensors must be on kv's device")
     bt, cu, used = _i32(block_table), _i32(cu_seqlens_q), _i32(seqused_kv)
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
-    rope._launch("sas_cache_append_v1", _APPEND.pack(
-        *b.pack(0 if out is None else out.data_ptr(), 0), cu.data_ptr(), used.data_ptr(), bt.data_ptr(), cache.data_ptr(),
-        B, bt.shape[1], cache.shape[1], cache.shape[0],
-        _lib.SAS_DT_FP8_E4M3_ROW656 if fp8 else _DT[kv.dtype], 0), dev, "append_kv_cache")
+    out = None if q is None else rope._out(q, b.q_like)
+    b.extra = _APPEND_DIMS.pack(B, bt.shape[1], cache.shape[1], cache.shape[0],
+                                _lib.SAS_DT_FP8_E4M3_ROW656 if fp8 else _DT[kv.dtype], 0)
+    if bt is block_table and cu is cu_seqlens_q and used is seqused_kv:
+        rope._keep(key, b, q, kv, positions, table, q_weight, weight)
+    rope._launch("sas_cache_append_v1", b.ptrs(out, None) + b.dims + _APPEND_PTRS.pack(
+        cu.data_ptr(), used.data_ptr(), bt.data_ptr(), cache.data_ptr()) + b.extra, dev, "append_kv_cache")
     return out

@@ -387,12 +387,22 @@ struct Tok {
 // token first; all head groups and splits of a token go to one XCD and share its
 // L2. Every XCD then gets the same mix of long and short token rows (causal
 // prefill: rows grow with the position), and the longest items start first.
+// A draft tree's nodes stay together instead: each XCD takes a contiguous share of
+// the tokens, whose window rows, and the compressed rows that siblings have in
+// common, it then fetches once.
+__device__ __forceinline__ int token_index(const FwdParams& p, int x, int q) {
+  if (p.tree) {
+    const int t0 = (int)((long long)x * p.T / p.nxcd), t1 = (int)((long long)(x + 1) * p.T / p.nxcd);
+    return t0 + q < t1 ? t0 + q : -1;
+  }
+  return p.T - 1 - (q * p.nxcd + x);
+}
 __device__ __forceinline__ int item_index(const FwdParams& p) {
   const unsigned nx = (unsigned)p.nxcd;
   const int x = (int)(blockIdx.x % nx), l = (int)(blockIdx.x / nx);
   const int per_tok = p.nhg * p.nsplit;
   const int q = l / per_tok, sub = l - q * per_tok;
-  const int t = p.T - 1 - (q * p.nxcd + x);
+  const int t = token_index(p, x, q);
   return t >= 0 ? t * per_tok + sub : -1;
 }
 

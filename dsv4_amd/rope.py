@@ -20,13 +20,18 @@ from . import _lib
 _DT = {torch.bfloat16: _lib.SAS_DT_BF16, torch.float16: _lib.SAS_DT_FP16}
 _raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
-# SasNormRopeArgs as packed bytes (eight pointers, seven int64, six int32, eps,
-# reserved) and what the backward and the append put behind them: filling ctypes
-# structures field by field took a third of a small call
-_ARGS = struct.Struct("@8Q7q6ifi")
-_GRAD = struct.Struct("@8Q7q6ifi7QQ3q")
-assert _ARGS.size == C.sizeof(_lib.SasNormRopeArgs) and _GRAD.size == C.sizeof(_lib.SasNormRopeBwdArgs)
+# SasNormRopeArgs as packed bytes: eight pointers, then what follows from a call's
+# geometry (seven int64, six int32, eps, reserved), kept per signature; the
+# backward and the append put theirs behind it. (ctypes structures filled field by
+# field, and every check made anew, took a small call 12.5 us of host time, 7.5 now.)
+_PTRS = struct.Struct("@8Q")
+_DIMS = struct.Struct("@7q6ifi")
+_GRAD_PTRS = struct.Struct("@6QQQ")
+_GRAD_STRIDES = struct.Struct("@3q")
+assert _PTRS.size + _DIMS.size == C.sizeof(_lib.SasNormRopeArgs)
+assert _PTRS.size + _DIMS.size + _GRAD_PTRS.size + _GRAD_STRIDES.size == C.sizeof(_lib.SasNormRopeBwdArgs)
 _raw_fns = {}
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _bytes_fn(name: str):
@@ -42,9 +47,10 @@ def _bytes_fn(name: str):
 
 def _launch(name: str, packed: bytes, dev: torch.device, what: str) -> None:
     """Queue a launch on ``dev``'s current stream."""
-    f = _bytes_fn(name)
-    stream = torch.cuda.current_stream(dev).cuda_stream if _raw is None else _raw(dev.index)
-    if dev.index == torch.cuda.current_device():
+    f = _raw_fns.get(name) or _bytes_fn(name)
+    index = dev.index
+    stream = torch.cuda.current_stream(dev).cuda_stream if _raw is None else _raw(index)
+    if index == _device():
         rc = f(packed, stream)
     else:
         with torch.cuda.device(dev):
@@ -117,17 +123,63 @@ def _table(table: Optional[torch.Tensor], positions: Optional[torch.Tensor], x: 
 
 
 class _Bound:
-    """Checked arguments of one call, in SasNormRopeArgs' order but for the
-    outputs, and the tensors they point into."""
+    """Checked arguments of one call: the tensors as the kernels take them, and
+    what follows from their geometry, packed behind the pointers (``dims``)."""
 
-    __slots__ = ("q", "kv", "qw", "kw", "table", "pos", "dims", "tail", "dev", "lead")
+    __slots__ = ("q", "kv", "qw", "kw", "table", "pos", "dims", "dev", "lead", "q_like", "kv_like", "extra")
 
-    def pack(self, q_out: int, kv_out: int) -> tuple:
-        q, kv = self.q, self.kv
-        return (0 if q is None else q.data_ptr(), 0 if kv is None else kv.data_ptr(),
-                0 if self.qw is None else self.qw.data_ptr(), 0 if self.kw is None else self.kw.data_ptr(),
-                0 if self.pos is None else self.pos.data_ptr(), 0 if self.table is None else self.table.data_ptr(),
-                q_out, kv_out) + self.dims + self.tail
+    def ptrs(self, q_out, kv_out) -> bytes:
+        return _pack_ptrs(self.q, self.kv, self.qw, self.kw, self.pos, self.table, q_out, kv_out)
+
+
+def _pack_ptrs(q, kv, qw, kw, pos, table, q_out, kv_out) -> bytes:
+    return _PTRS.pack(0 if q is None else q.data_ptr(), 0 if kv is None else kv.data_ptr(),
+                      0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(),
+                      0 if pos is None else pos.data_ptr(), 0 if table is None else table.data_ptr(),
+                      0 if q_out is None else q_out.data_ptr(), 0 if kv_out is None else kv_out.data_ptr())
+
+
+# Resolutions of the signatures seen (geometry, types and scalars alone: no address, no
+# tensor), of calls whose tensors are taken as given; dropped together when full.
+_SIGS_MAX = 256
+_sigs = {}
+
+
+def _signature(what, q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse):
+    return (what, None if q is None else (q.shape, q.stride(), q.dtype, q.get_device()),
+            None if kv is None else (kv.shape, kv.stride(), kv.dtype, kv.get_device()),
+            None if positions is None else (positions.shape, positions.dtype, positions.is_contiguous(), positions.get_device()),
+            None if table is None else (table.shape, table.dtype, table.is_contiguous(), table.get_device()),
+            q_norm_dim, kv_norm_dim,
+            None if q_weight is None else (q_weight.shape, q_weight.dtype, q_weight.stride(), q_weight.get_device()),
+            None if kv_weight is None else (kv_weight.shape, kv_weight.dtype, kv_weight.stride(), kv_weight.get_device()),
+            eps, interleaved, inverse)
+
+
+def _aligned(*tensors) -> bool:
+    a = 0
+    for t in tensors:
+        if t is not None:
+            a |= t.data_ptr()
+    return not a & 15
+
+
+def _keep(key, b: _Bound, q, kv, positions, table, q_weight, kv_weight) -> None:
+    """Keep what a call's geometry gives, where its tensors were taken as given."""
+    if (b.q is not q or b.kv is not kv or b.table is not table or (b.pos is not positions and table is not None)
+            or b.qw is not q_weight or b.kw is not kv_weight):
+        return
+    if len(_sigs) >= _SIGS_MAX:
+        _sigs.clear()
+    kept = _Bound()
+    kept.q = kept.kv = kept.qw = kept.kw = kept.table = kept.pos = None
+    kept.dims, kept.dev, kept.lead, kept.q_like, kept.kv_like, kept.extra = b.dims, b.dev, b.lead, b.q_like, b.kv_like, b.extra
+    _sigs[key] = kept
+
+
+def _out(t: torch.Tensor, like: bool) -> torch.Tensor:
+    """A new contiguous tensor of t's geometry."""
+    return torch.empty_like(t) if like else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse,
@@ -180,9 +232,11 @@ def _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight,
     b.table, table_rows, R, b.pos = _table(table, positions, x, need_positions)
     if b.pos is not None and b.pos.shape != lead:
         raise ValueError(f"positions must be {lead}, got {tuple(b.pos.shape)}")
-    b.dims = (T, H, D, qt, qh, kt, table_rows)
-    b.tail = (R, qn, kn, _DT[x.dtype], _lib.SAS_DT_FP32 if wf32 else _DT[x.dtype],
-              (0 if interleaved else _lib.SAS_ROPE_HALF) | (_lib.SAS_ROPE_INVERSE if inverse else 0), float(eps), 0)
+    b.q_like, b.kv_like = q is not None and q.is_contiguous(), kv is not None and kv.is_contiguous()
+    b.extra = None
+    b.dims = _DIMS.pack(T, H, D, qt, qh, kt, table_rows, R, qn, kn, _DT[x.dtype],
+                        _lib.SAS_DT_FP32 if wf32 else _DT[x.dtype],
+                        (0 if interleaved else _lib.SAS_ROPE_HALF) | (_lib.SAS_ROPE_INVERSE if inverse else 0), float(eps), 0)
     return b
 
 
@@ -219,11 +273,19 @@ def norm_rope(
     copied first. Returns contiguous ``q_out``, or ``(q_out, kv_out)`` where ``kv`` is
     given (``kv_out`` alone without ``q``).
     """
-    b = _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse)
-    qo = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=b.dev)
-    ko = None if kv is None else torch.empty(kv.shape, dtype=kv.dtype, device=b.dev)
-    _launch("sas_norm_rope_v1", _ARGS.pack(*b.pack(0 if qo is None else qo.data_ptr(), 0 if ko is None else ko.data_ptr())),
-            b.dev, "norm_rope")
+    key = _signature(0, q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse)
+    b = _sigs.get(key)
+    if b is not None and _aligned(q, kv, table, q_weight, kv_weight):
+        qo = None if q is None else _out(q, b.q_like)
+        ko = None if kv is None else _out(kv, b.kv_like)
+        packed = _pack_ptrs(q, kv, q_weight, kv_weight, positions, table, qo, ko)
+    else:
+        b = _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse)
+        qo = None if q is None else _out(q, b.q_like)
+        ko = None if kv is None else _out(kv, b.kv_like)
+        packed = b.ptrs(qo, ko)
+        _keep(key, b, q, kv, positions, table, q_weight, kv_weight)
+    _launch("sas_norm_rope_v1", packed + b.dims, b.dev, "norm_rope")
     return qo if kv is None else ko if q is None else (qo, ko)
 
 
@@ -238,7 +300,7 @@ def _grad_rows(name: str, g: Optional[torch.Tensor], x: Optional[torch.Tensor], 
 _plan = None
 
 
-def _workspace_bytes(args) -> int:
+def _workspace_bytes(packed: bytes) -> int:
     """What sas_norm_rope_bwd_plan reports for packed arguments."""
     global _plan
     if _plan is None:
@@ -247,7 +309,7 @@ def _workspace_bytes(args) -> int:
         f.restype = C.c_int
         _plan = f
     n = C.c_size_t(0)
-    _lib.check(_plan(_GRAD.pack(*args), C.byref(n)), "norm_rope_backward")
+    _lib.check(_plan(packed, C.byref(n)), "norm_rope_backward")
     return n.value
 
 
@@ -272,25 +334,39 @@ def norm_rope_backward(
     dq_weight, dkv_weight)``, None for what was not given; weight gradients in
     their weights' dtype, summed in fp32 over tokens and heads in a fixed order
     (the same call gives the same bits)."""
-    b = _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse)
-    gq, gk = _grad_rows("dq_out", dq_out, q, 3), _grad_rows("dkv_out", dkv_out, kv, 2)
-    dq = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=b.dev)
-    dkv = None if kv is None else torch.empty(kv.shape, dtype=kv.dtype, device=b.dev)
-    dqw = None if b.qw is None else torch.empty(b.qw.shape, dtype=torch.float32, device=b.dev)
-    dkw = None if b.kw is None else torch.empty(b.kw.shape, dtype=torch.float32, device=b.dev)
+    key = (_signature(1, q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse),
+           None if dq_out is None else (dq_out.shape, dq_out.stride(), dq_out.dtype, dq_out.get_device()),
+           None if dkv_out is None else (dkv_out.shape, dkv_out.stride(), dkv_out.dtype, dkv_out.get_device()))
+    b = _sigs.get(key)
+    hit = b is not None and _aligned(q, kv, table, q_weight, kv_weight, dq_out, dkv_out)
+    if hit:
+        gq, gk, qw, kw = dq_out, dkv_out, q_weight, kv_weight
+        strides, need = b.extra
+    else:
+        b = _bind(q, kv, positions, table, q_norm_dim, q_weight, kv_norm_dim, kv_weight, eps, interleaved, inverse)
+        gq, gk = _grad_rows("dq_out", dq_out, q, 3), _grad_rows("dkv_out", dkv_out, kv, 2)
+        qw, kw = b.qw, b.kw
+        strides = _GRAD_STRIDES.pack(0 if gq is None else gq.stride(0), 0 if gq is None else gq.stride(1),
+                                     0 if gk is None else gk.stride(0))
+    dq = None if q is None else _out(q, b.q_like)
+    dkv = None if kv is None else _out(kv, b.kv_like)
+    dqw = None if qw is None else torch.empty_like(qw, dtype=torch.float32)
+    dkw = None if kw is None else torch.empty_like(kw, dtype=torch.float32)
 
     def p(t):
         return 0 if t is None else t.data_ptr()
 
-    args = b.pack(0, 0) + (p(gq), p(gk), p(dq), p(dkv), p(dqw), p(dkw))
-    strides = (0 if gq is None else gq.stride(0), 0 if gq is None else gq.stride(1), 0 if gk is None else gk.stride(0))
+    grads = (p(gq), p(gk), p(dq), p(dkv), p(dqw), p(dkw))
+    head = (_pack_ptrs(q, kv, qw, kw, positions, table, None, None) if hit else b.ptrs(None, None)) + b.dims
+    if not hit:
+        need = _workspace_bytes(head + _GRAD_PTRS.pack(*grads, 0, 0) + strides)
+        b.extra = strides, need
+        if gq is dq_out and gk is dkv_out:
+            _keep(key, b, q, kv, positions, table, q_weight, kv_weight)
     # the partial sums of the weights' gradients, from the caching allocator: under
     # capture from the graph's own pool
-    ws = None
-    need = _workspace_bytes(args + (0, 0) + strides) if dqw is not None or dkw is not None else 0
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=b.dev)
-    _launch("sas_norm_rope_bwd_v1", _GRAD.pack(*args, p(ws), need, *strides), b.dev, "norm_rope_backward")
+    ws = torch.empty(need, dtype=torch.uint8, device=b.dev) if need else None
+    _launch("sas_norm_rope_bwd_v1", head + _GRAD_PTRS.pack(*grads, p(ws), need) + strides, b.dev, "norm_rope_backward")
 
     def like(g, w):
         if w is None:
