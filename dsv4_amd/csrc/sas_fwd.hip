@@ -43,6 +43,9 @@
 
 #include <mutex>
 
+#ifndef SAS_FWD_TREE
+#define SAS_FWD_TREE 0   // 1 (sas_fwd_tree.hip): the same kernels over draft trees
+#endif
 #ifndef SAS_PFK
 #define SAS_PFK 3   // K operand k-steps read ahead (32-row steps)
 #endif
@@ -68,6 +71,8 @@
 
 namespace sas {
 namespace {
+
+constexpr bool kTree = SAS_FWD_TREE;
 
 // ---------------------------------------------------------------------------
 // forward kernel
@@ -1650,7 +1655,7 @@ sas_fwd_kernel(const FwdParams p) {
   // in scalar registers, the step loop's bounds and DMA guards become scalar
   // branches instead of exec-mask updates
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int item = item_index(p);
+  const int item = item_index<kTree>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
   Fwd<HW, NW, D, QT, KVF> f(p, lane, wave);
@@ -1665,7 +1670,7 @@ sas_fwd_kernel(const FwdParams p) {
   if constexpr (C::QL) {
     if (wave >= 4) f.q_dma(k, wave);
   }
-  resolve<256, C::ROWB>(p, k, tid, lane, wave, [&] {
+  resolve<256, C::ROWB, kTree>(p, k, tid, lane, wave, [&] {
     if constexpr (C::QL) return;
     const uint4* qp = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq) * D * 2);
 #pragma unroll
@@ -1875,11 +1880,11 @@ sas_dec_kernel(const FwdParams p) {
   // in scalar registers, the step loop's bounds and DMA guards become scalar
   // branches instead of exec-mask updates
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int item = item_index(p);
+  const int item = item_index<kTree>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
   C f(p, lane);
-  resolve<256, C::ROWB>(p, k, tid, lane, wave, [] {});
+  resolve<256, C::ROWB, kTree>(p, k, tid, lane, wave, [] {});
   const int nvalid = __builtin_amdgcn_readfirstlane(k.nvalid);
   const int hq = k.hg * 16 + f.c16;
   // key-group share of wave `wave`: whole 16-row steps, wave 0 first
@@ -1934,7 +1939,7 @@ sas_combine_kernel(const FwdParams p) {
   // (measured: C2 call 24.3 -> 23.7 µs)
   const unsigned nx = (unsigned)p.nxcd;
   const int x = (int)(blockIdx.x % nx), l = (int)(blockIdx.x / nx);
-  const int t = token_index(p, x, l / nhb);
+  const int t = token_index<kTree>(p, x, l / nhb);
   if (t < 0) return;
   const int h0 = (l % nhb) * kHeads;
   merge_partials<QT>(p, t, h0, min(kHeads, p.H - h0), threadIdx.x, kCombineThreads);
@@ -2214,21 +2219,7 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
   return launch_combine(fp, a->out_dtype, st);
 }
 
-}  // namespace
-
-extern "C" int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* workspace_bytes) {
-  sas::clear_error();
-  Plan pl;
-  const int rc = make_plan(a, &pl);
-  if (rc) return rc;
-  if (num_splits) *num_splits = pl.nsplit;
-  if (workspace_bytes) *workspace_bytes = pl.ws;
-  return SAS_OK;
-}
-
-namespace {
-
-// sas_fwd_v1, or with tree_mask sas_fwd_tree_v1
+// sas_fwd_v1, or (kTree) sas_fwd_tree_v1
 int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, void* stream) {
   Plan pl;
   int rc = make_plan(a, &pl);
@@ -2301,11 +2292,12 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
   fp.tree_words = tree_words;
   hipStream_t st = (hipStream_t)stream;
 
-  // (runs of tokens are chains)
-  if (const int run = tree_mask ? 0 : win_run(a, pl)) return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
-  if (const int run = tree_mask ? 0 : dense_run(a, pl)) {
-    fp.nhg = (int)a->H / 64;
-    return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
+  if constexpr (!kTree) {   // (runs of tokens are chains)
+    if (const int run = win_run(a, pl)) return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
+    if (const int run = dense_run(a, pl)) {
+      fp.nhg = (int)a->H / 64;
+      return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
+    }
   }
   if (fp8) rc = dispatch_hw<576, __bf16, 1>(pl.hw, pl.nw, pl.exact, fp, nblocks, st);
   else if (a->q_dtype == SAS_DT_BF16)
@@ -2320,10 +2312,7 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
 
 }  // namespace
 
-extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
-  sas::clear_error();
-  return fwd_impl(a, nullptr, 0, stream);
-}
+#if SAS_FWD_TREE
 
 extern "C" int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream) {
   sas::clear_error();
@@ -2333,6 +2322,23 @@ extern "C" int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream) {
   if (a->fwd.T > 0 && (!a->tree_mask || (uintptr_t)a->tree_mask % 8))
     return sas::set_error(SAS_EINVAL, "tree_mask must be an 8-byte aligned device pointer");
   return fwd_impl(&a->fwd, a->tree_mask, (int)a->tree_words, stream);
+}
+
+#else
+
+extern "C" int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* workspace_bytes) {
+  sas::clear_error();
+  Plan pl;
+  const int rc = make_plan(a, &pl);
+  if (rc) return rc;
+  if (num_splits) *num_splits = pl.nsplit;
+  if (workspace_bytes) *workspace_bytes = pl.ws;
+  return SAS_OK;
+}
+
+extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
+  sas::clear_error();
+  return fwd_impl(a, nullptr, 0, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -2411,5 +2417,7 @@ extern "C" int sas_combine_v1(const SasCombineArgs* a, void* stream) {
   sas::clear_error();
   return combine_impl(a, (hipStream_t)stream);
 }
+
+#endif  // SAS_FWD_TREE
 
 }  // namespace sas

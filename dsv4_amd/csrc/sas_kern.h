@@ -130,7 +130,7 @@ struct FwdParams {
   int nxcd;      // XCDs the grid is dealt over (device_xcds())
   int part_nt;   // 1: split partials go out with non-temporal stores
   int out_nt;    // 1: the output (one split) goes out with non-temporal stores
-  const uint64_t* tree;   // draft trees: [T, tree_words] attended slots of the token's sequence, or NULL
+  const uint64_t* tree;   // draft trees: [T, tree_words] attended slots of the token's sequence
   int tree_words;         // 64-slot words a token, at most 64
 };
 
@@ -390,19 +390,21 @@ struct Tok {
 // A draft tree's nodes stay together instead: each XCD takes a contiguous share of
 // the tokens, whose window rows, and the compressed rows that siblings have in
 // common, it then fetches once.
+template <bool TREE>
 __device__ __forceinline__ int token_index(const FwdParams& p, int x, int q) {
-  if (p.tree) {
+  if constexpr (TREE) {
     const int t0 = (int)((long long)x * p.T / p.nxcd), t1 = (int)((long long)(x + 1) * p.T / p.nxcd);
     return t0 + q < t1 ? t0 + q : -1;
   }
   return p.T - 1 - (q * p.nxcd + x);
 }
+template <bool TREE = false>
 __device__ __forceinline__ int item_index(const FwdParams& p) {
   const unsigned nx = (unsigned)p.nxcd;
   const int x = (int)(blockIdx.x % nx), l = (int)(blockIdx.x / nx);
   const int per_tok = p.nhg * p.nsplit;
   const int q = l / per_tok, sub = l - q * per_tok;
-  const int t = token_index(p, x, q);
+  const int t = token_index<TREE>(p, x, q);
   return t >= 0 ? t * per_tok + sub : -1;
 }
 
@@ -436,7 +438,9 @@ __device__ __forceinline__ int nth_bit(uint64_t m, int k) {
 struct Tree {
   uint64_t word;   // this lane's
   int count;       // set bits of all words
-  __device__ __forceinline__ Tree(uint64_t w, int lane, int first, int end) : word(w) {
+  // valid slots: [first, end)
+  __device__ __forceinline__ void mask(uint64_t w, int lane, int first, int end) {
+    word = w;
     const int lo = first - 64 * lane, hi = end - 64 * lane;   // this word's valid bits: [lo, hi)
     if (lo > 0) word = lo < 64 ? word >> lo << lo : 0;
     if (hi < 64) word = hi > 0 ? word & ((1ull << hi) - 1ull) : 0;
@@ -473,7 +477,7 @@ struct Tree {
 // (4K prefill 580 -> 573 µs with 4 resolving waves). `mid` runs after the
 // block-table loads are issued (a caller can put its own loads behind them
 // there).
-template <int NT, int ROWB, typename Mid>
+template <int NT, int ROWB, bool TREE = false, typename Mid>
 __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int lane, int wave, Mid&& mid) {
   constexpr int NWV = NT / 64;
   constexpr int kRounds = (kMaxSlots + NT - 1) / NT;
@@ -504,7 +508,7 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
     // the difference of two entries (loaded in the same round trip)
     const bool cu = p.act_q == nullptr;
     uint64_t tree_word = 0;
-    if (p.tree && lane < p.tree_words) tree_word = p.tree[(size_t)t * p.tree_words + lane];
+    if (TREE && lane < p.tree_words) tree_word = p.tree[(size_t)t * p.tree_words + lane];
     int qp0 = INT_MAX, aq0 = 0, akv0 = 0;
     if (lane < p.B) { qp0 = p.q_prefix[lane]; aq0 = cu ? p.q_prefix[lane + 1] : p.act_q[lane]; akv0 = p.act_kv[lane]; }
     // token -> (batch, position): largest b with q_prefix[b] <= t (q_prefix is
@@ -529,8 +533,9 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
     // causal position. Of a draft tree's node: its depth below the rows before
     // the drafts (its set bits, itself among them, come last), and the window
     // takes its `path` nearest drafts, then the rows before the drafts.
-    const Tree tree(tree_word, lane, aq - akv, p.tree ? aq : 0);
-    const int sg = p.tree ? max(akv - aq, 0) + tree.count - 1 : akv - aq + spos;
+    Tree tree{0, 0};
+    if constexpr (TREE) tree.mask(tree_word, lane, aq - akv, aq);
+    const int sg = TREE ? max(akv - aq, 0) + tree.count - 1 : akv - aq + spos;
     const int nwin = (padded || sg < 0) ? 0 : min(sg, p.win_left) + 1;
     const int wlo = sg - nwin + 1;                               // = max(sg - win_left, 0)
     const int thr = (padded || sg + 1 <= 0) ? 0 : (sg + 1) / p.cmp_ratio;
@@ -552,10 +557,10 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
       const int j = s0 + r * NT + tid;
       const bool live = j < s1 && !padded;
       int draft = 0;   // its slot, for window slots from nwin - path on
-      if (p.tree && s0 + r * NT < wincap) draft = tree.slot(tree.count - nwin + j);   // wave-uniform
+      if (TREE && s0 + r * NT < wincap) draft = tree.slot(tree.count - nwin + j);   // wave-uniform
       int blk;
       if (j < wincap) {
-        const int pos = p.tree && j >= nwin - path ? max(akv - aq + draft, 0) : wlo + j;
+        const int pos = TREE && j >= nwin - path ? max(akv - aq + draft, 0) : wlo + j;
         blk = pos / p.ori_bs;
         off[r] = pos - blk * p.ori_bs;
         ok[r] = live && j < nwin && blk < p.ori_bt_stride;
