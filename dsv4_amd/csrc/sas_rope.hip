@@ -43,7 +43,8 @@ struct RopePart {
 
 struct RopeParams {
   RopePart part[2];            // KV rows, queries
-  const int32_t* pos;          // [T] or null (append: the cache positions)
+  const int32_t* pos;          // [T]; any readable address where there are none
+  int has_pos;                 // 0: none (append: the cache positions)
   const float* table;          // [table_rows, R / 2, 2]
   int table_rows, D, R, T;
   int wf32;                    // weights are fp32 (else the rows' type)
@@ -55,6 +56,7 @@ struct RopeParams {
   const int32_t* bt;
   uint8_t* cache;
   int B, bt_stride, bs, nblocks;
+  int bs_shift;                // log2 of bs, or -1
 };
 
 template <int CTRL>
@@ -118,27 +120,30 @@ template <typename QT>
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack2<QT>(f[0], f[1]), pack2<QT>(f[2], f[3]), pack2<QT>(f[4], f[5]), pack2<QT>(f[6], f[7]));
 }
-// The part's weights as fp32 in LDS, ones past them (and where there are none, if
-// the caller asks for a part without): a workgroup's rows share them, in global
-// memory each wave would fetch its chunks' anew, in two types. `get` issues the
-// loads, `put` writes them behind the caller's own loads.
+// The part's weights as fp32 in LDS, ones past them and where there are none: a
+// workgroup's rows share them, in global memory each wave would fetch its chunks'
+// anew, in two types. `get` issues the loads (whole dwords, whatever the type: a load
+// under a branch waits for itself there), `put` writes them behind the caller's own.
 template <typename QT, int NI>
 struct Weights {
   static constexpr int kAll = NI * kLanes * 8, N = (kAll + kRopeThreads - 1) / kRopeThreads;
-  float w[N];
+  uint32_t w[N];
   __device__ __forceinline__ void get(const RopeParams& p, const RopePart& a, int tid) {
+    const uint64_t base = reinterpret_cast<uint64_t>(a.w);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int j = tid + k * kRopeThreads;
-      w[k] = 1.f;
-      if (a.w && j < a.n) w[k] = p.wf32 ? reinterpret_cast<const float*>(a.w)[j] : (float)reinterpret_cast<const QT*>(a.w)[j];
+      const int j = min(tid + k * kRopeThreads, max(a.n, 1) - 1);
+      w[k] = *reinterpret_cast<const SAS_GLOBAL uint32_t*>(base + (p.wf32 ? 4u * (uint32_t)j : 2u * (uint32_t)(j & ~1)));
     }
   }
-  __device__ __forceinline__ void put(float* lds, int tid) const {
+  __device__ __forceinline__ void put(const RopeParams& p, const RopePart& a, float* lds, int tid) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int j = tid + k * kRopeThreads;
-      if (kAll % kRopeThreads == 0 || j < kAll) lds[j] = w[k];
+      if (a.w) asm volatile("" : "+v"(w[k]));
+      const uint16_t h = (uint16_t)(j & 1 ? w[k] >> 16 : w[k]);
+      const float f = p.wf32 ? __uint_as_float(w[k]) : (float)__builtin_bit_cast(QT, h);
+      if (kAll % kRopeThreads == 0 || j < kAll) lds[j] = a.w && j < a.n ? f : 1.f;
     }
     asm volatile("" ::: "memory");
     lds_barrier();
@@ -158,26 +163,30 @@ __device__ __forceinline__ void weights8(uint32_t lds, int c, float (&f)[8]) {
 // `seq` holds the lane's own sequence of the first 64, loaded ahead of the row.
 struct Seq { int q0, q1, kv; };
 __device__ __forceinline__ Seq seq_of(const RopeParams& p, int i) {
-  return i < p.B ? Seq{p.cu[i], p.cu[i + 1], p.used[i]} : Seq{INT_MAX, 0, 0};
+  const int j = min(i, p.B - 1);
+  const Seq s{p.cu[j], p.cu[j + 1], p.used[j]};
+  return {i < p.B ? s.q0 : INT_MAX, s.q1, s.kv};
 }
 struct Place { int slot, b; bool padded; };
 __device__ __forceinline__ Place place_of(const RopeParams& p, Seq seq, int t, int lane) {
   Place o{0, 0, true};
   int len = 0, start = 0;
-  for (int c0 = 0;;) {
+  auto among = [&](const Seq& s, int c0) {   // whether a row's sequence may lie past these 64
     int n = 0;
 #pragma unroll
     for (int j = 0; j < kWaveRows; ++j) {
-      const int m = __popcll(__ballot(seq.q0 <= __builtin_amdgcn_readlane(t, kLanes * j)));
+      const int m = __popcll(__ballot(s.q0 <= __builtin_amdgcn_readlane(t, kLanes * j)));
       n = lane / kLanes == j ? m : n;
     }
     const int at = max(n - 1, 0);
-    const int s = __shfl(seq.q0, at), e = __shfl(seq.q1, at), u = __shfl(seq.kv, at);
-    if (n > 0) { o.b = c0 + at; start = s; len = e - s; o.slot = u - len + (t - s); o.padded = false; }
-    c0 += 64;
-    if (c0 >= p.B || __ballot(n == 64) == 0) break;   // wave-uniform: no row's sequence lies further on
-    seq = seq_of(p, c0 + lane);
-  }
+    const int q0 = __shfl(s.q0, at), q1 = __shfl(s.q1, at), kv = __shfl(s.kv, at);
+    if (n > 0) { o.b = c0 + at; start = q0; len = q1 - q0; o.slot = kv - len + (t - q0); o.padded = false; }
+    return __ballot(n == 64) != 0;
+  };
+  // (the first step apart: at the head of a loop the wait for `seq` would be for
+  // every load in flight)
+  bool more = among(seq, 0);
+  for (int c0 = 64; more && c0 < p.B; c0 += 64) more = among(seq_of(p, c0 + lane), c0);
   o.padded = o.padded || t < start || t - start >= len || o.slot < 0;
   return o;
 }
@@ -188,7 +197,10 @@ struct Head { uint32_t t, h; };
 __device__ __forceinline__ Head head_of(uint32_t r0, uint32_t H, int lane, bool live) {
   const uint32_t t0 = r0 / H, h0 = r0 - t0 * H;
   uint32_t t = t0, h = h0 + lane / kLanes;
-  if (H >= (uint32_t)kWaveRows) {
+  if (H == 1) {
+    t += h;
+    h = 0;
+  } else if (H >= (uint32_t)kWaveRows) {
     if (h >= H) { h -= H; ++t; }
   } else {
     const uint32_t k = h / H;
@@ -285,31 +297,34 @@ struct Turn {
 // type, 656-byte fp8 rows of the paged cache.
 enum { kToRows = 0, kToCache = 1, kToFp8 = 2 };
 
-// 128 latent channels, one iteration of the row's lanes, share a scale
-__device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, const float (&x)[8], bool write) {
+// 128 latent channels x m, one iteration of the row's lanes, share a scale. (The
+// quotients by reciprocal: within an ulp of the true ones, which move a byte only
+// where its value lies that near a tie.)
+__device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, const float (&x)[8], float m, bool write) {
   float amax = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
-  amax = max16(amax);
-  const float scale = amax > 0.f ? amax / kFp8Max : 1.f;
+  amax = max16(amax * m);
+  const float scale = amax > 0.f ? amax * (1.f / kFp8Max) : 1.f;
   // (at most the largest float: zeros beside channels below 1e-36 stay zeros)
-  const float inv = amax > 0.f ? fminf(kFp8Max / amax, 3.402823466e38f) : 1.f;
-  uint32_t q[2];
+  const float inv = amax > 0.f ? fminf(kFp8Max * __builtin_amdgcn_rcpf(amax), 3.402823466e38f) : 1.f;
+  const float q = m * inv;
+  uint32_t w[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    auto cl = [&](float f) { return __builtin_amdgcn_fmed3f(f * inv, -kFp8Max, kFp8Max); };
+    auto cl = [&](float f) { return __builtin_amdgcn_fmed3f(f * q, -kFp8Max, kFp8Max); };
     int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j]), cl(x[4 * j + 1]), 0, false);
     t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j + 2]), cl(x[4 * j + 3]), t, true);
-    q[j] = (uint32_t)t;
+    w[j] = (uint32_t)t;
   }
   if (!write) return;
-  *reinterpret_cast<uint2*>(dst + 128 * g + 8 * sub) = make_uint2(q[0], q[1]);
+  *reinterpret_cast<uint2*>(dst + 128 * g + 8 * sub) = make_uint2(w[0], w[1]);
   if (sub == 0) *reinterpret_cast<float*>(dst + kFp8ScaleOff + 4 * g) = scale;
 }
 
 // Rows of one part: workgroup `blk` of its grid. `cached`: they go to the cache
 // (workgroup-uniform; DST says how).
-template <typename QT, int NI, bool LAST, bool HALF, int DST, bool APPEND>
+template <typename QT, int NI, bool LAST, bool HALF, int DST, bool APPEND, bool NT>
 __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a, uint32_t blk, int tid, float* lds,
                                           bool cached) {
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -320,25 +335,19 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
   const auto [t, h] = head_of(r0, a.H, lane, live);
   Row<QT, NI, LAST, HALF> r(p, a.n, lane);
   const uint8_t* x = a.x + (long long)t * a.st + (long long)h * a.sh;
-  // what positions and places hang on goes first, the row behind it
+  // Loads in the order of their chains, straight on (where paths with other loads in
+  // flight meet, the compiler waits for all of them): what positions and places
+  // hang on, the row, the weights; then the angles and the block, which come back
+  // while the weights go to LDS.
   Seq seq{};
   if constexpr (APPEND) seq = seq_of(p, lane);
-  int pos = 0;
-  const bool own = !APPEND || p.pos;   // positions are given
-  if (p.R && own) pos = p.pos[t];
-  if (a.w) {   // workgroup-uniform
-    Weights<QT, NI> w;
-    w.get(p, a, tid);
-    either(p.nt_load, [&] { r.template load<true>(x); }, [&] { r.template load<false>(x); });
-    w.put(lds, tid);
-  } else {
-    either(p.nt_load, [&] { r.template load<true>(x); }, [&] { r.template load<false>(x); });
-  }
-  if (w0 >= a.rows) return;
-
+  int pos = p.pos[p.has_pos ? t : 0];
+  r.template load<NT>(x);
+  Weights<QT, NI> w;
+  if (a.w) w.get(p, a, tid);   // workgroup-uniform
   Place at{0, 0, false};
   if constexpr (APPEND) at = place_of(p, seq, (int)t, lane);
-  if (!own) pos = at.slot;
+  if (!p.has_pos) pos = at.slot;
   const bool in = (!p.R || (pos >= 0 && pos < p.table_rows)) && !at.padded;
   const float* cs = p.table + (size_t)(in ? pos : 0) * p.R;
   Turn<QT, HALF> last;   // of iteration NI - 1
@@ -347,13 +356,15 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
   if (!cached) {
     if (live) dst = a.y + (size_t)row * p.D * 2;
   } else {
-    const int blkno = in ? at.slot / p.bs : 0;
+    const int blkno = !in ? 0 : p.bs_shift >= 0 ? at.slot >> p.bs_shift : at.slot / p.bs;
     const bool okt = in && blkno < p.bt_stride;
     const int phys = p.bt[okt ? (size_t)at.b * p.bt_stride + blkno : 0];
     if (live && okt && phys >= 0 && phys < p.nblocks)
       dst = p.cache + ((size_t)phys * p.bs + (at.slot - blkno * p.bs)) * (DST == kToFp8 ? kRow656 : p.D * 2);
   }
   const bool write = dst != nullptr;
+  if (a.w) w.put(p, a, lds, tid);
+  if (w0 >= a.rows) return;
 
   // the norm
   float rinv = 1.f;
@@ -369,23 +380,33 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
     }
     rinv = rsqrtf(sum16(ss) / (float)a.n + p.eps);
   }
-  auto normed = [&](const uint4& v, int c, float (&f)[8]) {
+  // x w, and the factor that is left
+  auto weighted = [&](const uint4& v, int c, float (&f)[8]) {
     unpack8<QT>(v, f);
-    const float s = c < r.nn ? rinv : 1.f;
     if (a.w) {
       float w[8];
       weights8(lds_addr_of(lds), c, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= s * w[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= s;
+      for (int k = 0; k < 8; ++k) f[k] *= w[k];
     }
+    return c < r.nn ? rinv : 1.f;
+  };
+  auto normed = [&](const uint4& v, int c, float (&f)[8]) {
+    const float s = weighted(v, c, f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] *= s;
   };
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     const int c = r.chunk(i);
     float f[8];
+    if constexpr (DST == kToFp8 && LAST) {
+      if (i < 4) {   // latent channels, none of them rotated
+        const float s = weighted(r.v[i], c, f);
+        put_fp8_group(dst, i, r.sub, f, s, write);
+        continue;
+      }
+    }
     normed(r.v[i], c, f);
     if (p.R && r.turns(i)) {
       Turn<QT, HALF> one;
@@ -399,7 +420,7 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
       for (int k = 0; k < 8; ++k) f[k] = c >= r.rc0 && c < r.nch ? o[k] : f[k];
     }
     if constexpr (DST == kToFp8) {
-      if (i < 4) put_fp8_group(dst, i, r.sub, f, write);
+      if (i < 4) put_fp8_group(dst, i, r.sub, f, 1.f, write);
       else if (write && r.sub < 8) *reinterpret_cast<uint4*>(dst + kFp8RopeOff + 16 * r.sub) = pack8<__bf16>(f);
     } else if (write && r.has(i)) {
       uint4 o = pack8<QT>(f);
@@ -411,7 +432,8 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
 
 // Workgroups [0, part[0].blocks) take the KV rows (the longer chain of loads
 // starts first), the others the queries.
-template <typename QT, int NI, bool LAST, bool HALF, int DST>
+// NT: the rows are read past the caches (appends never are)
+template <typename QT, int NI, bool LAST, bool HALF, int DST, bool NT>
 __global__ void __launch_bounds__(kRopeThreads) sas_rope_kernel(const RopeParams p) {
   constexpr bool kAppend = DST != kToRows;
   __shared__ __attribute__((aligned(16))) float lds[Weights<QT, NI>::kAll];
@@ -420,10 +442,10 @@ __global__ void __launch_bounds__(kRopeThreads) sas_rope_kernel(const RopeParams
   const RopePart& a = p.part[b < nkv ? 0 : 1];
   const uint32_t blk = b < nkv ? b : b - nkv;
   if constexpr (DST == kToFp8) {
-    if (b < nkv) rope_rows<QT, NI, LAST, HALF, kToFp8, true>(p, a, blk, threadIdx.x, lds, true);
-    else rope_rows<QT, NI, LAST, HALF, kToCache, true>(p, a, blk, threadIdx.x, lds, false);
+    if (b < nkv) rope_rows<QT, NI, LAST, HALF, kToFp8, true, NT>(p, a, blk, threadIdx.x, lds, true);
+    else rope_rows<QT, NI, LAST, HALF, kToCache, true, NT>(p, a, blk, threadIdx.x, lds, false);
   } else {
-    rope_rows<QT, NI, LAST, HALF, DST, kAppend>(p, a, blk, threadIdx.x, lds, kAppend && b < nkv);
+    rope_rows<QT, NI, LAST, HALF, DST, kAppend, NT>(p, a, blk, threadIdx.x, lds, kAppend && b < nkv);
   }
 }
 
@@ -445,22 +467,20 @@ __global__ void __launch_bounds__(kRopeThreads, NI <= 5 ? 3 : 2) sas_rope_grad_k
   const uint32_t nkv = (uint32_t)p.part[0].blocks;
   const RopePart& a = p.part[blockIdx.x < nkv ? 0 : 1];
   const uint32_t blk = blockIdx.x < nkv ? blockIdx.x : blockIdx.x - nkv;
-  {
-    Weights<QT, NI> w;   // ones where there are none
-    w.get(p, a, tid);
-    w.put(lds, tid);
-  }
+  Weights<QT, NI> w;   // ones where there are none
+  if (a.w) w.get(p, a, tid);
   float dw[W ? NI : 1][8];
 #pragma unroll
   for (int i = 0; i < (W ? NI : 1); ++i)
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = 0.f;
   Row<QT, NI, LAST, HALF> r(p, a.n, lane), g(p, a.n, lane);
+  w.put(p, a, lds, tid);
   for (uint32_t r0 = blk * kRopeRows + wave * kWaveRows; r0 < a.rows; r0 += (uint32_t)a.blocks * kRopeRows) {
     const uint32_t row = r0 + lane / kLanes;
     const bool live = row < a.rows;
     const auto [t, h] = head_of(r0, a.H, lane, live);
-    const int pos = p.R ? p.pos[t] : 0;
+    const int pos = p.pos[p.has_pos ? t : 0];
     // (kept out of registers: hoisted out of the loop the weights cost a wave a SIMD)
     uint32_t wl = lds_addr_of(lds);
     asm volatile("" : "+v"(wl));
@@ -645,7 +665,9 @@ int check_rope(const SasNormRopeArgs* a, const char* what) {
 }
 
 void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
-  p->pos = a->positions;
+  // (no rotation, or an append's own positions: an address that is read and ignored)
+  p->has_pos = a->positions != nullptr;
+  p->pos = a->positions ? a->positions : (const int32_t*)(a->kv ? a->kv : a->q);
   p->table = a->table;
   p->table_rows = (int)a->table_rows;
   p->D = (int)a->D; p->R = a->rope_dim; p->T = (int)a->T;
@@ -704,10 +726,15 @@ int launch_rope(const SasNormRopeArgs* a, const RopeParams& p, hipStream_t st, c
   return by_width(a, [&](auto ni, auto last, auto half) {
     constexpr int NI = decltype(ni)::value;
     constexpr bool L = decltype(last)::value, HF = decltype(half)::value;
-    if (a->dtype == SAS_DT_BF16)
-      hipLaunchKernelGGL((sas_rope_kernel<__bf16, NI, L, HF, DST>), grid, dim3(kRopeThreads), 0, st, p);
-    else
-      hipLaunchKernelGGL((sas_rope_kernel<_Float16, NI, L, HF, DST>), grid, dim3(kRopeThreads), 0, st, p);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kRopeThreads), 0, st, p); };
+    const bool nt = DST == kToRows && p.nt_load;
+    if (a->dtype == SAS_DT_BF16) {
+      if (nt) go(sas_rope_kernel<__bf16, NI, L, HF, DST, DST == kToRows>);
+      else go(sas_rope_kernel<__bf16, NI, L, HF, DST, false>);
+    } else {
+      if (nt) go(sas_rope_kernel<_Float16, NI, L, HF, DST, DST == kToRows>);
+      else go(sas_rope_kernel<_Float16, NI, L, HF, DST, false>);
+    }
     return launched(what);
   });
 }
@@ -858,17 +885,18 @@ extern "C" int sas_cache_append_v1(const SasCacheAppendArgs* a, void* stream) {
   fill_rope(r, &p);
   p.cu = a->cu_seqlens_q; p.used = a->act_kv; p.bt = a->block_table; p.cache = (uint8_t*)a->cache;
   p.B = (int)a->B; p.bt_stride = (int)a->bt_stride; p.bs = (int)a->block_size; p.nblocks = (int)a->num_blocks;
+  p.bs_shift = p.bs & (p.bs - 1) ? -1 : __builtin_ctz(p.bs);
   hipStream_t st = (hipStream_t)stream;
   if (!fp8) return launch_rope<kToCache>(r, p, st, "cache_append");
   const dim3 grid((unsigned)(p.part[0].blocks + p.part[1].blocks)), block(kRopeThreads);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   const bool half = r->flags & SAS_ROPE_HALF;
   if (r->rope_dim == 64 || r->rope_dim == 0) {
-    if (half) go(sas_rope_kernel<__bf16, 5, true, true, kToFp8>);
-    else go(sas_rope_kernel<__bf16, 5, true, false, kToFp8>);
+    if (half) go(sas_rope_kernel<__bf16, 5, true, true, kToFp8, false>);
+    else go(sas_rope_kernel<__bf16, 5, true, false, kToFp8, false>);
   } else {
-    if (half) go(sas_rope_kernel<__bf16, 5, false, true, kToFp8>);
-    else go(sas_rope_kernel<__bf16, 5, false, false, kToFp8>);
+    if (half) go(sas_rope_kernel<__bf16, 5, false, true, kToFp8, false>);
+    else go(sas_rope_kernel<__bf16, 5, false, false, kToFp8, false>);
   }
   return launched("cache_append");
 }
