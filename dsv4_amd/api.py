@@ -874,7 +874,8 @@ def sparse_attn_sharedkv_tree(
     the committed and compressed rows alone.
 
     The other arguments and the result are :func:`sparse_attn_sharedkv`'s; a chain
-    (bits ``0 .. i`` of node ``i``) gives what that function gives.
+    (bits ``0 .. i`` of node ``i``) gives what that function gives, up to rounding where
+    the two take different kernels.
     """
     lead = tuple(q.shape[:-2])
     if tree_mask.dtype is not torch.int64 or tree_mask.dim() != len(lead) + 1 or tuple(tree_mask.shape[:-1]) != lead or \

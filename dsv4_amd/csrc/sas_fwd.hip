@@ -40,6 +40,9 @@
 // :877 (P cast), :1135-1145 (LSE), and golden.py:69-204.
 
 #include "sas_fwd_win.h"
+#if SAS_FWD_TREE
+#include "sas_fwd_pair.h"
+#endif
 
 #include <mutex>
 
@@ -2219,6 +2222,15 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
   return launch_combine(fp, a->out_dtype, st);
 }
 
+#if SAS_FWD_TREE
+// Whether a call takes two workgroups a CU (sas_fwd_pair.h): more (token, 64 heads)
+// items than CUs, all of a token's slots in one workgroup.
+bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
+  return a->kv_dtype == a->q_dtype && a->H % 64 == 0 && pl.nsplit == 1 && pl.nslots <= kMaxSlots && a->head_waves == 0 &&
+         a->waves == 0 && a->T * (a->H / 64) > sas::device_cus();
+}
+#endif
+
 // sas_fwd_v1, or (kTree) sas_fwd_tree_v1
 int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, void* stream) {
   Plan pl;
@@ -2299,6 +2311,14 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
       return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
     }
   }
+#if SAS_FWD_TREE
+  if (use_pairs(a, pl)) {
+    fp.nhg = (int)a->H / 64;
+    const long long nb = (a->T + fp.nxcd - 1) / fp.nxcd * fp.nhg * fp.nxcd;
+    if (a->q_dtype == SAS_DT_BF16) return a->D == 576 ? launch_pair<576, __bf16>(fp, (int)nb, st) : launch_pair<512, __bf16>(fp, (int)nb, st);
+    return a->D == 576 ? launch_pair<576, _Float16>(fp, (int)nb, st) : launch_pair<512, _Float16>(fp, (int)nb, st);
+  }
+#endif
   if (fp8) rc = dispatch_hw<576, __bf16, 1>(pl.hw, pl.nw, pl.exact, fp, nblocks, st);
   else if (a->q_dtype == SAS_DT_BF16)
     rc = a->D == 576 ? dispatch_hw<576, __bf16, 0>(pl.hw, pl.nw, pl.exact, fp, nblocks, st)

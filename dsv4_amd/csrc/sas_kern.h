@@ -477,8 +477,11 @@ struct Tree {
 // (4K prefill 580 -> 573 µs with 4 resolving waves). `mid` runs after the
 // block-table loads are issued (a caller can put its own loads behind them
 // there).
-template <int NT, int ROWB, bool TREE = false, typename Mid>
-__device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int lane, int wave, Mid&& mid) {
+// With LIST the rows go to `list` instead, as 32-bit cache row indices (bit 31: a
+// compressed row).
+template <int NT, int ROWB, bool TREE = false, bool LIST = false, typename Mid>
+__device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int lane, int wave, Mid&& mid,
+                                        uint32_t* list = nullptr) {
   constexpr int NWV = NT / 64;
   constexpr int kRounds = (kMaxSlots + NT - 1) / NT;
   static_assert(kRounds <= kRoundsMax && NWV <= kMaxWaves, "resolve geometry");
@@ -584,7 +587,8 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
       const bool inb = phys[r] >= 0 && phys[r] < (ori[r] ? p.ori_nblocks : p.cmp_nblocks);
       val[r] = ok[r] && inb;
       const int row = val[r] ? phys[r] * (ori[r] ? p.ori_bs : p.cmp_bs) + off[r] : 0;
-      rad[r] = reinterpret_cast<uint64_t>(ori[r] ? p.ori_kv : p.cmp_kv) + (uint64_t)(uint32_t)row * ROWB;
+      rad[r] = LIST ? (uint64_t)((uint32_t)row | (ori[r] ? 0u : 1u << 31))
+                    : reinterpret_cast<uint64_t>(ori[r] ? p.ori_kv : p.cmp_kv) + (uint64_t)(uint32_t)row * ROWB;
     }
   } else {
     mid();
@@ -608,8 +612,11 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
       wpre += w < wave ? cw : 0;
       tot += cw;
     }
-    if (val[r])
-      lds_rows[nvalid + wpre + __popcll(vmask[r] & ((1ull << lane) - 1ull))] = rad[r];
+    const int at = nvalid + wpre + __popcll(vmask[r] & ((1ull << lane) - 1ull));
+    if (val[r]) {
+      if constexpr (LIST) list[at] = (uint32_t)rad[r];
+      else lds_rows[at] = rad[r];
+    }
     nvalid += tot;
   }
   k.b = lds_tok[0];
