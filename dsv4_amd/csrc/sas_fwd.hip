@@ -2224,10 +2224,15 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 
 #if SAS_FWD_TREE
 // Whether a call takes two workgroups a CU (sas_fwd_pair.h): more (token, 64 heads)
-// items than CUs, all of a token's slots in one workgroup.
+// items than CUs, all of a token's slots in one workgroup. fp8 rows, whose other kernel
+// takes 32 heads a workgroup: long rows of up to 1.5 items a CU are three of its rounds and
+// stay there (320 items: 1152 slots 123 us against 133, 640 slots 79 both, 256 slots 46
+// against 41; 480 items 164 / 135, 106 / 82, 58 / 41).
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
-  return a->kv_dtype == a->q_dtype && a->H % 64 == 0 && pl.nsplit == 1 && pl.nslots <= kMaxSlots && a->head_waves == 0 &&
-         a->waves == 0 && a->T * (a->H / 64) > sas::device_cus();
+  const long long items = a->T * (a->H / 64), cus = sas::device_cus();
+  if (a->H % 64 || pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0 || items <= cus)
+    return false;
+  return a->kv_dtype == a->q_dtype || pl.nslots <= 640 || 2 * items > 3 * cus;
 }
 #endif
 
@@ -2315,6 +2320,7 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
   if (use_pairs(a, pl)) {
     fp.nhg = (int)a->H / 64;
     const long long nb = (a->T + fp.nxcd - 1) / fp.nxcd * fp.nhg * fp.nxcd;
+    if (fp8) return launch_pair8(fp, (int)nb, st);
     if (a->q_dtype == SAS_DT_BF16) return a->D == 576 ? launch_pair<576, __bf16>(fp, (int)nb, st) : launch_pair<512, __bf16>(fp, (int)nb, st);
     return a->D == 576 ? launch_pair<576, _Float16>(fp, (int)nb, st) : launch_pair<512, _Float16>(fp, (int)nb, st);
   }

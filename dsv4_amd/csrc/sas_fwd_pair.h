@@ -21,6 +21,71 @@
 namespace sas {
 namespace {
 
+constexpr int kPairPT = 4, kPairSRB = kPairPT * 32 + 16, kPairStage = 16 * kPairSRB;   // output staging of a wave
+
+// 16 heads x 512 channels (lane (g, c16): channels 16 i + 4 g .. + 3 of head c16) scaled
+// by inv, kPairPT channel tiles at a time through the wave's own LDS rows, out in
+// whole runs of a head's row
+template <typename QT>
+__device__ __forceinline__ void put_out(const f32x4 (&acc)[kDV / 16], float inv, uint8_t* sb, uint8_t* ob, int lane) {
+  constexpr int CPR = kPairPT * 2;
+  const int c16 = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int c = 0; c < kDV / 16; c += kPairPT) {
+#pragma unroll
+    for (int i = 0; i < kPairPT; ++i)
+      *reinterpret_cast<uint2*>(sb + c16 * kPairSRB + (i * 16 + 4 * g) * 2) =
+          make_uint2(pack2<QT>(acc[c + i][0] * inv, acc[c + i][1] * inv), pack2<QT>(acc[c + i][2] * inv, acc[c + i][3] * inv));
+#pragma unroll
+    for (int i = 0; i < 16 * CPR / 64; ++i) {
+      const int e = i * 64 + lane, r = e / CPR, q = e - r * CPR;
+      const u32x4g w = *reinterpret_cast<const u32x4g*>(sb + r * kPairSRB + q * 16);
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4g*>(ob + (size_t)r * kDV * 2 + c * 32 + q * 16));
+    }
+  }
+}
+// an item without rows: zeros, and the sink (a padded token: 0)
+__device__ __forceinline__ void put_none(uint8_t* ob, float* lse, float lse0, int lane) {
+  uint4* o = reinterpret_cast<uint4*>(ob);
+#pragma unroll
+  for (int i = 0; i < 16 * kDV * 2 / 16 / 64; ++i) o[i * 64 + lane] = make_uint4(0, 0, 0, 0);
+  if (lane < 16) lse[lane] = lse0;
+}
+
+// Online softmax of a step's scores (lane (g, c16): keys 16 mt + 4 g + j of head c16;
+// nk of the 32 keys count), in the log2 domain: P in s, the lane's sum in l, and O and l
+// rescaled in place where a row's maximum rises by more than 2^8 over the reference m.
+__device__ __forceinline__ void softmax_step(f32x4 (&s)[2], f32x4 (&acc)[kDV / 16], float& m, float& l, float scale,
+                                             int nk, int g) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) s[mt] *= scale;
+  if (nk < 32) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (16 * mt + 4 * g + j >= nk) s[mt][j] = -INFINITY;
+  }
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt) mx = fmaxf(mx, fmaxf(fmaxf(s[mt][0], s[mt][1]), fmaxf(s[mt][2], s[mt][3])));
+  mx = rows_max(mx);
+  if (__ballot(mx > m + kLazyLog2)) {
+    const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    l *= al;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < kDV / 16; ++i)   // in place: written as a product, the accumulators are copied on both paths
+      asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3"
+                   : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]) : "v"(al));
+  }
+  const float mb = m == -INFINITY ? 0.f : m;             // no sink and no finite score yet: every P is 0
+#pragma unroll
+  for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { s[mt][j] = __builtin_amdgcn_exp2f(s[mt][j] - mb); l += s[mt][j]; }
+}
+
 template <int D, typename QT>
 __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p) {
   // slot: the 32 rows' latent chunks [32][64] (chunk c of row r at c ^ swz<64>(r)), then,
@@ -28,8 +93,7 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   // instruction, eight rows' rope another
   constexpr int KS = D / 32, NT = kDV / 16, LCH = 64, ROPE = D > kDV, RI = 8 + ROPE;
   constexpr int LAT = 32 * LCH * 16, SLOT = LAT + ROPE * 32 * 128;
-  constexpr int PT = 4, SRB = PT * 32 + 16, CPR = PT * 2;   // channel tiles staged at a time, staged row bytes, chunks
-  static_assert(4 * 16 * SRB <= SLOT, "the output is staged in the first slot");
+  static_assert(4 * kPairStage <= SLOT, "the output is staged in the first slot");
   static_assert(2 * SLOT + kMaxSlots * 4 + 1024 <= 80 * 1024, "two workgroups share a CU's LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * SLOT];
   __shared__ uint32_t rows[kMaxSlots];
@@ -50,11 +114,8 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   uint8_t* ob = p.out + ((size_t)k.t * p.H + hq) * kDV * 2;
   float* lse = p.lse + (size_t)k.t * p.H + hq;
   const float sink2 = p.sinks[hq + c16] * kLog2e;
-  if (n == 0) {                                            // padded, or nothing attended: the sink alone
-    uint4* o = reinterpret_cast<uint4*>(ob);
-#pragma unroll
-    for (int i = 0; i < 16 * kDV * 2 / 16 / 64; ++i) o[i * 64 + lane] = make_uint4(0, 0, 0, 0);
-    if (g == 0) lse[c16] = k.padded ? 0.f : sink2 * kLn2;
+  if (n == 0) {
+    put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
     return;
   }
 
@@ -129,36 +190,10 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
       }
       ++ps;
     }
-    // lane (g, c16): keys 16 mt + 4 g + j of head c16
-    const int nk = n - st * 32;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) s[mt] *= p.scale_log2;
-    if (nk < 32) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (16 * mt + 4 * lg + j >= nk) s[mt][j] = -INFINITY;
-    }
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) mx = fmaxf(mx, fmaxf(fmaxf(s[mt][0], s[mt][1]), fmaxf(s[mt][2], s[mt][3])));
-    mx = rows_max(mx);
-    if (__ballot(mx > m + kLazyLog2)) {
-      const float mn = fmaxf(m, mx), al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= al;
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < NT; ++i)   // in place: written as a product, the accumulators are copied on both paths
-        asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3"
-                     : "+v"(acc[i][0]), "+v"(acc[i][1]), "+v"(acc[i][2]), "+v"(acc[i][3]) : "v"(al));
-    }
-    const float mb = m == -INFINITY ? 0.f : m;             // no sink and no finite score yet: every P is 0
+    softmax_step(s, acc, m, l, p.scale_log2, n - st * 32, lg);
     uint32_t pk[4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { s[mt][j] = __builtin_amdgcn_exp2f(s[mt][j] - mb); l += s[mt][j]; }
       pk[2 * mt] = pack2<QT>(s[mt][0], s[mt][1]);
       pk[2 * mt + 1] = pack2<QT>(s[mt][2], s[mt][3]);
     }
@@ -195,31 +230,193 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   wait_vm<0>();                                            // the spare step's DMA
   lds_barrier();                                           // every wave has done with the ring: the output is staged there
   asm volatile("" ::: "memory");
-  // 16 heads x 512 channels (lane (g, c16): channels 16 i + 4 g .. + 3 of head c16), PT
-  // channel tiles at a time through the wave's own LDS rows, out in whole runs of a head's row
-  uint8_t* sb = ring + wave * 16 * SRB;
-#pragma unroll
-  for (int c = 0; c < NT; c += PT) {
-#pragma unroll
-    for (int i = 0; i < PT; ++i)
-      *reinterpret_cast<uint2*>(sb + c16 * SRB + (i * 16 + 4 * g) * 2) =
-          make_uint2(pack2<QT>(acc[c + i][0] * inv, acc[c + i][1] * inv), pack2<QT>(acc[c + i][2] * inv, acc[c + i][3] * inv));
-#pragma unroll
-    for (int i = 0; i < 16 * CPR / 64; ++i) {
-      const int e = i * 64 + lane, r = e / CPR, q = e - r * CPR;
-      const u32x4g w = *reinterpret_cast<const u32x4g*>(sb + r * SRB + q * 16);
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4g*>(ob + (size_t)r * kDV * 2 + c * 32 + q * 16));
-    }
-  }
+  put_out<QT>(acc, inv, ring + wave * kPairStage, ob, lane);
   if (g == 0) lse[c16] = m * kLn2 + logf(l);
 }
 
+// The same over fp8 rows (576 channels): two slots of 21 KB that keep the rows as they
+// are, and in the LDS that leaves the first kPair8Q k-steps of Q^T (with all of it in
+// registers eight fragments spill, and each step's reloads wait for the row DMA). A slot holds latent bytes [32 rows][32 chunks] (chunk c of
+// row r at c ^ sw(r), sw a bijection of the 32 rows, even below row 16), rope [32][8] (at c ^
+// (r >> 1)), and the rows' four scales [32][1]. Fragments are converted to bf16 (exactly, unscaled)
+// as they are read; a scale group's four k-steps are a chain of their own, folded into S
+// with the rows' fp32 scales, and P x scale is what is rounded for P.V. Bound by the
+// conversions (256 a step and wave beside 68 MFMAs). us against the 32-head kernel, which
+// needs four rounds: 480 nodes, 64 heads, 128-row window 28 against 67, with 512 / 1024 top-k
+// rows 82 / 135 against 106 / 164; 4 trees of 64 nodes, 128 heads, 1024 rows 134 against 162.
+constexpr int kPair8Slot = 21 * 1024, kPair8Rope = 16 * 1024, kPair8Scl = 20 * 1024, kPair8Q = 8;
+__device__ __forceinline__ int pair8_swz(int r) { return ((r << 1) | (r >> 4)) & 31; }
+
+__global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p) {
+  constexpr int D = 576, KS = D / 32, NT = kDV / 16, NS = 2, NQ = kPair8Q;
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  static_assert(4 * kPairStage <= kPair8Slot && NS * kPair8Slot + 4 * NQ * 1024 + kMaxSlots * 4 + 1024 <= 80 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * kPair8Slot];
+  __shared__ uint32_t rows[kMaxSlots];
+  __shared__ __attribute__((aligned(16))) uint4 qs[4][NQ][64];   // a wave's Q^T fragments, k-steps 0 .. NQ - 1
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int c16 = lane & 15, g = lane >> 4;
+  const int item = item_index<true>(p);
+  if (item < 0) return;
+  Tok k = item_of(p, item);
+  const int hq = k.hg * 64 + wave * 16;
+  uint4 qf[KS];
+  resolve<256, kRow656, true, true>(p, k, tid, lane, wave, [&] {
+    const uint4* q = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq + c16) * D * 2) + g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = q[ks * 4];
+  }, rows);
+  const int n = __builtin_amdgcn_readfirstlane(k.nvalid), steps = (n + 31) >> 5;
+  uint8_t* ob = p.out + ((size_t)k.t * p.H + hq) * kDV * 2;
+  float* lse = p.lse + (size_t)k.t * p.H + hq;
+  const float sink2 = p.sinks[hq + c16] * kLog2e;
+  if (n == 0) {
+    put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
+    return;
+  }
+
+  // producer: of a step's 21 DMA instructions wave w issues latent ones w + 4 j (two rows
+  // each), rope one w (eight rows) and, wave 0, the scales' (32 rows); rows past the last
+  // repeat it
+  const uint64_t ob_ = reinterpret_cast<uint64_t>(p.ori_kv), cb_ = reinterpret_cast<uint64_t>(p.cmp_kv);
+  auto fire = [&](int step, int j, int ln) {
+    const int r = j < 4 ? 2 * (wave + 4 * j) + (ln >> 5) : j == 4 ? 8 * wave + (ln >> 3) : ln & 31;
+    const uint32_t col = j < 4 ? (uint32_t)(((ln & 31) ^ pair8_swz(r)) * 16)
+                         : j == 4 ? 528u + (uint32_t)(((ln & 7) ^ ((r >> 1) & 7)) * 16) : 512u;
+    const uint32_t e = rows[min(step * 32 + r, n - 1)];
+    const uint64_t a = (e >> 31 ? cb_ : ob_) + (uint64_t)(e & 0x7fffffffu) * kRow656 + col;
+    const int i = j < 4 ? wave + 4 * j : j == 4 ? 16 + wave : 20;
+    dma16(reinterpret_cast<const void*>(a),
+          __builtin_amdgcn_readfirstlane(lds_addr_of(ring) + (uint32_t)(step % NS) * kPair8Slot + i * 1024));
+  };
+  auto fire_all = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) fire(step, j, lane);
+    if (wave == 0) fire(step, 5, lane);
+  };
+  f32x4 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = sink2, l = 0.f;                                // l: this lane's keys
+#pragma unroll
+  for (int ks = 0; ks < NQ; ++ks) qs[wave][ks][lane] = qf[ks];   // (its own reads alone follow)
+  __builtin_amdgcn_s_waitcnt(0);                           // the query is here before the loop, as above
+  fire_all(0);
+  for (int st = 0; st < steps; ++st) {
+    wait_vm<0>();                                          // my DMA of this step
+    lds_barrier();
+    asm volatile("" ::: "memory");
+    const uint32_t kt = lds_addr_of(ring) + (uint32_t)(st % NS) * kPair8Slot;
+    // (lane offsets made anew each step: kept, they spill, and a reload waits for the DMA)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int lc = ln & 15, lg = ln >> 4;
+    const uint32_t k0 = (uint32_t)(lc * 512 + (((lg >> 1) ^ pair8_swz(lc)) * 16) + 8 * (lg & 1));   // rows lc
+    const uint32_t k1 = (k0 ^ 16u) + 16 * 512;                                                      // rows 16 + lc
+    const uint32_t kr = (uint32_t)(kPair8Rope + lc * 128 + ((lg ^ ((lc >> 1) & 7)) * 16));
+    auto kraw = [&](int ks, int mt) {
+      return *reinterpret_cast<const LDS_AS u32x2*>((size_t)(kt + ((mt ? k1 : k0) ^ (uint32_t)(ks * 32))));
+    };
+    auto scales = [&](int G, int mt) {   // of the lane's keys 16 mt + 4 g + j
+      const LDS_AS float* f = reinterpret_cast<const LDS_AS float*>((size_t)(kt + kPair8Scl + (uint32_t)((16 * mt + 4 * lg) * 16 + 4 * G)));
+      return f32x4{f[0], f[4], f[8], f[12]};
+    };
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    const uint32_t qa = lds_addr_of(&qs[wave][0][0]) + 16u * (uint32_t)ln;
+    auto qraw = [&](int ks) { return *reinterpret_cast<const LDS_AS u32x4g*>((size_t)(qa + (uint32_t)(ks * 1024))); };
+    constexpr int PF = 1;   // (2: a fragment of Q^T spills)
+    u32x2 a[PF][2];
+    u32x4g qn = qraw(0);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) { a[i][0] = kraw(i, 0); a[i][1] = kraw(i, 1); }
+#pragma unroll
+    for (int G = 0; G < 4; ++G) {
+      f32x4 gacc[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ks = 4 * G + i;
+        const uint4 q = ks < NQ ? __builtin_bit_cast(uint4, qn) : qf[ks];
+        if (ks + 1 < NQ) qn = qraw(ks + 1);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const u32x2 raw = a[ks % PF][mt];
+          if (ks + PF < 16) a[ks % PF][mt] = kraw(ks + PF, mt);
+          uint4 b;
+          e4m3x4_to_bf16(raw.x, b.x, b.y);
+          e4m3x4_to_bf16(raw.y, b.z, b.w);
+          gacc[mt] = mfma32k<__bf16>(b, q, i == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : gacc[mt]);
+        }
+        if (i == 1) fire(st + 1, G, ln);                   // into the slot that step st - 1 left
+        __builtin_amdgcn_sched_barrier(0);                 // (reads and conversions of many k-steps at once spill)
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) s[mt] += scales(G, mt) * gacc[mt];
+    }
+    fire(st + 1, 4, ln);
+    if (wave == 0) fire(st + 1, 5, ln);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const u32x4g b = *reinterpret_cast<const LDS_AS u32x4g*>((size_t)(kt + (kr ^ (uint32_t)(h * 64)) + mt * 16 * 128));
+        s[mt] = mfma32k<__bf16>(__builtin_bit_cast(uint4, b), qf[16 + h], s[mt]);
+      }
+    softmax_step(s, acc, m, l, p.scale_log2, n - st * 32, lg);
+    // V^T: the 8-bit transposed read gives lane j of 16 byte j % 8 of the addresses of lanes
+    // 2 i + (j >= 8), i = 0 .. 7, so lane (g, c16) points at key 4 g + i (i < 4) or 12 + 4 g + i, i = c16
+    // >> 1, and receives channel c16 of its group's eight keys in the order of its P
+    int vn = lane;
+    asm volatile("" : "+v"(vn));
+    const int vi = (vn & 15) >> 1, vr = (vi < 4 ? 0 : 12) + 4 * (vn >> 4) + vi;
+    const uint32_t va = (uint32_t)(vr * 512 + pair8_swz(vr) * 16 + 8 * (vn & 1));
+    auto vraw = [&](int ct) {
+      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS_AS v2i*)(size_t)(kt + (va ^ (uint32_t)(ct * 16))));
+    };
+    constexpr int PV = 4;
+    v2i v[PV];
+#pragma unroll
+    for (int i = 0; i < PV; ++i) v[i] = vraw(i);
+#pragma unroll
+    for (int G = 0; G < 4; ++G) {
+      const f32x4 f0 = scales(G, 0) * s[0], f1 = scales(G, 1) * s[1];
+      const uint4 pf = make_uint4(pack2<__bf16>(f0[0], f0[1]), pack2<__bf16>(f0[2], f0[3]), pack2<__bf16>(f1[0], f1[1]),
+                                  pack2<__bf16>(f1[2], f1[3]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int ct = 8 * G + i;
+        const v2i raw = v[ct % PV];
+        if (ct + PV < NT) v[ct % PV] = vraw(ct + PV);
+        uint4 b;
+        e4m3x4_to_bf16((uint32_t)raw.x, b.x, b.y);
+        e4m3x4_to_bf16((uint32_t)raw.y, b.z, b.w);
+        acc[ct] = mfma32k<__bf16>(b, pf, acc[ct]);
+        if (i & 1) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  l = rows_sum(l) + __builtin_amdgcn_exp2f(sink2 - (m == -INFINITY ? 0.f : m));
+  const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no sink, no row)
+  wait_vm<0>();                                            // the spare step's DMA
+  lds_barrier();                                           // every wave has done with the ring: the output is staged there
+  asm volatile("" ::: "memory");
+  put_out<__bf16>(acc, inv, ring + wave * kPairStage, ob, lane);
+  if (g == 0) lse[c16] = m * kLn2 + logf(l);
+}
+
+int pair_launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? SAS_OK : sas::set_error(SAS_ELAUNCH, "sas_fwd_pair launch: %s", hipGetErrorString(e));
+}
 template <int D, typename QT>
 int launch_pair(const FwdParams& fp, int nblocks, hipStream_t st) {
   hipLaunchKernelGGL((sas_fwd_pair_kernel<D, QT>), dim3(nblocks), dim3(256), 0, st, fp);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return sas::set_error(SAS_ELAUNCH, "sas_fwd_pair launch: %s", hipGetErrorString(e));
-  return SAS_OK;
+  return pair_launched();
+}
+int launch_pair8(const FwdParams& fp, int nblocks, hipStream_t st) {
+  hipLaunchKernelGGL(sas_fwd_pair8_kernel, dim3(nblocks), dim3(256), 0, st, fp);
+  return pair_launched();
 }
 
 }  // namespace

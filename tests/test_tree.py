@@ -219,6 +219,10 @@ CASES = {
     "pairs_fp16": dict(kind="scfa", dt="fp16", H=128, D=512, ql=[70, 65], kl=[400, 65], K=90, bs=16),
     "pairs_narrow": dict(kind="swa", dt="bf16", H=64, D=576, ql=[60] * 5, kl=[60, 61, 70, 200, 500], win=1),
     "pairs_missing": dict(kind="scfa", dt="bf16", H=64, D=576, ql=[130, 140], kl=[5, 30], K=70, win=200),
+    "pairs_fp8": dict(kind="scfa", dt="fp8", H=64, D=576, ql=[30, 0, 41] + [24] * 9, kl=[300, 9, 41] + [40 + 70 * i for i in range(9)],
+                      K=150, ratio=8, tail=5, holes=True),
+    "pairs_fp8_swa": dict(kind="swa", dt="fp8", H=128, D=576, ql=[60] * 3, kl=[60, 61, 500], win=3),
+    "pairs_fp8_cfa": dict(kind="cfa", dt="fp8", H=128, D=576, ql=[66, 70], kl=[5, 800], ratio=4, win=200),
     "long_topk": dict(kind="scfa", dt="bf16", H=128, D=576, ql=[33], kl=[5000], K=1024),
 }
 
@@ -246,11 +250,12 @@ def test_gpu_rows_without_bits(dt):
 
 
 @pytest.mark.gpu
-def test_gpu_pairs_rows_without_bits():
+@pytest.mark.parametrize("dt", ["bf16", "fp8"])
+def test_gpu_pairs_rows_without_bits(dt):
     """As above, with more items than compute units: half the trees attend
     nothing, some of them without committed rows; a sink of -inf beside them."""
     trees = [[[]] * 20 if b % 2 else [list(range(i + 1)) for i in range(20)] for b in range(14)]
-    c = Case(kind="scfa", dt="bf16", H=64, D=512, ql=[20] * 14, kl=[20 + 9 * (b // 2) for b in range(14)], K=64, trees=trees)
+    c = Case(kind="scfa", dt=dt, H=64, D=576, ql=[20] * 14, kl=[20 + 9 * (b // 2) for b in range(14)], K=64, trees=trees)
     out, lse = _run(c)
     c.check(out, lse)
     assert bool((out[20:40] == 0).all()) and torch.allclose(lse[20].cpu(), c.sinks, atol=1e-6)
