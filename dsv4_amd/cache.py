@@ -221,7 +221,7 @@ def append_kv_cache(
     b.extra = _APPEND_DIMS.pack(B, bt.shape[1], cache.shape[1], cache.shape[0],
                                 _lib.SAS_DT_FP8_E4M3_ROW656 if fp8 else _DT[kv.dtype], 0)
     if bt is block_table and cu is cu_seqlens_q and used is seqused_kv:
-        rope._keep(key, b, q, kv, positions, table, q_weight, weight)
+        rope._keep(key, b, q, kv, positions, table, q_weight, weight, (q_norm_dim, norm_dim, eps, interleaved))
     rope._launch("sas_cache_append_v1", b.ptrs(out, None) + b.dims + _APPEND_PTRS.pack(
         cu.data_ptr(), used.data_ptr(), bt.data_ptr(), cache.data_ptr()) + b.extra, dev, "append_kv_cache")
     return out

@@ -630,6 +630,7 @@ __global__ void __launch_bounds__(kSumThreads) sas_rope_dw_kernel(const RopeSum 
 // ---------------------------------------------------------------------------
 
 constexpr double kInfinityCache = 256e6;
+constexpr double kMostRows = (1 << 28) - 2 * kRopeRows;
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -648,8 +649,9 @@ int check_rope(const SasNormRopeArgs* a, const char* what) {
       a->kv_norm_dim % 8)
     return set_error(SAS_EINVAL, "%s: norm dims must be multiples of 8 in [0, D]", what);
   if (!(a->eps >= 0.f)) return set_error(SAS_EINVAL, "%s: eps must not be negative", what);
-  if ((double)a->T * (double)std::max<int64_t>(a->H, 1) > 2147483000.0)
-    return set_error(SAS_EINVAL, "%s: more than 2^31 rows", what);
+  // (a launch has fewer than 2^32 threads, sixteen of them a row)
+  const double rows = (double)a->T * ((double)a->H + (a->kv ? 1 : 0));
+  if (rows > kMostRows) return set_error(SAS_EINVAL, "%s: more than 2^%d rows", what, rows >= 2147483648.0 ? 31 : 28);
   if (a->T == 0) return SAS_OK;
   if ((a->H > 0) != (a->q != nullptr)) return set_error(SAS_EINVAL, "%s: q and H go together", what);
   if (!a->q && !a->kv) return set_error(SAS_EINVAL, "%s: null device pointer", what);
@@ -666,8 +668,8 @@ int check_rope(const SasNormRopeArgs* a, const char* what) {
 
 void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
   // (no rotation, or an append's own positions: an address that is read and ignored)
-  p->has_pos = a->positions != nullptr;
-  p->pos = a->positions ? a->positions : (const int32_t*)(a->kv ? a->kv : a->q);
+  p->has_pos = a->positions && a->rope_dim;
+  p->pos = p->has_pos ? a->positions : (const int32_t*)(a->kv ? a->kv : a->q);
   p->table = a->table;
   p->table_rows = (int)a->table_rows;
   p->D = (int)a->D; p->R = a->rope_dim; p->T = (int)a->T;
@@ -681,11 +683,11 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
   kv.n = a->kv_norm_dim;
   q.n = a->q_norm_dim;
   if (a->kv) {
-    kv.x = (const uint8_t*)a->kv; kv.y = (uint8_t*)a->kv_out; kv.w = (const uint8_t*)a->kv_weight;
+    kv.x = (const uint8_t*)a->kv; kv.y = (uint8_t*)a->kv_out; kv.w = kv.n ? (const uint8_t*)a->kv_weight : nullptr;
     kv.st = a->kv_stride_t * 2; kv.rows = (uint32_t)a->T;
   }
   if (a->q) {
-    q.x = (const uint8_t*)a->q; q.y = (uint8_t*)a->q_out; q.w = (const uint8_t*)a->q_weight;
+    q.x = (const uint8_t*)a->q; q.y = (uint8_t*)a->q_out; q.w = q.n ? (const uint8_t*)a->q_weight : nullptr;
     q.st = a->q_stride_t * 2; q.sh = a->q_stride_h * 2; q.rows = (uint32_t)(a->T * a->H);
   }
   for (RopePart& x : p->part) x.blocks = (int)((x.rows + kRopeRows - 1) / kRopeRows);

@@ -164,10 +164,15 @@ def _aligned(*tensors) -> bool:
     return not a & 15
 
 
-def _keep(key, b: _Bound, q, kv, positions, table, q_weight, kv_weight) -> None:
-    """Keep what a call's geometry gives, where its tensors were taken as given."""
-    if (b.q is not q or b.kv is not kv or b.table is not table or (b.pos is not positions and table is not None)
-            or b.qw is not q_weight or b.kw is not kv_weight):
+_SCALARS = (int, float, bool, type(None))
+
+
+def _keep(key, b: _Bound, q, kv, positions, table, q_weight, kv_weight, scalars) -> None:
+    """Keep what a call's geometry gives, where its tensors were taken as given
+    (positions too: without a table they were not looked at) and its scalars are
+    plain ones (a tensor would be found again by its identity)."""
+    if (b.q is not q or b.kv is not kv or b.table is not table or b.pos is not positions
+            or b.qw is not q_weight or b.kw is not kv_weight or any(type(x) not in _SCALARS for x in scalars)):
         return
     if len(_sigs) >= _SIGS_MAX:
         _sigs.clear()
@@ -284,7 +289,7 @@ def norm_rope(
         qo = None if q is None else _out(q, b.q_like)
         ko = None if kv is None else _out(kv, b.kv_like)
         packed = b.ptrs(qo, ko)
-        _keep(key, b, q, kv, positions, table, q_weight, kv_weight)
+        _keep(key, b, q, kv, positions, table, q_weight, kv_weight, (q_norm_dim, kv_norm_dim, eps, interleaved, inverse))
     _launch("sas_norm_rope_v1", packed + b.dims, b.dev, "norm_rope")
     return qo if kv is None else ko if q is None else (qo, ko)
 
@@ -359,10 +364,11 @@ def norm_rope_backward(
     grads = (p(gq), p(gk), p(dq), p(dkv), p(dqw), p(dkw))
     head = (_pack_ptrs(q, kv, qw, kw, positions, table, None, None) if hit else b.ptrs(None, None)) + b.dims
     if not hit:
-        need = _workspace_bytes(head + _GRAD_PTRS.pack(*grads, 0, 0) + strides)
+        with torch.cuda.device(b.dev):   # (the plan counts its compute units)
+            need = _workspace_bytes(head + _GRAD_PTRS.pack(*grads, 0, 0) + strides)
         b.extra = strides, need
         if gq is dq_out and gk is dkv_out:
-            _keep(key, b, q, kv, positions, table, q_weight, kv_weight)
+            _keep(key, b, q, kv, positions, table, q_weight, kv_weight, (q_norm_dim, kv_norm_dim, eps, interleaved, inverse))
     # the partial sums of the weights' gradients, from the caching allocator: under
     # capture from the graph's own pool
     ws = torch.empty(need, dtype=torch.uint8, device=b.dev) if need else None
@@ -400,6 +406,9 @@ def norm_rope_autograd(q: Optional[torch.Tensor], kv: Optional[torch.Tensor] = N
                        q_weight: Optional[torch.Tensor] = None, kv_weight: Optional[torch.Tensor] = None, **kwargs):
     """:func:`norm_rope` recorded for autograd: gradients flow to ``q``, ``kv`` and
     the weights through :func:`norm_rope_backward` (not to ``table``). Other
-    arguments and the result as for :func:`norm_rope`."""
+    arguments and the result as for :func:`norm_rope`. To capture a training step
+    while an eager graph of the same leaves lives, capture ``torch.autograd.grad``
+    or :func:`norm_rope_backward`: PyTorch ends the process where a captured
+    ``backward()`` accumulates into such leaves."""
     qo, ko = _NormRopeFn.apply(q, kv, q_weight, kv_weight, kwargs)
     return qo if kv is None else ko if q is None else (qo, ko)

@@ -338,15 +338,16 @@ int sas_cache_write_v1(const SasCacheWriteArgs* a, void* stream);
  * [0, table_rows) is padding: its output rows are zeros.
  * D a multiple of 8 in [8, 1024], rope_dim a multiple of 8 (SAS_ROPE_HALF: 16)
  * in [0, D], norm dims multiples of 8 in [0, D] (0: no norm); strides multiples
- * of 8 elements, every tensor 16-byte aligned. Outputs must not overlap inputs.
+ * of 8 elements, every tensor 16-byte aligned, fewer than 2^28 rows in all. Outputs
+ * must not overlap inputs.
  */
 typedef struct SasNormRopeArgs {
   const void* q;                 /* [T, H, D], or NULL with H = 0 */
   const void* kv;                /* [T, D], or NULL */
   const void* q_weight;          /* [q_norm_dim] weight_dtype, or NULL: ones */
   const void* kv_weight;         /* [kv_norm_dim] weight_dtype, or NULL: ones */
-  const int32_t* positions;      /* [T]; NULL with rope_dim 0 */
-  const float* table;            /* [table_rows, rope_dim / 2, 2]; NULL with rope_dim 0 */
+  const int32_t* positions;      /* [T]; not read with rope_dim 0 */
+  const float* table;            /* [table_rows, rope_dim / 2, 2]; not read with rope_dim 0 */
   void* q_out;                   /* [T, H, D] contiguous */
   void* kv_out;                  /* [T, D] contiguous */
   int64_t T, H, D;

@@ -681,3 +681,52 @@ def test_gpu_training_step_through_the_attention():
         torch.cuda.synchronize()
         for a, b in zip(got, norm_rope_backward(gq, qd, gk, kd, **args)):
             assert a is b is None or torch.equal(a, b)
+
+
+def test_abi_refuses_more_rows_than_a_launch_has_threads_for():
+    L = _lib.lib()
+    small = dict(H=0, q=None, q_out=None, D=8, kv_stride_t=8, rope_dim=0, kv_norm_dim=8, q_norm_dim=0)
+    for over in (dict(small, T=1 << 28), dict(T=(1 << 24) - 1, H=16, kv=None)):
+        if "kv" in over:   # the queries alone reach it from 2^28 - 31 rows on
+            over["T"] += 1
+        assert L.sas_norm_rope_v1(C.byref(_args(**over)), None) == _lib.SAS_EINVAL
+        assert "2^28" in L.sas_last_error().decode()
+        ca = _lib.SasCacheAppendArgs(rope=_args(**over), cu_seqlens_q=FAKE, act_kv=FAKE, block_table=FAKE, cache=FAKE, B=1,
+                                     bt_stride=1, block_size=64, num_blocks=1, cache_dtype=_lib.SAS_DT_BF16)
+        assert L.sas_cache_append_v1(C.byref(ca), None) == _lib.SAS_EINVAL
+        assert "2^28" in L.sas_last_error().decode()
+    n = C.c_size_t(0)
+    ba = _lib.SasNormRopeBwdArgs(fwd=_args(T=(1 << 28) // 17 - 16), dq_weight=FAKE)
+    assert L.sas_norm_rope_bwd_plan(C.byref(ba), C.byref(n)) == _lib.SAS_OK and n.value > 0
+
+
+@pytest.mark.gpu
+def test_gpu_positions_without_a_table_are_not_read():
+    """The same signature twice: the second call takes the kept resolution."""
+    from dsv4_amd.cache import append_kv_cache
+    from dsv4_amd.rope import norm_rope, norm_rope_backward
+    q = torch.randn(40, 16, 512, device="cuda").to(torch.bfloat16)
+    kv = q[:, 0].contiguous()
+    want = norm_rope(q, kv)
+    for pos in (torch.zeros(3, dtype=torch.int64, device="cuda"), torch.zeros(40, dtype=torch.int32)):
+        for _ in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(norm_rope(q, kv, positions=pos), want))
+        grads = [norm_rope_backward(q, q, positions=pos)[0] for _ in range(2)]
+        assert torch.equal(*grads) and torch.equal(grads[0], norm_rope_backward(q, q)[0])
+        for _ in range(2):
+            cache = torch.zeros(3, 16, 1, 512, device="cuda", dtype=torch.bfloat16)
+            args = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, 1, 2]], [0, 40], [40])]
+            assert torch.equal(append_kv_cache(kv, cache, *args, positions=pos, q=q), want[0])
+            assert torch.equal(cache.view(48, 512)[:40], want[1])
+
+
+@pytest.mark.gpu
+def test_gpu_scalars_in_tensors_are_read_anew():
+    from dsv4_amd.rope import norm_rope
+    q = torch.randn(4, 16, 128, device="cuda").to(torch.bfloat16)
+    eps = torch.tensor(1e-6)
+    n = torch.tensor(128)
+    norm_rope(q, eps=eps, q_norm_dim=n)
+    eps.fill_(1.0)
+    n.fill_(64)
+    assert torch.equal(norm_rope(q, eps=eps, q_norm_dim=n), norm_rope(q, eps=1.0, q_norm_dim=64))
