@@ -2223,16 +2223,20 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 }
 
 #if SAS_FWD_TREE
-// Whether a call takes two workgroups a CU (sas_fwd_pair.h): more (token, 64 heads)
-// items than CUs, all of a token's slots in one workgroup. fp8 rows, whose other kernel
-// takes 32 heads a workgroup: long rows of up to 1.5 items a CU are three of its rounds and
-// stay there (320 items: 1152 slots 123 us against 133, 640 slots 79 both, 256 slots 46
-// against 41; 480 items 164 / 135, 106 / 82, 58 / 41).
+// Whether a call takes the kernels of two workgroups a CU (sas_fwd_pair.h): all of a
+// token's slots in one workgroup, and
+//  - more (token, 64 heads) items than CUs: the other kernels need a second round; or
+//  - fp8 rows, whose other kernel takes 32 heads a workgroup, from half as many on: 160 to
+//    256 items of 256 / 640 rows 26-28 / 52-53 us against 31-32 / 53-55 (1152 rows: 86-87
+//    against 83-86, left there); or
+//  - a window that the exact schedule holds, from 32 items on (128 rows, 32 to 256 items of
+//    576 channels: 13.0-15.5 us against 14.4-17.5, fp8 16.8-19.2 against 17.7-34; 64 rows 10.9-12.4
+//    against 11.3-14.3; fewer items: the same within 4%).
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
+  if (a->H % 64 || pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
   const long long items = a->T * (a->H / 64), cus = sas::device_cus();
-  if (a->H % 64 || pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0 || items <= cus)
-    return false;
-  return a->kv_dtype == a->q_dtype || pl.nslots <= 640 || 2 * items > 3 * cus;
+  if (pl.exact) return items >= 32;
+  return items > cus || (a->kv_dtype != a->q_dtype && 2 * items > cus && pl.nslots <= 640);
 }
 #endif
 

@@ -1,5 +1,6 @@
-// Draft trees of more (token, 64 heads) items than compute units: one item a
-// workgroup of 4 waves, two workgroups on a CU, MI355X (gfx950).
+// Draft trees of more (token, 64 heads) items than compute units, and windows of fewer
+// (use_pairs() has the rule): one item a workgroup of 4 waves, two workgroups on a CU,
+// MI355X (gfx950).
 //
 // The 8-wave kernel has a CU to itself: its ring fills the LDS, and nothing runs
 // beside a token's slot resolution, its first rows and its output (8 of 46 us at 640
@@ -14,6 +15,11 @@
 // with 512 top-k rows D = 512 55 / 102 against 65 / 128, D = 576 56 / 110 against 66 / 127;
 // over contexts of 8 K to 32 K, read from HBM, 62 / 115 against 71 / 133 and 65 / 123 against
 // 73 / 141. With lane offsets that spilled it was no faster at D = 576.
+//
+// What bounds it (518 nodes, 64 heads, 640 rows of 576 channels): no unit alone. Of a CU's
+// time MFMAs take a third, LDS 37%, VALU 35%; a wave's phases hang on each other and only
+// two waves share a SIMD. K and V operands read further ahead, wave priorities and rows in
+// cache order gave nothing. 512 items take 57 us, the next six 18 more.
 #pragma once
 
 #include "sas_kern.h"
@@ -234,27 +240,25 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   if (g == 0) lse[c16] = m * kLn2 + logf(l);
 }
 
-// The same over fp8 rows (576 channels): two slots of 21 KB that keep the rows as they
-// are, and in the LDS that leaves the first kPair8Q k-steps of Q^T (with all of it in
-// registers eight fragments spill, and each step's reloads wait for the row DMA). A slot holds latent bytes [32 rows][32 chunks] (chunk c of
-// row r at c ^ sw(r), sw a bijection of the 32 rows, even below row 16), rope [32][8] (at c ^
-// (r >> 1)), and the rows' four scales [32][1]. Fragments are converted to bf16 (exactly, unscaled)
-// as they are read; a scale group's four k-steps are a chain of their own, folded into S
-// with the rows' fp32 scales, and P x scale is what is rounded for P.V. Bound by the
-// conversions (256 a step and wave beside 68 MFMAs). us against the 32-head kernel, which
-// needs four rounds: 480 nodes, 64 heads, 128-row window 28 against 67, with 512 / 1024 top-k
-// rows 82 / 135 against 106 / 164; 4 trees of 64 nodes, 128 heads, 1024 rows 134 against 162.
-constexpr int kPair8Slot = 21 * 1024, kPair8Rope = 16 * 1024, kPair8Scl = 20 * 1024, kPair8Q = 8;
-__device__ __forceinline__ int pair8_swz(int r) { return ((r << 1) | (r >> 4)) & 31; }
+// The same over fp8 rows (576 channels): two slots of 21 KB take the rows as they are
+// (latent bytes [32 rows][512], rope [32][8 chunks] (chunk c of row r at c ^ (r >> 1)), the
+// rows' four scales [32][16 bytes]), and at a step's head each wave turns the latent bytes
+// that it loaded into bf16 (exactly, unscaled) in one tile of the other kernel's layout: one
+// conversion a value where a fragment converted as it is read has one in each of four
+// waves (4 trees of 64 nodes, 128 heads, 1152 rows: 115 us against 134, 729 VALU instructions a
+// step and wave against 375, 68 of them MFMAs). A scale group's four k-steps are a chain of their
+// own, folded into S with the rows' fp32 scales, and P x scale is what is rounded for P.V.
+// us against the 32-head kernel, which needs four rounds: 480 nodes, 64 heads, 128-row window
+// 27 against 67, with 128 / 512 / 1024 top-k rows 38 / 73 / 119 against 59 / 105 / 164.
+constexpr int kPair8Slot = 21 * 1024, kPair8Rope = 16 * 1024, kPair8Scl = 20 * 1024;
 
 __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p) {
-  constexpr int D = 576, KS = D / 32, NT = kDV / 16, NS = 2, NQ = kPair8Q;
-  typedef int v2i __attribute__((ext_vector_type(2)));
+  constexpr int D = 576, KS = D / 32, NT = kDV / 16, LCH = 64;
   typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-  static_assert(4 * kPairStage <= kPair8Slot && NS * kPair8Slot + 4 * NQ * 1024 + kMaxSlots * 4 + 1024 <= 80 * 1024, "LDS");
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * kPair8Slot];
+  static_assert(4 * kPairStage <= kPair8Slot && 2 * kPair8Slot + 32 * LCH * 16 + kMaxSlots * 4 + 1024 <= 80 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * kPair8Slot];
+  __shared__ __attribute__((aligned(1024))) uint8_t tile[32 * LCH * 16];
   __shared__ uint32_t rows[kMaxSlots];
-  __shared__ __attribute__((aligned(16))) uint4 qs[4][NQ][64];   // a wave's Q^T fragments, k-steps 0 .. NQ - 1
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c16 = lane & 15, g = lane >> 4;
@@ -277,122 +281,131 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
     return;
   }
 
-  // producer: of a step's 21 DMA instructions wave w issues latent ones w + 4 j (two rows
-  // each), rope one w (eight rows) and, wave 0, the scales' (32 rows); rows past the last
-  // repeat it
+  // producer: of a step's 21 DMA instructions wave w issues latent ones w + 4 j (rows 2 w + 8 j
+  // and the next), rope one w (eight rows) and, wave 0, the scales' (32 rows); rows past the
+  // last repeat it
   const uint64_t ob_ = reinterpret_cast<uint64_t>(p.ori_kv), cb_ = reinterpret_cast<uint64_t>(p.cmp_kv);
   auto fire = [&](int step, int j, int ln) {
     const int r = j < 4 ? 2 * (wave + 4 * j) + (ln >> 5) : j == 4 ? 8 * wave + (ln >> 3) : ln & 31;
-    const uint32_t col = j < 4 ? (uint32_t)(((ln & 31) ^ pair8_swz(r)) * 16)
+    const uint32_t col = j < 4 ? (uint32_t)((ln & 31) * 16)
                          : j == 4 ? 528u + (uint32_t)(((ln & 7) ^ ((r >> 1) & 7)) * 16) : 512u;
     const uint32_t e = rows[min(step * 32 + r, n - 1)];
     const uint64_t a = (e >> 31 ? cb_ : ob_) + (uint64_t)(e & 0x7fffffffu) * kRow656 + col;
     const int i = j < 4 ? wave + 4 * j : j == 4 ? 16 + wave : 20;
     dma16(reinterpret_cast<const void*>(a),
-          __builtin_amdgcn_readfirstlane(lds_addr_of(ring) + (uint32_t)(step % NS) * kPair8Slot + i * 1024));
+          __builtin_amdgcn_readfirstlane(lds_addr_of(ring) + (uint32_t)(step & 1) * kPair8Slot + i * 1024));
   };
-  auto fire_all = [&](int step) {
 #pragma unroll
-    for (int j = 0; j < 5; ++j) fire(step, j, lane);
-    if (wave == 0) fire(step, 5, lane);
-  };
+  for (int j = 0; j < 5; ++j) fire(0, j, lane);
+  if (wave == 0) fire(0, 5, lane);
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = sink2, l = 0.f;                                // l: this lane's keys
-#pragma unroll
-  for (int ks = 0; ks < NQ; ++ks) qs[wave][ks][lane] = qf[ks];   // (its own reads alone follow)
   __builtin_amdgcn_s_waitcnt(0);                           // the query is here before the loop, as above
-  fire_all(0);
   for (int st = 0; st < steps; ++st) {
     wait_vm<0>();                                          // my DMA of this step
-    lds_barrier();
+    lds_barrier();                                         // the last step's tile has been read
     asm volatile("" ::: "memory");
-    const uint32_t kt = lds_addr_of(ring) + (uint32_t)(st % NS) * kPair8Slot;
+    const uint32_t sl = lds_addr_of(ring) + (uint32_t)(st & 1) * kPair8Slot, kt = lds_addr_of(tile);
     // (lane offsets made anew each step: kept, they spill, and a reload waits for the DMA)
     int ln = lane;
     asm volatile("" : "+v"(ln));
+    {
+      const uint32_t src = sl + (uint32_t)(2 * wave * 512 + ln * 8), dst = kt + (uint32_t)(2 * wave * 1024);
+      constexpr int kBatch = 4;
+#pragma unroll
+      for (int b0 = 0; b0 < 8; b0 += kBatch) {
+        u32x2 raw[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {   // row 2 wave + 8 (i / 2) + i % 2
+          const int e = b0 + i;
+          raw[i] = *reinterpret_cast<const LDS_AS u32x2*>((size_t)(src + (uint32_t)((e >> 1) * 8 + (e & 1)) * 512));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int e = b0 + i;
+          uint4 b;
+          e4m3x4_to_bf16(raw[i].x, b.x, b.y);
+          e4m3x4_to_bf16(raw[i].y, b.z, b.w);
+          *reinterpret_cast<LDS_AS u32x4g*>((size_t)(dst + (uint32_t)((ln ^ swz<LCH>(2 * wave + (e & 1))) * 16) +
+                                                     (uint32_t)((e >> 1) * 8 + (e & 1)) * 1024)) = __builtin_bit_cast(u32x4g, b);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    lds_barrier();
+    asm volatile("" ::: "memory");
     const int lc = ln & 15, lg = ln >> 4;
-    const uint32_t k0 = (uint32_t)(lc * 512 + (((lg >> 1) ^ pair8_swz(lc)) * 16) + 8 * (lg & 1));   // rows lc
-    const uint32_t k1 = (k0 ^ 16u) + 16 * 512;                                                      // rows 16 + lc
-    const uint32_t kr = (uint32_t)(kPair8Rope + lc * 128 + ((lg ^ ((lc >> 1) & 7)) * 16));
-    auto kraw = [&](int ks, int mt) {
-      return *reinterpret_cast<const LDS_AS u32x2*>((size_t)(kt + ((mt ? k1 : k0) ^ (uint32_t)(ks * 32))));
+    const uint32_t ka = kt + (uint32_t)(lc * 1024 + ((lg ^ swz<LCH>(lc)) * 16));
+    const uint32_t kr = sl + (uint32_t)(kPair8Rope + lc * 128 + ((lg ^ ((lc >> 1) & 7)) * 16));
+    const uint32_t sa = sl + (uint32_t)(kPair8Scl + lg * 64);
+    auto kfrag = [&](int ks, int mt) {
+      return __builtin_bit_cast(uint4, *reinterpret_cast<const LDS_AS u32x4g*>((size_t)(
+          ks < 16 ? (ka ^ (uint32_t)((ks & 3) * 64)) + (uint32_t)((ks >> 2) * 256 + mt * 16 * 1024)
+                  : (kr ^ (uint32_t)((ks & 1) * 64)) + (uint32_t)(mt * 16 * 128))));
     };
     auto scales = [&](int G, int mt) {   // of the lane's keys 16 mt + 4 g + j
-      const LDS_AS float* f = reinterpret_cast<const LDS_AS float*>((size_t)(kt + kPair8Scl + (uint32_t)((16 * mt + 4 * lg) * 16 + 4 * G)));
+      const LDS_AS float* f = reinterpret_cast<const LDS_AS float*>((size_t)(sa + (uint32_t)(16 * mt * 16 + 4 * G)));
       return f32x4{f[0], f[4], f[8], f[12]};
     };
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    const uint32_t qa = lds_addr_of(&qs[wave][0][0]) + 16u * (uint32_t)ln;
-    auto qraw = [&](int ks) { return *reinterpret_cast<const LDS_AS u32x4g*>((size_t)(qa + (uint32_t)(ks * 1024))); };
-    constexpr int PF = 1;   // (2: a fragment of Q^T spills)
-    u32x2 a[PF][2];
-    u32x4g qn = qraw(0);
-#pragma unroll
-    for (int i = 0; i < PF; ++i) { a[i][0] = kraw(i, 0); a[i][1] = kraw(i, 1); }
-#pragma unroll
-    for (int G = 0; G < 4; ++G) {
+    {
+      uint4 a[2] = {kfrag(0, 0), kfrag(0, 1)};   // (two k-steps ahead, a fragment of Q^T spills: 115 -> 122 us)
       f32x4 gacc[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ks = 4 * G + i;
-        const uint4 q = ks < NQ ? __builtin_bit_cast(uint4, qn) : qf[ks];
-        if (ks + 1 < NQ) qn = qraw(ks + 1);
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const u32x2 raw = a[ks % PF][mt];
-          if (ks + PF < 16) a[ks % PF][mt] = kraw(ks + PF, mt);
-          uint4 b;
-          e4m3x4_to_bf16(raw.x, b.x, b.y);
-          e4m3x4_to_bf16(raw.y, b.z, b.w);
-          gacc[mt] = mfma32k<__bf16>(b, q, i == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : gacc[mt]);
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint4 a0 = a[0], a1 = a[1];
+        if (ks + 1 < KS) { a[0] = kfrag(ks + 1, 0); a[1] = kfrag(ks + 1, 1); }
+        if (ks < 16) {
+          const bool first = ks % 4 == 0;
+          gacc[0] = mfma32k<__bf16>(a0, qf[ks], first ? f32x4{0.f, 0.f, 0.f, 0.f} : gacc[0]);
+          gacc[1] = mfma32k<__bf16>(a1, qf[ks], first ? f32x4{0.f, 0.f, 0.f, 0.f} : gacc[1]);
+          if (ks % 4 == 3) {
+            s[0] += scales(ks / 4, 0) * gacc[0];
+            s[1] += scales(ks / 4, 1) * gacc[1];
+            __builtin_amdgcn_sched_barrier(0);   // (the next groups' scales at once spill)
+          }
+        } else {
+          s[0] = mfma32k<__bf16>(a0, qf[ks], s[0]);
+          s[1] = mfma32k<__bf16>(a1, qf[ks], s[1]);
         }
-        if (i == 1) fire(st + 1, G, ln);                   // into the slot that step st - 1 left
-        __builtin_amdgcn_sched_barrier(0);                 // (reads and conversions of many k-steps at once spill)
+        if (ks % 3 == 1 && ks / 3 < 5) fire(st + 1, ks / 3, ln);   // (past the last step: its last row again)
       }
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) s[mt] += scales(G, mt) * gacc[mt];
+      if (wave == 0) fire(st + 1, 5, ln);
     }
-    fire(st + 1, 4, ln);
-    if (wave == 0) fire(st + 1, 5, ln);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const u32x4g b = *reinterpret_cast<const LDS_AS u32x4g*>((size_t)(kt + (kr ^ (uint32_t)(h * 64)) + mt * 16 * 128));
-        s[mt] = mfma32k<__bf16>(__builtin_bit_cast(uint4, b), qf[16 + h], s[mt]);
-      }
     softmax_step(s, acc, m, l, p.scale_log2, n - st * 32, lg);
-    // V^T: the 8-bit transposed read gives lane j of 16 byte j % 8 of the addresses of lanes
-    // 2 i + (j >= 8), i = 0 .. 7, so lane (g, c16) points at key 4 g + i (i < 4) or 12 + 4 g + i, i = c16
-    // >> 1, and receives channel c16 of its group's eight keys in the order of its P
     int vn = lane;
     asm volatile("" : "+v"(vn));
-    const int vi = (vn & 15) >> 1, vr = (vi < 4 ? 0 : 12) + 4 * (vn >> 4) + vi;
-    const uint32_t va = (uint32_t)(vr * 512 + pair8_swz(vr) * 16 + 8 * (vn & 1));
-    auto vraw = [&](int ct) {
-      return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS_AS v2i*)(size_t)(kt + (va ^ (uint32_t)(ct * 16))));
+    const int vr = 4 * (vn >> 4) + ((vn & 15) >> 2);
+    const uint32_t va = kt + (uint32_t)(vr * 1024 + ((((vn & 3) >> 1) ^ swz<LCH>(vr)) * 16) + (vn & 1) * 8);
+    auto vfrag = [&](int ct) {
+      const uint32_t b0 = (va ^ (uint32_t)((ct & 7) * 32)) + (uint32_t)((ct >> 3) * 256);
+      const uint2 u0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)(size_t)b0));
+      const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)(size_t)(b0 + 16 * 1024)));
+      return make_uint4(u0.x, u0.y, u1.x, u1.y);
     };
     constexpr int PV = 4;
-    v2i v[PV];
+    uint4 v[PV];
 #pragma unroll
-    for (int i = 0; i < PV; ++i) v[i] = vraw(i);
+    for (int i = 0; i < PV; ++i) v[i] = vfrag(i);
 #pragma unroll
     for (int G = 0; G < 4; ++G) {
-      const f32x4 f0 = scales(G, 0) * s[0], f1 = scales(G, 1) * s[1];
-      const uint4 pf = make_uint4(pack2<__bf16>(f0[0], f0[1]), pack2<__bf16>(f0[2], f0[3]), pack2<__bf16>(f1[0], f1[1]),
-                                  pack2<__bf16>(f1[2], f1[3]));
+      uint32_t pk[4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const f32x4 f = scales(G, mt) * s[mt];
+        pk[2 * mt] = pack2<__bf16>(f[0], f[1]);
+        pk[2 * mt + 1] = pack2<__bf16>(f[2], f[3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const uint4 pf = make_uint4(pk[0], pk[1], pk[2], pk[3]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int ct = 8 * G + i;
-        const v2i raw = v[ct % PV];
-        if (ct + PV < NT) v[ct % PV] = vraw(ct + PV);
-        uint4 b;
-        e4m3x4_to_bf16((uint32_t)raw.x, b.x, b.y);
-        e4m3x4_to_bf16((uint32_t)raw.y, b.z, b.w);
-        acc[ct] = mfma32k<__bf16>(b, pf, acc[ct]);
-        if (i & 1) __builtin_amdgcn_sched_barrier(0);
+        const uint4 a = v[ct % PV];
+        if (ct + PV < NT) v[ct % PV] = vfrag(ct + PV);
+        acc[ct] = mfma32k<__bf16>(a, pf, acc[ct]);
       }
     }
   }

@@ -385,3 +385,40 @@ def test_gpu_draft_step_append_and_tree_captured():
         assert torch.equal(out, got[0]) and torch.equal(lse, got[1])
         c.q, c.rows = cq.cpu(), kw["ori_kv"].cpu().view(-1, 576)
         c.check(*got)
+
+
+# windows on either side of 32 (token, 64 heads) items, fp8 rows from half as many items
+# as compute units
+MORE = {
+    "window_31": dict(kind="swa", dt="bf16", H=64, D=576, ql=[31], kl=[500]),
+    "window_32": dict(kind="swa", dt="fp16", H=64, D=512, ql=[20, 12], kl=[25, 700], bs=16),
+    "window_32_h128": dict(kind="swa", dt="bf16", H=128, D=576, ql=[1] * 16, kl=[1, 2, 31, 32, 33, 64, 127, 128] * 2, tail=3),
+    "window_32_fp8": dict(kind="swa", dt="fp8", H=64, D=576, ql=[33], kl=[90], win=64, holes=True),
+    "half_fp8": dict(kind="scfa", dt="fp8", H=64, D=576, ql=[64, 66], kl=[300, 5000], K=512),
+    "half_fp8_h128": dict(kind="cfa", dt="fp8", H=128, D=576, ql=[33, 34], kl=[2000, 40], ratio=8, win=100),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(MORE))
+def test_gpu_tree_around_the_rules(name):
+    c = Case(**MORE[name])
+    out, lse = _run(c)
+    c.check(out, lse)
+
+
+@pytest.mark.gpu
+def test_gpu_pairs_fp8_rows_of_far_apart_scales():
+    """A row's groups of 128 channels and the rows among themselves lie up to 2^16
+    apart; rows of zeros between them."""
+    c = Case(kind="scfa", dt="fp8", H=64, D=576, ql=[40] * 7, kl=[200 + 30 * i for i in range(7)], K=96)
+    g = torch.Generator().manual_seed(8)
+    for name in ("cache", "ccache"):
+        rows = torch.randn(*getattr(c, name).shape[:2], 1, 576, generator=g)
+        e = torch.randint(-16, 1, (*rows.shape[:3], 5), generator=g).repeat_interleave(128, -1)[..., :576]
+        rows = torch.where(torch.rand(rows.shape[:3] + (1,), generator=g) < 0.1, 0.0, rows * torch.exp2(e.float()))
+        cache = paged.quantize_kv_fp8(rows.to(torch.bfloat16))
+        setattr(c, name, cache)
+        setattr(c, {"cache": "rows", "ccache": "crows"}[name], paged.dequantize_kv_fp8(cache).view(-1, 576))
+    out, lse = _run(c)
+    c.check(out, lse)
