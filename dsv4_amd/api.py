@@ -871,7 +871,8 @@ def sparse_attn_sharedkv_tree(
     rows count from that position as ever (indices below ``(n + c) // cmp_ratio``;
     pass -1 for rows that hold tokens of another branch). Bits past a sequence's
     nodes, and of rows before position 0, are ignored; a token without any attends
-    the committed and compressed rows alone.
+    the committed and compressed rows alone, and nodes past ``64 W`` are attended
+    by none.
 
     The other arguments and the result are :func:`sparse_attn_sharedkv`'s; a chain
     (bits ``0 .. i`` of node ``i``) gives what that function gives, up to rounding where

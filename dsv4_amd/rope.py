@@ -118,6 +118,10 @@ def _table(table: Optional[torch.Tensor], positions: Optional[torch.Tensor], x: 
     else:
         if positions.device != x.device:
             raise ValueError("all tensors must be on one device")
+        if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype is torch.bool:
+            raise ValueError(f"positions must be integers, got {positions.dtype}")
+        if positions.dtype is torch.int64:   # (one past 32 bits stays outside the table)
+            positions = positions.clamp(-1, 2 ** 31 - 1)
         positions = _i32(positions)
     return table, table.shape[0], 2 * table.shape[1], positions
 

@@ -730,3 +730,24 @@ def test_gpu_scalars_in_tensors_are_read_anew():
     eps.fill_(1.0)
     n.fill_(64)
     assert torch.equal(norm_rope(q, eps=eps, q_norm_dim=n), norm_rope(q, eps=1.0, q_norm_dim=64))
+
+
+@pytest.mark.gpu
+def test_gpu_positions_past_32_bits_are_padding():
+    from dsv4_amd.cache import append_kv_cache
+    from dsv4_amd.rope import norm_rope, norm_rope_backward, rope_table
+    q = torch.randn(6, 16, 512, device="cuda").to(torch.bfloat16)
+    kv = q[:, 0].contiguous()
+    pos = torch.tensor([3, -1, 2 ** 32 + 3, -2 ** 63, 2 ** 63 - 1, -2 ** 32 + 3], device="cuda")
+    table = rope_table(8)
+    a = norm_rope(q, positions=pos, table=table)
+    assert torch.equal(a[0], norm_rope(q[:1], positions=pos[:1].int(), table=table)[0]) and bool((a[1:] == 0).all())
+    d = norm_rope_backward(q, q, positions=pos, table=table)[0]
+    assert bool((d[0] != 0).any()) and bool((d[1:] == 0).all())
+    cache = torch.zeros(1, 16, 1, 512, device="cuda", dtype=torch.bfloat16)
+    args = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0]], [0, 6], [6])]
+    assert torch.equal(append_kv_cache(kv, cache, *args, table=table, positions=pos, q=q), a)
+    assert bool((cache[0, 0] != 0).any()) and bool((cache[0, 1:] == 0).all())
+    for bad in (pos.float(), pos > 0):
+        with pytest.raises(ValueError, match="integers"):
+            norm_rope(q, positions=bad, table=table)

@@ -422,3 +422,20 @@ def test_gpu_pairs_fp8_rows_of_far_apart_scales():
         setattr(c, {"cache": "rows", "ccache": "crows"}[name], paged.dequantize_kv_fp8(cache).view(-1, 576))
     out, lse = _run(c)
     c.check(out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["swa", "scfa"])
+def test_gpu_empty_call_and_nodes_past_the_words(kind):
+    from dsv4_amd.api import sparse_attn_sharedkv_tree
+    c = Case(kind=kind, dt="bf16", H=64, D=512, ql=[80], kl=[200], K=64, reach=1)
+    kw = c.kwargs()
+    none = dict(kw, cu_seqlens_q=torch.zeros_like(kw["cu_seqlens_q"]))
+    if kind == "scfa":
+        none["cmp_sparse_indices"] = kw["cmp_sparse_indices"][:0]
+    out, lse = sparse_attn_sharedkv_tree(c.q.cuda()[:0], tree_mask=c.mask.cuda()[:0], return_softmax_lse=True, **none)
+    assert out.shape == (0, 64, 512) and lse.shape == (0, 64)
+    # one word: what the first 64 nodes of the chain are for the others
+    c.trees = [[[j for j in t if j < 64] for t in c.trees[0]]]
+    c.mask = c.mask[:, :1].contiguous()
+    c.check(*_run(c))
