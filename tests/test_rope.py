@@ -751,3 +751,42 @@ def test_gpu_positions_past_32_bits_are_padding():
     for bad in (pos.float(), pos > 0):
         with pytest.raises(ValueError, match="integers"):
             norm_rope(q, positions=bad, table=table)
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    """Rows, gradients, table and cache of more than 4 GiB: the last tokens are what
+    a call of their own gives."""
+    from dsv4_amd.cache import append_kv_cache
+    from dsv4_amd.rope import norm_rope, norm_rope_backward, rope_table
+    g = torch.Generator(device="cuda").manual_seed(5)
+    T, H, D, k = 60000, 64, 576, 50
+    table = rope_table(1 << 16)
+    q = torch.empty(T, H, D, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    assert q.numel() * 2 > 1 << 32
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    last = dict(positions=pos[-k:], table=table)
+    out = norm_rope(q, positions=pos, table=table)
+    assert torch.equal(out[-k:], norm_rope(q[-k:], **last))
+    d = norm_rope_backward(out, q, positions=pos, table=table)[0]
+    assert torch.equal(d[-k:], norm_rope_backward(out[-k:], q[-k:], **last)[0])
+    del out, d
+    # a table of 2^27 rows of 8 rotated channels
+    n = 1 << 27
+    wide = torch.zeros(n, 4, 2, device="cuda")
+    wide[-k:] = rope_table(k, 8)
+    far = dict(positions=torch.arange(n - k, n, device="cuda", dtype=torch.int32), table=wide)
+    near = dict(positions=torch.arange(k, device="cuda", dtype=torch.int32), table=rope_table(k, 8))
+    assert torch.equal(norm_rope(q[:k], **far), norm_rope(q[:k], **near))
+    del wide, far
+    kv = q[:k, 0].contiguous()
+    del q
+    for dt, row in ((torch.bfloat16, D), (torch.uint8, 656)):
+        blocks = (1 << 32) // (64 * row * dt.itemsize) + 2
+        cache = torch.zeros(blocks, 64, 1, row, device="cuda", dtype=dt)
+        small = torch.zeros(1, 64, 1, row, device="cuda", dtype=dt)
+        cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, k], [k]))
+        for c, b in ((cache, blocks - 1), (small, 0)):
+            append_kv_cache(kv, c, torch.tensor([[b]], dtype=torch.int32, device="cuda"), cu, used, table=table)
+        assert bool((small != 0).any()) and torch.equal(cache[-1], small[0])
+        del cache

@@ -439,3 +439,23 @@ def test_gpu_empty_call_and_nodes_past_the_words(kind):
     c.trees = [[[j for j in t if j < 64] for t in c.trees[0]]]
     c.mask = c.mask[:, :1].contiguous()
     c.check(*_run(c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp8"])
+@pytest.mark.parametrize("ql", [[3, 2], [140, 135]], ids=["few", "pairs"])
+def test_gpu_cache_past_32_bits(dt, ql):
+    """The rows of a small cache behind 4 GiB of others give the same bits."""
+    from dsv4_amd.api import sparse_attn_sharedkv_tree
+    c = Case(kind="scfa", dt=dt, H=64, D=576, ql=ql, kl=[q + 100 for q in ql], K=64)
+    want = _run(c)
+    kw = c.kwargs()
+    for name, table in (("ori_kv", "ori_block_table"), ("cmp_kv", "cmp_block_table")):
+        x = kw[name]
+        ahead = (1 << 32) // (x[0].numel() * x.element_size()) + 1
+        far = torch.zeros(ahead + x.shape[0], *x.shape[1:], dtype=x.dtype, device="cuda")
+        far[ahead:] = x
+        kw[name], kw[table] = far, torch.where(kw[table] >= 0, kw[table] + ahead, kw[table])
+    got = sparse_attn_sharedkv_tree(c.q.cuda(), tree_mask=c.mask.cuda(), return_softmax_lse=True, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    c.check(*got)
