@@ -832,11 +832,8 @@ def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, 
     return (out, lse) if return_softmax_lse else out
 
 
-def _geometry(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.dtype, t.get_device(), t.is_contiguous())
-
-
 TREE_WORDS_MAX = 64
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def sparse_attn_sharedkv_tree(
@@ -878,9 +875,8 @@ def sparse_attn_sharedkv_tree(
     (bits ``0 .. i`` of node ``i``) gives what that function gives, up to rounding where
     the two take different kernels.
     """
-    lead = tuple(q.shape[:-2])
-    if tree_mask.dtype is not torch.int64 or tree_mask.dim() != len(lead) + 1 or tuple(tree_mask.shape[:-1]) != lead or \
-            not 1 <= tree_mask.shape[-1] <= TREE_WORDS_MAX:
+    lead, at = q.shape[:-2], tree_mask.shape
+    if tree_mask.dtype is not torch.int64 or len(at) != len(lead) + 1 or at[:-1] != lead or not 1 <= at[-1] <= TREE_WORDS_MAX:
         raise ValueError(f"tree_mask must be int64 {[*lead, 'W']}, W from 1 to {TREE_WORDS_MAX}, got {tree_mask.dtype} "
                          f"{tuple(tree_mask.shape)}")
     if tree_mask.device != q.device:
@@ -890,11 +886,23 @@ def sparse_attn_sharedkv_tree(
     if cmp_kv is not None and cmp_sparse_indices is None and seqused_kv.numel():
         cfa_k = int(seqused_kv.max().item())
     # resolutions are kept as sparse_attn_sharedkv's are; they hold nothing of the mask
-    key = ("tree", _geometry(q), _geometry(ori_kv), _geometry(ori_block_table), _geometry(seqused_kv), _geometry(sinks),
-           _geometry(cu_seqlens_q), _geometry(cmp_kv), _geometry(cmp_block_table), _geometry(cmp_sparse_indices),
+    # (the tensors' geometries spelt out: ten helper calls cost 1.5 us)
+    key = ("tree", q.shape, q.dtype, q.get_device(), q.is_contiguous(),
+           ori_kv.shape, ori_kv.dtype, ori_kv.get_device(), ori_kv.is_contiguous(),
+           ori_block_table.shape, ori_block_table.dtype, ori_block_table.get_device(), ori_block_table.is_contiguous(),
+           seqused_kv.shape, seqused_kv.dtype, seqused_kv.get_device(), seqused_kv.is_contiguous(),
+           sinks.shape, sinks.dtype, sinks.get_device(), sinks.is_contiguous(),
+           None if cu_seqlens_q is None else
+           (cu_seqlens_q.shape, cu_seqlens_q.dtype, cu_seqlens_q.get_device(), cu_seqlens_q.is_contiguous()),
+           None if cmp_kv is None else (cmp_kv.shape, cmp_kv.dtype, cmp_kv.get_device(), cmp_kv.is_contiguous()),
+           None if cmp_block_table is None else
+           (cmp_block_table.shape, cmp_block_table.dtype, cmp_block_table.get_device(), cmp_block_table.is_contiguous()),
+           None if cmp_sparse_indices is None else
+           (cmp_sparse_indices.shape, cmp_sparse_indices.dtype, cmp_sparse_indices.get_device(),
+            cmp_sparse_indices.is_contiguous()),
            float(softmax_scale), cmp_ratio, ori_win_left, layout_q, cfa_k)
     dev = q.device
-    if q.is_cuda and dev.index != torch.cuda.current_device():
+    if q.is_cuda and dev.index != _device():
         with torch.cuda.device(dev):
             return sparse_attn_sharedkv_tree(
                 q, tree_mask=mask, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices,
