@@ -459,3 +459,36 @@ def test_gpu_cache_past_32_bits(dt, ql):
     got = sparse_attn_sharedkv_tree(c.q.cuda(), tree_mask=c.mask.cuda(), return_softmax_lse=True, **kw)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     c.check(*got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("scale", [-0.06, 0.0])
+def test_gpu_pairs_scales_of_other_signs(dt, scale):
+    c = Case(kind="scfa", dt=dt, H=64, D=576, ql=[45] * 6, kl=[45 + 60 * i for i in range(6)], K=64)
+    c.scale = scale
+    c.check(*_run(c))
+
+
+@pytest.mark.gpu
+def test_gpu_pairs_on_another_stream_captured():
+    """Replays on new inputs give what the eager call gives."""
+    from dsv4_amd.api import sparse_attn_sharedkv_tree
+    for dt in ("bf16", "fp8"):
+        c = Case(kind="scfa", dt=dt, H=64, D=576, ql=[45] * 6, kl=[45 + 60 * i for i in range(6)], K=64)
+        q, mask, kw = c.q.cuda(), c.mask.cuda(), c.kwargs()
+        eager = sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            assert torch.equal(sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw), eager)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw)
+        for _ in range(3):
+            q.copy_(torch.randn(q.shape, device="cuda"))
+            graph.replay()
+            got = captured.clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw))
