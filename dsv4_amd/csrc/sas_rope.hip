@@ -432,7 +432,7 @@ __device__ __forceinline__ void rope_rows(const RopeParams& p, const RopePart& a
 
 // Workgroups [0, part[0].blocks) take the KV rows (the longer chain of loads
 // starts first), the others the queries.
-// NT: the rows are read past the caches (appends never are)
+// NT: the rows are read past the caches
 template <typename QT, int NI, bool LAST, bool HALF, int DST, bool NT>
 __global__ void __launch_bounds__(kRopeThreads) sas_rope_kernel(const RopeParams p) {
   constexpr bool kAppend = DST != kToRows;
@@ -697,7 +697,8 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
   // channels: 2048 tokens 42 / 43 / 45, 103 / 103 / 113; 4096 94 / 80 / 88, 217 / 206 /
   // 215; 8192 187 / 181 / 173, 421 / 414 / 415. Smaller outputs are left for their
   // reader: written past the caches, 43 -> 38 us alone for 5300 tokens of 16 heads, but
-  // call and attention of 2048 tokens 103 -> 115.
+  // call and attention of 2048 tokens 103 -> 115. Appends with their queries, loads alone: 64
+  // heads of 512, 2000 / 3000 / 4096 tokens 42 -> 42, 71 -> 60, 94 -> 81; fp8 rows 48 -> 48, 82 -> 68, 111 -> 105.
   const double bytes = 2.0 * a->D * ((double)p->part[0].rows + p->part[1].rows);
   p->nt_load = 2 * bytes >= kInfinityCache;
   p->nt_store = bytes >= 2 * kInfinityCache;
@@ -729,12 +730,11 @@ int launch_rope(const SasNormRopeArgs* a, const RopeParams& p, hipStream_t st, c
     constexpr int NI = decltype(ni)::value;
     constexpr bool L = decltype(last)::value, HF = decltype(half)::value;
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(kRopeThreads), 0, st, p); };
-    const bool nt = DST == kToRows && p.nt_load;
     if (a->dtype == SAS_DT_BF16) {
-      if (nt) go(sas_rope_kernel<__bf16, NI, L, HF, DST, DST == kToRows>);
+      if (p.nt_load) go(sas_rope_kernel<__bf16, NI, L, HF, DST, true>);
       else go(sas_rope_kernel<__bf16, NI, L, HF, DST, false>);
     } else {
-      if (nt) go(sas_rope_kernel<_Float16, NI, L, HF, DST, DST == kToRows>);
+      if (p.nt_load) go(sas_rope_kernel<_Float16, NI, L, HF, DST, true>);
       else go(sas_rope_kernel<_Float16, NI, L, HF, DST, false>);
     }
     return launched(what);
@@ -893,12 +893,12 @@ extern "C" int sas_cache_append_v1(const SasCacheAppendArgs* a, void* stream) {
   const dim3 grid((unsigned)(p.part[0].blocks + p.part[1].blocks)), block(kRopeThreads);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, st, p); };
   const bool half = r->flags & SAS_ROPE_HALF;
-  if (r->rope_dim == 64 || r->rope_dim == 0) {
-    if (half) go(sas_rope_kernel<__bf16, 5, true, true, kToFp8, false>);
-    else go(sas_rope_kernel<__bf16, 5, true, false, kToFp8, false>);
-  } else {
-    if (half) go(sas_rope_kernel<__bf16, 5, false, true, kToFp8, false>);
-    else go(sas_rope_kernel<__bf16, 5, false, false, kToFp8, false>);
-  }
+  auto by_load = [&](auto last, auto hf) {
+    constexpr bool L = decltype(last)::value, HF = decltype(hf)::value;
+    if (p.nt_load) go(sas_rope_kernel<__bf16, 5, L, HF, kToFp8, true>);
+    else go(sas_rope_kernel<__bf16, 5, L, HF, kToFp8, false>);
+  };
+  if (r->rope_dim == 64 || r->rope_dim == 0) half ? by_load(std::true_type{}, std::true_type{}) : by_load(std::true_type{}, std::false_type{});
+  else half ? by_load(std::false_type{}, std::true_type{}) : by_load(std::false_type{}, std::false_type{});
   return launched("cache_append");
 }
