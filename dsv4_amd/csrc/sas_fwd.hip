@@ -2225,18 +2225,24 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 #if SAS_FWD_TREE
 // Whether a call takes the kernels of two workgroups a CU (sas_fwd_pair.h): all of a
 // token's slots in one workgroup, and
-//  - more (token, 64 heads) items than CUs: the other kernels need a second round; or
-//  - fp8 rows, whose other kernel takes 32 heads a workgroup, from half as many on: 160 to
-//    256 items of 256 / 640 rows 26-28 / 52-53 us against 31-32 / 53-55 (1152 rows: 86-87
-//    against 83-86, left there); or
-//  - a window that the exact schedule holds, from 32 items on (128 rows, 32 to 256 items of
-//    576 channels: 13.0-15.5 us against 14.4-17.5, fp8 16.8-19.2 against 17.7-34; 64 rows 10.9-12.4
-//    against 11.3-14.3; fewer items: the same within 4%).
+//  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows, 32
+//    to 256 items of 576 channels: 13.0-15.5 us against 14.4-17.5, fp8 16.8-19.2 against
+//    17.7-34; fewer items: the same within 4%); or
+//  - more workgroups of the other kernel than CUs, which hold one each (a second round).
+//    480 nodes, 128 + 1024 rows, 16 / 32 / 48 / 64 / 96 heads: 73 / 81 / 92 / 102 / 170 us against
+//    166 / 99 / 454 / 127 / 265 (heads that are no multiple of 32 leave it 16 a workgroup); 96
+//    nodes of 48 heads 51 against 143. With fp8 rows 97 / - / 113 / 123 / 223 against 110 / 89 /
+//    324 / 164 / 247; there the kernel of 32 heads a workgroup stays for 32 heads (it holds
+//    them all: 56 us against 64 at 640 rows), and for long rows of up to one item a CU (160 to
+//    256 items of 256 / 640 / 1152 rows 26-28 / 52-53 / 86-87 us against 31-32 / 53-55 / 83-86).
+//    (288 nodes of 96 heads, 1152 fp8 rows: 182 against 163, the one size found slower.)
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
-  if (a->H % 64 || pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
-  const long long items = a->T * (a->H / 64), cus = sas::device_cus();
+  if (pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
+  const long long items = a->T * ((a->H + 63) / 64), cus = sas::device_cus();
   if (pl.exact) return items >= 32;
-  return items > cus || (a->kv_dtype != a->q_dtype && 2 * items > cus && pl.nslots <= 640);
+  if (a->T * pl.nhg <= cus) return false;
+  if (a->kv_dtype != a->q_dtype && pl.hw == 2) return a->H > 32 && (items > cus || pl.nslots <= 640);
+  return true;
 }
 #endif
 
@@ -2322,7 +2328,7 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
   }
 #if SAS_FWD_TREE
   if (use_pairs(a, pl)) {
-    fp.nhg = (int)a->H / 64;
+    fp.nhg = (int)(a->H + 63) / 64;
     const long long nb = (a->T + fp.nxcd - 1) / fp.nxcd * fp.nhg * fp.nxcd;
     if (fp8) return launch_pair8(fp, (int)nb, st);
     if (a->q_dtype == SAS_DT_BF16) return a->D == 576 ? launch_pair<576, __bf16>(fp, (int)nb, st) : launch_pair<512, __bf16>(fp, (int)nb, st);

@@ -1,6 +1,6 @@
 // Draft trees of more (token, 64 heads) items than compute units, and windows of fewer
 // (use_pairs() has the rule): one item a workgroup of 4 waves, two workgroups on a CU,
-// MI355X (gfx950).
+// MI355X (gfx950). Where heads are no multiple of 64, waves without heads only move rows.
 //
 // The 8-wave kernel has a CU to itself: its ring fills the LDS, and nothing runs
 // beside a token's slot resolution, its first rows and its output (8 of 46 us at 640
@@ -109,7 +109,9 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   const int item = item_index<true>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
-  const int hq = k.hg * 64 + wave * 16;
+  // (heads past the last: a wave without heads only moves rows; its addresses stay valid)
+  const bool mine = k.hg * 64 + wave * 16 < p.H;
+  const int hq = mine ? k.hg * 64 + wave * 16 : p.H - 16;
   uint4 qf[KS];
   resolve<256, D * 2, true, true>(p, k, tid, lane, wave, [&] {
     const uint4* q = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq + c16) * D * 2) + g;
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
   float* lse = p.lse + (size_t)k.t * p.H + hq;
   const float sink2 = p.sinks[hq + c16] * kLog2e;
   if (n == 0) {
-    put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
+    if (mine) put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
     return;
   }
 
@@ -157,6 +159,18 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
 #pragma unroll
   for (int m = 0; m < RI; ++m) fire(m, lane);
   ++ps;
+  if (!mine) {   // wave-uniform; the same barriers as below
+    for (int st = 0; st < steps; ++st, ++ps) {
+      wait_vm<0>();
+      lds_barrier();
+      prep(lane);
+#pragma unroll
+      for (int m = 0; m < RI; ++m) fire(m, lane);
+    }
+    wait_vm<0>();
+    lds_barrier();
+    return;
+  }
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -265,7 +279,9 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
   const int item = item_index<true>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
-  const int hq = k.hg * 64 + wave * 16;
+  // (heads past the last: a wave without heads only moves rows; its addresses stay valid)
+  const bool mine = k.hg * 64 + wave * 16 < p.H;
+  const int hq = mine ? k.hg * 64 + wave * 16 : p.H - 16;
   uint4 qf[KS];
   resolve<256, kRow656, true, true>(p, k, tid, lane, wave, [&] {
     const uint4* q = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq + c16) * D * 2) + g;
@@ -277,7 +293,7 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
   float* lse = p.lse + (size_t)k.t * p.H + hq;
   const float sink2 = p.sinks[hq + c16] * kLog2e;
   if (n == 0) {
-    put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
+    if (mine) put_none(ob, lse, k.padded ? 0.f : sink2 * kLn2, lane);
     return;
   }
 
@@ -295,9 +311,46 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
     dma16(reinterpret_cast<const void*>(a),
           __builtin_amdgcn_readfirstlane(lds_addr_of(ring) + (uint32_t)(step & 1) * kPair8Slot + i * 1024));
   };
+  // my rows of the slot at sl, bf16, into the tile
+  auto convert = [&](uint32_t sl, int ln) {
+    const uint32_t src = sl + (uint32_t)(2 * wave * 512 + ln * 8), dst = lds_addr_of(tile) + (uint32_t)(2 * wave * 1024);
+    constexpr int kBatch = 4;
+#pragma unroll
+    for (int b0 = 0; b0 < 8; b0 += kBatch) {
+      u32x2 raw[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {   // row 2 wave + 8 (i / 2) + i % 2
+        const int e = b0 + i;
+        raw[i] = *reinterpret_cast<const LDS_AS u32x2*>((size_t)(src + (uint32_t)((e >> 1) * 8 + (e & 1)) * 512));
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int e = b0 + i;
+        uint4 b;
+        e4m3x4_to_bf16(raw[i].x, b.x, b.y);
+        e4m3x4_to_bf16(raw[i].y, b.z, b.w);
+        *reinterpret_cast<LDS_AS u32x4g*>((size_t)(dst + (uint32_t)((ln ^ swz<LCH>(2 * wave + (e & 1))) * 16) +
+                                                   (uint32_t)((e >> 1) * 8 + (e & 1)) * 1024)) = __builtin_bit_cast(u32x4g, b);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
 #pragma unroll
   for (int j = 0; j < 5; ++j) fire(0, j, lane);
   if (wave == 0) fire(0, 5, lane);
+  if (!mine) {   // wave-uniform; the same barriers as below (wave 0 always has heads)
+    for (int st = 0; st < steps; ++st) {
+      wait_vm<0>();
+      lds_barrier();
+      convert(lds_addr_of(ring) + (uint32_t)(st & 1) * kPair8Slot, lane);
+      lds_barrier();
+#pragma unroll
+      for (int j = 0; j < 5; ++j) fire(st + 1, j, lane);
+    }
+    wait_vm<0>();
+    lds_barrier();
+    return;
+  }
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -311,29 +364,7 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
     // (lane offsets made anew each step: kept, they spill, and a reload waits for the DMA)
     int ln = lane;
     asm volatile("" : "+v"(ln));
-    {
-      const uint32_t src = sl + (uint32_t)(2 * wave * 512 + ln * 8), dst = kt + (uint32_t)(2 * wave * 1024);
-      constexpr int kBatch = 4;
-#pragma unroll
-      for (int b0 = 0; b0 < 8; b0 += kBatch) {
-        u32x2 raw[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {   // row 2 wave + 8 (i / 2) + i % 2
-          const int e = b0 + i;
-          raw[i] = *reinterpret_cast<const LDS_AS u32x2*>((size_t)(src + (uint32_t)((e >> 1) * 8 + (e & 1)) * 512));
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int e = b0 + i;
-          uint4 b;
-          e4m3x4_to_bf16(raw[i].x, b.x, b.y);
-          e4m3x4_to_bf16(raw[i].y, b.z, b.w);
-          *reinterpret_cast<LDS_AS u32x4g*>((size_t)(dst + (uint32_t)((ln ^ swz<LCH>(2 * wave + (e & 1))) * 16) +
-                                                     (uint32_t)((e >> 1) * 8 + (e & 1)) * 1024)) = __builtin_bit_cast(u32x4g, b);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+    convert(sl, ln);
     lds_barrier();
     asm volatile("" ::: "memory");
     const int lc = ln & 15, lg = ln >> 4;

@@ -492,3 +492,25 @@ def test_gpu_pairs_on_another_stream_captured():
             got = captured.clone()
             torch.cuda.synchronize()
             assert torch.equal(got, sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw))
+
+
+# heads that do not fill a workgroup's four waves of sixteen
+PARTS = {
+    "h16": dict(kind="scfa", dt="bf16", H=16, D=576, ql=[90, 0, 100, 77], kl=[300, 9, 100, 700], K=100, tail=4, holes=True),
+    "h48_fp16": dict(kind="scfa", dt="fp16", H=48, D=512, ql=[150, 130], kl=[400, 131], K=90, bs=16),
+    "h96": dict(kind="cfa", dt="bf16", H=96, D=576, ql=[70, 65], kl=[400, 65], ratio=4, win=200),
+    "h80_window": dict(kind="swa", dt="bf16", H=80, D=512, ql=[20, 3], kl=[300, 3]),
+    "h16_window": dict(kind="swa", dt="fp16", H=16, D=576, ql=[33], kl=[90], win=100),
+    "h16_fp8": dict(kind="scfa", dt="fp8", H=16, D=576, ql=[140, 130], kl=[300, 131], K=100, tail=2, holes=True),
+    "h48_fp8": dict(kind="cfa", dt="fp8", H=48, D=576, ql=[140, 130], kl=[5, 700], ratio=8, win=60),
+    "h112_fp8_window": dict(kind="swa", dt="fp8", H=112, D=576, ql=[60, 5], kl=[60, 300], win=64),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(PARTS))
+def test_gpu_tree_heads_short_of_a_workgroup(name):
+    c = Case(**PARTS[name])
+    guard = _run(c)
+    c.check(*guard)
+    assert all(torch.equal(a, b) for a, b in zip(guard, _run(c)))
