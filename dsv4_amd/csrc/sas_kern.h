@@ -151,8 +151,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // lo = bytes 0-1, hi = bytes 2-3. gfx950's v_cvt_scalef32_pk_bf16_fp8
 // converts two OCP e4m3fn bytes (bias 7, subnormals m * 2^-9) straight to a
 // bf16 pair; with scale 1 the result is exact (every e4m3fn value is a bf16
-// value). 0x7f / 0xff (NaN) are never written by the cache writer, which
-// saturates at 448.
+// value). 0x7f / 0xff are NaN, which the writers leave where they are given one.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));

@@ -70,11 +70,13 @@ __device__ __forceinline__ float sum16(float x) {
   x += dpp<0x141>(x);
   return x + dpp<0x140>(x);
 }
+// of magnitudes, NaN above all of them: by their bits
 __device__ __forceinline__ float max16(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));
-  x = fmaxf(x, dpp<0x4E>(x));
-  x = fmaxf(x, dpp<0x141>(x));
-  return fmaxf(x, dpp<0x140>(x));
+  uint32_t u = __float_as_uint(x);
+  u = max(u, __float_as_uint(dpp<0xB1>(__uint_as_float(u))));
+  u = max(u, __float_as_uint(dpp<0x4E>(__uint_as_float(u))));
+  u = max(u, __float_as_uint(dpp<0x141>(__uint_as_float(u))));
+  return __uint_as_float(max(u, __float_as_uint(dpp<0x140>(__uint_as_float(u)))));
 }
 
 // v as a value of its own: what was computed from it before is not kept for later
@@ -299,12 +301,13 @@ enum { kToRows = 0, kToCache = 1, kToFp8 = 2 };
 
 // 128 latent channels x m, one iteration of the row's lanes, share a scale. (The
 // quotients by reciprocal: within an ulp of the true ones, which move a byte only
-// where its value lies that near a tie.)
+// where its value lies that near a tie.) A NaN stays one, with scale 1 for its group; an
+// infinity makes its group NaN, with a scale of infinity: as the codec of fp8 rows has it.
 __device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, const float (&x)[8], float m, bool write) {
   float amax = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
-  amax = max16(amax * m);
+  for (int k = 0; k < 8; ++k) amax = __builtin_elementwise_maximum(amax, fabsf(x[k]));   // (keeps a NaN)
+  amax = max16(fabsf(amax * m));
   const float scale = amax > 0.f ? amax * (1.f / kFp8Max) : 1.f;
   // (at most the largest float: zeros beside channels below 1e-36 stay zeros)
   const float inv = amax > 0.f ? fminf(kFp8Max * __builtin_amdgcn_rcpf(amax), 3.402823466e38f) : 1.f;
@@ -316,6 +319,13 @@ __device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, cons
     int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j]), cl(x[4 * j + 1]), 0, false);
     t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j + 2]), cl(x[4 * j + 3]), t, true);
     w[j] = (uint32_t)t;
+  }
+  if (!(amax < INFINITY)) {   // the clamp made -448 of each NaN: 0xfe
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float v = x[k] * q;
+      if (v != v) w[k / 4] |= 0x7fu << 8 * (k % 4);
+    }
   }
   if (!write) return;
   *reinterpret_cast<uint2*>(dst + 128 * g + 8 * sub) = make_uint2(w[0], w[1]);

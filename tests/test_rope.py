@@ -790,3 +790,93 @@ def test_gpu_offsets_past_32_bits():
             append_kv_cache(kv, c, torch.tensor([[b]], dtype=torch.int32, device="cuda"), cu, used, table=table)
         assert bool((small != 0).any()) and torch.equal(cache[-1], small[0])
         del cache
+
+
+# ---------------------------------------------------------------------------
+# fp8 appends of rows out of the ordinary
+# ---------------------------------------------------------------------------
+
+def _append_fp8(kv, n, rope_dim=0):
+    """The 656-byte rows that an append of kv [T, 576] (one sequence) leaves, on the CPU."""
+    from dsv4_amd.cache import append_kv_cache
+    T = kv.shape[0]
+    cache = torch.zeros(-(-T // 16), 16, 1, 656, dtype=torch.uint8, device="cuda")
+    table = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None]
+    cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, T], [T]))
+    rope = _table(T, rope_dim)
+    append_kv_cache(kv.cuda(), cache, table, cu, used, norm_dim=n, table=None if rope is None else rope.cuda())
+    return cache.view(-1, 656)[:T].cpu()
+
+
+def _check_fp8(rows, y, slack):
+    """rows against y [T, 576] in 64 bits, by 128-channel groups: the scale amax / 448 (1
+    where amax is 0 or NaN), each byte within half a step of its value, a NaN where the
+    value over the scale is one. `slack` [T, 1]: the fp32 error of y."""
+    lat = y[:, :512].unflatten(-1, (4, 128))
+    amax = lat.abs().amax(-1)                       # (torch's keeps a NaN)
+    scale = rows[:, 512:528].contiguous().view(torch.float32).double()
+    want = torch.where(amax > 0, amax / 448, 1.0)
+    inf = want.isinf()
+    assert torch.equal(scale.isinf(), inf)
+    # (half a step of the smallest floats below 2^-126)
+    assert bool(((scale - want).abs() <= 2.0 ** -16 * want + slack / 448 + 2.0 ** -150)[~inf].all())
+    # what the byte stands for: the value over the scale, clamped (scale 1 beside a NaN)
+    code = rows[:, :512].contiguous().view(torch.float8_e4m3fn).double().unflatten(-1, (4, 128))
+    val = (lat / want[..., None]).clamp(-448, 448)
+    assert torch.equal(code.isnan(), val.isnan())
+    bound = torch.maximum(val.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10, dtype=torch.float64)) * (1 + 2.0 ** -10)
+    bound = bound + slack[..., None] / scale[..., None]
+    assert bool(((code - val).abs() <= bound)[~val.isnan()].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rope_dim", [0, 32], ids=["plain", "rotated32"])
+@pytest.mark.parametrize("n", [0, 256, 512, 576])
+def test_gpu_append_fp8_keeps_nan_and_infinities(n, rope_dim):
+    """A channel that is NaN or infinite: the row is what the formulas and the codec
+    make of it, no finite value in its place; the rows beside it are as without it."""
+    g = torch.Generator().manual_seed(31)
+    clean = torch.randn(40, 576, generator=g).to(torch.bfloat16)
+    kv = clean.clone()
+    bad = {3: (5, NAN), 4: (300, float("inf")), 9: (511, -float("inf")), 10: (255, NAN), 11: (575, NAN), 17: (560, float("inf"))}
+    for r, (c, v) in bad.items():
+        kv[r, c] = v
+    kv[20, 130], kv[20, 140], kv[20, 400] = float("inf"), NAN, -NAN
+    kv[21, 0:512:3] = float("inf")
+    rows, want = _append_fp8(kv, n, rope_dim), _append_fp8(clean, n, rope_dim)
+    hit = torch.zeros(40, dtype=torch.bool)
+    hit[[*bad, 20, 21]] = True
+    assert torch.equal(rows[~hit], want[~hit])
+    y = R.norm_rope(kv, n, None, _table(40, rope_dim) if rope_dim else None)
+    big = y.abs().nan_to_num(0.0, 0.0, 0.0).amax(-1, keepdim=True)
+    _check_fp8(rows, y, 2.0 ** -16 * big)
+    tail = rows[:, 528:].contiguous().view(torch.bfloat16).double()
+    assert torch.equal(tail.isnan(), y[:, 512:].isnan()) and torch.equal(tail.isinf(), y[:, 512:].isinf())
+
+
+@pytest.mark.gpu
+def test_gpu_fp8_rows_of_nan_reach_the_attention():
+    """A token that attends an appended NaN row gives NaN, as over a bf16 cache; the
+    tokens before it, and the other sequence's, what they gave without it."""
+    from dsv4_amd.api import sparse_attn_sharedkv, sparse_attn_sharedkv_tree
+    from dsv4_amd.cache import append_kv_cache
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(16, 16, 576, generator=g).to(torch.bfloat16).cuda()
+    clean = torch.randn(16, 576, generator=g).to(torch.bfloat16)
+    kv = clean.clone()
+    kv[5, 17] = NAN
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 9, 16], [9, 7]))
+    mask = torch.tensor([(2 << i) - 1 for i in (*range(9), *range(7))], dtype=torch.int64, device="cuda")[:, None]
+    outs = []
+    for rows, row in ((clean, 656), (kv, 656), (kv, 576)):
+        cache = torch.zeros(2, 16, 1, row, dtype=torch.uint8 if row == 656 else torch.bfloat16, device="cuda")
+        append_kv_cache(rows.cuda(), cache, table, cu, used, norm_dim=512)
+        kw = dict(ori_kv=cache, ori_block_table=table, cu_seqlens_q=cu, seqused_kv=used, sinks=torch.zeros(16, device="cuda"),
+                  softmax_scale=0.04)
+        outs.append((sparse_attn_sharedkv(q, **kw), sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw)))
+    sees = torch.zeros(16, dtype=torch.bool)
+    sees[5:9] = True
+    for without, fp8, bf16 in zip(*outs):
+        assert bool(fp8[sees].isnan().all()) and bool(bf16[sees].isnan().all())
+        assert torch.equal(fp8[~sees], without[~sees])
