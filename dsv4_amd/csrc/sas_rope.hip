@@ -309,23 +309,26 @@ __device__ __forceinline__ void put_fp8_group(uint8_t* dst, int g, int sub, cons
   for (int k = 0; k < 8; ++k) amax = __builtin_elementwise_maximum(amax, fabsf(x[k]));   // (keeps a NaN)
   amax = max16(fabsf(amax * m));
   const float scale = amax > 0.f ? amax * (1.f / kFp8Max) : 1.f;
-  // (at most the largest float: zeros beside channels below 1e-36 stay zeros)
-  const float inv = amax > 0.f ? fminf(kFp8Max * __builtin_amdgcn_rcpf(amax), 3.402823466e38f) : 1.f;
-  const float q = m * inv;
+  const float q = amax > 0.f ? m * (kFp8Max * __builtin_amdgcn_rcpf(amax)) : m;
   uint32_t w[2];
+  auto pack = [&](auto&& value) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    auto cl = [&](float f) { return __builtin_amdgcn_fmed3f(f * q, -kFp8Max, kFp8Max); };
-    int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j]), cl(x[4 * j + 1]), 0, false);
-    t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(x[4 * j + 2]), cl(x[4 * j + 3]), t, true);
-    w[j] = (uint32_t)t;
-  }
-  if (!(amax < INFINITY)) {   // the clamp made -448 of each NaN: 0xfe
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float v = x[k] * q;
-      if (v != v) w[k / 4] |= 0x7fu << 8 * (k % 4);
+    for (int j = 0; j < 2; ++j) {
+      auto cl = [&](int k) { return __builtin_amdgcn_fmed3f(value(4 * j + k), -kFp8Max, kFp8Max); };
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(0), cl(1), 0, false);
+      w[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cl(2), cl(3), t, true);
     }
+  };
+  pack([&](int k) { return x[k] * q; });
+  // Not of finite factors: NaN and infinities, channels below 1e-33. These are raised by 2^64
+  // ahead of the quotient (q past the largest float made NaN of the zeros beside them).
+  if (!(amax < INFINITY && q < INFINITY)) {
+    const float s = amax < 1.f ? 0x1p64f : 1.f, inv = amax > 0.f ? kFp8Max * __builtin_amdgcn_rcpf(amax * s) : 1.f;
+    auto value = [&](int k) { return x[k] * m * s * inv; };
+    pack(value);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)   // (the clamp makes -448 of a NaN: 0xfe)
+      if (value(k) != value(k)) w[k / 4] |= 0x7fu << 8 * (k % 4);
   }
   if (!write) return;
   *reinterpret_cast<uint2*>(dst + 128 * g + 8 * sub) = make_uint2(w[0], w[1]);

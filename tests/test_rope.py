@@ -796,7 +796,7 @@ def test_gpu_offsets_past_32_bits():
 # fp8 appends of rows out of the ordinary
 # ---------------------------------------------------------------------------
 
-def _append_fp8(kv, n, rope_dim=0):
+def _append_fp8(kv, n, rope_dim=0, **kw):
     """The 656-byte rows that an append of kv [T, 576] (one sequence) leaves, on the CPU."""
     from dsv4_amd.cache import append_kv_cache
     T = kv.shape[0]
@@ -804,7 +804,7 @@ def _append_fp8(kv, n, rope_dim=0):
     table = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None]
     cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, T], [T]))
     rope = _table(T, rope_dim)
-    append_kv_cache(kv.cuda(), cache, table, cu, used, norm_dim=n, table=None if rope is None else rope.cuda())
+    append_kv_cache(kv.cuda(), cache, table, cu, used, norm_dim=n, table=None if rope is None else rope.cuda(), **kw)
     return cache.view(-1, 656)[:T].cpu()
 
 
@@ -880,3 +880,26 @@ def test_gpu_fp8_rows_of_nan_reach_the_attention():
     for without, fp8, bf16 in zip(*outs):
         assert bool(fp8[sees].isnan().all()) and bool(bf16[sees].isnan().all())
         assert torch.equal(fp8[~sees], without[~sees])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rope_dim", [0, 32], ids=["plain", "rotated32"])
+@pytest.mark.parametrize("n,eps", [(0, 0.0), (512, 1e-6), (512, 1e-12)])
+def test_gpu_append_fp8_groups_of_tiny_channels(n, eps, rope_dim):
+    """Groups whose channels lie below 1e-34 down to the smallest bf16 values, zeros among
+    them: 448 over their maximum, times the norm's factor, is past the largest float."""
+    g = torch.Generator().manual_seed(33)
+    kv = torch.randn(24, 576, generator=g)
+    zero = torch.rand(24, 512, generator=g) < 0.3
+    kv[:, :512] = torch.where(zero, 0.0, kv[:, :512] * 10.0 ** -torch.linspace(33, 40.4, 24)[:, None])
+    kv[::4, 128:256] = 0.0
+    kv[5, 256:384] = 0.0
+    kv[5, 300] = -1e-40                              # one channel, the others zeros
+    kv = kv.to(torch.bfloat16)
+    rows = _append_fp8(kv, n, rope_dim, eps=eps)
+    y = R.norm_rope(kv, n, None, _table(24, rope_dim) if rope_dim else None, eps=eps)
+    # by groups: each is of its own magnitude; fp32 values below 2^-126 have steps of 2^-149
+    big = y[:, :512].unflatten(-1, (4, 128)).abs().amax(-1)
+    _check_fp8(rows, y, 2.0 ** -16 * big + 2.0 ** -149 * (n > 0))
+    zeros = rows[:, :512][kv[:, :512] == 0]
+    assert bool(((zeros == 0) | (zeros == 0x80)).all())
