@@ -129,15 +129,20 @@ __device__ __forceinline__ void put_fp8_row(uint8_t* dst, const uint4& w, const 
   // (the same bytes as torch's float8_e4m3fn conversion for every bf16
   // input; 2x faster here than a bit-level encoder)
   uint32_t q[2];
+  auto pack = [&](auto&& value) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    int t = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(x[4 * h] * inv, -kE4m3Max, kE4m3Max),
-                                            __builtin_amdgcn_fmed3f(x[4 * h + 1] * inv, -kE4m3Max, kE4m3Max),
-                                            0, false);
-    t = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(x[4 * h + 2] * inv, -kE4m3Max, kE4m3Max),
-                                        __builtin_amdgcn_fmed3f(x[4 * h + 3] * inv, -kE4m3Max, kE4m3Max),
-                                        t, true);
-    q[h] = (uint32_t)t;
+    for (int h = 0; h < 2; ++h) {
+      auto cl = [&](int k) { return __builtin_amdgcn_fmed3f(value(4 * h + k), -kE4m3Max, kE4m3Max); };
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(cl(0), cl(1), 0, false);
+      q[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(cl(2), cl(3), t, true);
+    }
+  };
+  pack([&](int k) { return x[k] * inv; });
+  // Below 1e-36 inv is infinite, and the zeros beside such channels x inv NaN: the group
+  // is raised by 2^64 (exact) ahead of the quotient.
+  if (!(inv < INFINITY)) {
+    const float up = 0x1p64f, inv2 = kE4m3Max / (amax * up);
+    pack([&](int k) { return x[k] * up * inv2; });
   }
   *reinterpret_cast<uint2*>(dst + lane * 8) = make_uint2(q[0], q[1]);
   if ((lane & 15) == 0) *reinterpret_cast<float*>(dst + kScaleOff + (lane >> 4) * 4) = scale;

@@ -281,7 +281,8 @@ def quantize_kv_fp8(kv: torch.Tensor) -> torch.Tensor:
     ``byte = e4m3fn(clamp(x * inv, -448, 448))`` with ``inv = 448 / amax``
     (both 1 for an all-zero group), rounded to nearest even: one division per
     group, a multiply per value (the device writer computes the same fp32
-    products, so both write the same bytes).
+    products, so both write the same bytes). Groups below 1 are raised by 2^64
+    ahead of it, which changes no byte but keeps ``inv`` finite for the smallest.
     """
     if kv.shape[-1] != FP8_LATENT + FP8_ROPE:
         raise ValueError(f"fp8 rows need 576 channels, got {kv.shape[-1]}")
@@ -293,9 +294,10 @@ def quantize_kv_fp8(kv: torch.Tensor) -> torch.Tensor:
     scale = torch.where(nz, amax / E4M3_MAX, torch.ones_like(amax))
     # a tensor / tensor division (correctly rounded, as on the device); torch
     # evaluates `scalar / tensor` as reciprocal(tensor) * scalar
-    inv = torch.where(nz, torch.full_like(amax, E4M3_MAX).div(torch.where(nz, amax, torch.ones_like(amax))),
+    up = torch.where(amax < 1, 2.0 ** 64, 1.0).to(amax)
+    inv = torch.where(nz, torch.full_like(amax, E4M3_MAX).div(torch.where(nz, amax * up, torch.ones_like(amax))),
                       torch.ones_like(amax))
-    q8 = (lat * inv.unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    q8 = (lat * up.unsqueeze(-1) * inv.unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     rows = torch.empty((x.shape[0], FP8_ROW_BYTES), dtype=torch.uint8, device=kv.device)
     rows[:, :FP8_LATENT] = q8.reshape(-1, FP8_LATENT).view(torch.uint8)
     rows[:, FP8_SCALE_OFF:FP8_ROPE_OFF] = scale.contiguous().view(torch.uint8).reshape(-1, 16)

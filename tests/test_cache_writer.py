@@ -225,3 +225,60 @@ def test_gpu_cache_write_int64_indices_on_a_side_stream():
     torch.cuda.synchronize()
     del junk
     assert torch.equal(d.cpu(), ref), f"{int((d.cpu() != ref).sum())} bytes differ"
+
+
+# ---------------------------------------------------------------------------
+# rows out of the ordinary
+# ---------------------------------------------------------------------------
+
+def _tiny_rows():
+    """Groups from 1e-33 down to the smallest bf16 value, zeros among their channels."""
+    g = torch.Generator().manual_seed(13)
+    kv = torch.randn(40, 576, generator=g)
+    zero = torch.rand(40, 512, generator=g) < 0.3
+    kv[:, :512] = torch.where(zero, 0.0, kv[:, :512] * 10.0 ** -torch.linspace(33, 40.4, 40)[:, None])
+    kv[::4, 128:256] = 0.0
+    kv[5, 256:384] = 0.0
+    kv[5, 300] = -1e-40                                # one channel, the others zeros
+    return kv.to(torch.bfloat16)
+
+
+def _check_rows(rows, kv):
+    """rows against kv in 64 bits: scale = amax / 448 within half a float (2^-24 of it, or
+    2^-150 below 2^-126), every byte within half a step of the value over it (2^-4 of
+    the value, or 2^-10 below 2^-6; 2^-20 more for the product's two roundings)."""
+    lat = kv[:, :512].double().reshape(-1, 4, 128)
+    amax = lat.abs().amax(-1)
+    want = torch.where(amax > 0, amax / 448.0, 1.0)
+    scale = rows[:, 512:528].contiguous().view(torch.float32).double()
+    assert bool(((scale - want).abs() <= 2.0 ** -24 * want + 2.0 ** -150).all())
+    code = rows[:, :512].contiguous().view(torch.float8_e4m3fn).double().reshape(-1, 4, 128)
+    val = lat / want[..., None]
+    bound = torch.where(val.abs() >= 2.0 ** -6, val.abs() * 2.0 ** -4, torch.full_like(val, 2.0 ** -10)) * (1 + 2.0 ** -20)
+    assert bool(((code - val).abs() <= bound).all())
+
+
+def test_codec_groups_of_tiny_channels():
+    kv = _tiny_rows()
+    _check_rows(paged.quantize_kv_fp8(kv), kv)
+    # the same bytes as ever where 448 / amax is a float
+    g = torch.Generator().manual_seed(14)
+    rows = (torch.randn(200, 576, generator=g) * torch.logspace(-35.5, 36, 200).unsqueeze(1)).to(torch.bfloat16)
+    assert torch.equal(paged.quantize_kv_fp8(rows), torch.stack([R.quantize_row_fp8(r) for r in rows]))
+
+
+def _write(kv):
+    from dsv4_amd.cache import write_kv_cache
+    n = kv.shape[0]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cache = torch.zeros(n, 1, 1, 656, dtype=torch.uint8, device="cuda")
+    write_kv_cache(kv.cuda(), cache, torch.arange(n, **i32)[:, None], torch.arange(n, **i32), torch.zeros(n, **i32))
+    return cache.view(n, 656).cpu()
+
+
+@pytest.mark.gpu
+def test_gpu_cache_write_groups_of_tiny_channels():
+    kv = _tiny_rows()
+    rows = _write(kv)
+    _check_rows(rows, kv)
+    assert torch.equal(rows, paged.quantize_kv_fp8(kv))
