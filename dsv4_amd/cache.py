@@ -176,7 +176,7 @@ def append_kv_cache(
     ``cache`` is ``[num_blocks, block_size, 1, D]`` in ``kv``'s dtype, or uint8
     ``[num_blocks, block_size, 1, 656]`` (bf16 ``kv`` with D = 576), quantised from
     the fp32 values (NaN and infinities as :func:`dsv4_amd.paged.quantize_kv_fp8`
-    has them: no finite value in their place). Tokens behind the last sequence, at
+    has them: a group with one holds a NaN). Tokens behind the last sequence, at
     a negative position or at one outside ``table`` are padding: nothing of the
     cache is written for them and their queries come back as zeros; rows without a
     block are skipped, as by :func:`write_kv_cache`. The rows of one call must go

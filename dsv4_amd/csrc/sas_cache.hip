@@ -120,9 +120,9 @@ __device__ __forceinline__ void put_fp8_row(uint8_t* dst, const uint4& w, const 
                       bf16_lo(w.z), bf16_hi(w.z), bf16_lo(w.w), bf16_hi(w.w)};
   float amax = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
+  for (int k = 0; k < 8; ++k) amax = __builtin_elementwise_maximum(amax, fabsf(x[k]));   // (keeps a NaN)
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  for (int o = 8; o >= 1; o >>= 1) amax = __builtin_elementwise_maximum(amax, __shfl_xor(amax, o));
   const float scale = amax > 0.f ? amax / kE4m3Max : 1.f;
   const float inv = amax > 0.f ? kE4m3Max / amax : 1.f;
   // v_cvt_pk_fp8_f32: two floats -> two OCP e4m3fn bytes, nearest even
@@ -138,11 +138,17 @@ __device__ __forceinline__ void put_fp8_row(uint8_t* dst, const uint4& w, const 
     }
   };
   pack([&](int k) { return x[k] * inv; });
-  // Below 1e-36 inv is infinite, and the zeros beside such channels x inv NaN: the group
-  // is raised by 2^64 (exact) ahead of the quotient.
-  if (!(inv < INFINITY)) {
-    const float up = 0x1p64f, inv2 = kE4m3Max / (amax * up);
-    pack([&](int k) { return x[k] * up * inv2; });
+  // Not of finite factors. Below 1e-36 inv is infinite, and the zeros beside such channels
+  // x inv NaN: the group is raised by 2^64 (exact) ahead of the quotient. A NaN stays
+  // one (the clamp makes -448 of it, 0xfe), with scale 1 for its group; an infinity is NaN
+  // under its group's scale of infinity.
+  if (!(amax < INFINITY && inv < INFINITY)) {
+    const float up = amax < 1.f ? 0x1p64f : 1.f, inv2 = amax > 0.f ? kE4m3Max / (amax * up) : 1.f;
+    auto value = [&](int k) { return x[k] * up * inv2; };
+    pack(value);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (value(k) != value(k)) q[k / 4] |= 0x7fu << 8 * (k % 4);
   }
   *reinterpret_cast<uint2*>(dst + lane * 8) = make_uint2(q[0], q[1]);
   if ((lane & 15) == 0) *reinterpret_cast<float*>(dst + kScaleOff + (lane >> 4) * 4) = scale;

@@ -282,3 +282,33 @@ def test_gpu_cache_write_groups_of_tiny_channels():
     rows = _write(kv)
     _check_rows(rows, kv)
     assert torch.equal(rows, paged.quantize_kv_fp8(kv))
+
+
+@pytest.mark.gpu
+def test_gpu_cache_write_keeps_nan_and_infinities():
+    """The codec's bytes (those of NaN apart: they have many): a NaN channel stays one, an infinite one
+    makes its group NaN by its scale; the rows and groups beside them are as ever."""
+    g = torch.Generator().manual_seed(15)
+    kv = torch.randn(30, 576, generator=g).to(torch.bfloat16)
+    nan, inf = float("nan"), float("inf")
+    for r, c, v in ((1, 0, nan), (2, 127, inf), (3, 128, -inf), (4, 511, -nan), (5, 575, nan), (6, 512, inf)):
+        kv[r, c] = v
+    kv[7, 130], kv[7, 140], kv[7, 400] = inf, nan, nan
+    kv[8, :512] = nan
+    kv[9, :512] = inf
+    kv[10, :128], kv[10, 3] = 0.0, nan
+    kv[11, :128], kv[11, 3] = 1e-39, inf
+    kv[12, :128], kv[12, 3] = 1e5, nan                 # beside a NaN the scale is 1: 448
+    rows, want = _write(kv), paged.quantize_kv_fp8(kv)
+    lat = want[:, :512].view(torch.float8_e4m3fn)
+    assert int(lat.isnan().sum()) > 1000 and torch.equal(rows[:, :512].view(torch.float8_e4m3fn).isnan(), lat.isnan())
+    tail = kv[:, 512:].isnan().repeat_interleave(2, 1)
+    assert torch.equal(rows[:, 528:].contiguous().view(torch.bfloat16).isnan(), kv[:, 512:].isnan())
+    same = ~torch.cat([lat.isnan(), torch.zeros(30, 16, dtype=torch.bool), tail], 1)
+    assert torch.equal(rows[same], want[same])
+    deq = paged.dequantize_kv_fp8(rows)
+    x, deq = kv[:, :512].float().reshape(30, 4, 128), deq[:, :512].reshape(30, 4, 128)
+    bad, nans = ~x.isfinite(), x.isnan()
+    # (an infinity beside a NaN is clamped, as the scale is 1: the group has its NaN)
+    assert bool(deq[nans | (bad & ~nans.any(-1, keepdim=True))].isnan().all())
+    assert bool(deq[~bad.any(-1)].isfinite().all())
