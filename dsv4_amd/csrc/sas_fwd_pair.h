@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
     for (int st = 0; st < steps; ++st, ++ps) {
       wait_vm<0>();
       lds_barrier();
+      asm volatile("" ::: "memory");   // (the barrier's builtins alone hold no memory access back)
       prep(lane);
 #pragma unroll
       for (int m = 0; m < RI; ++m) fire(m, lane);
@@ -342,8 +343,10 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
     for (int st = 0; st < steps; ++st) {
       wait_vm<0>();
       lds_barrier();
+      asm volatile("" ::: "memory");
       convert(lds_addr_of(ring) + (uint32_t)(st & 1) * kPair8Slot, lane);
       lds_barrier();
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int j = 0; j < 5; ++j) fire(st + 1, j, lane);
     }
