@@ -903,3 +903,87 @@ def test_gpu_append_fp8_groups_of_tiny_channels(n, eps, rope_dim):
     _check_fp8(rows, y, 2.0 ** -16 * big + 2.0 ** -149 * (n > 0))
     zeros = rows[:, :512][kv[:, :512] == 0]
     assert bool(((zeros == 0) | (zeros == 0x80)).all())
+
+
+# ---------------------------------------------------------------------------
+# calls past the caches: rows read (and written) non-temporally, by builds and
+# branches of their own
+# ---------------------------------------------------------------------------
+
+def _randn(shape, dt, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, device="cuda", dtype=dt).normal_(generator=g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,fp8,D,rope_dim,half", [
+    ("bf16", False, 512, 64, False), ("fp16", False, 576, 64, True), ("bf16", True, 576, 64, False),
+    ("bf16", True, 576, 32, True), ("fp16", False, 640, 32, False)])
+def test_gpu_append_past_the_caches(dt, fp8, D, rope_dim, half):
+    """2501 tokens of 64 heads, more than 128 MB of rows: the same bits as the same
+    tokens in steps of 400."""
+    from dsv4_amd.cache import append_kv_cache
+    from dsv4_amd.rope import rope_table
+    T, H, bs, step = 2501, 64, 64, 400
+    assert T * (H + 1) * D * 4 >= 256e6 > step * (H + 1) * D * 4
+    q, kv = _randn((T, H, D), DT[dt], 41), _randn((T, D), DT[dt], 42)
+    w = 1 + 0.2 * torch.randn(D, device="cuda")
+    blocks = -(-T // bs)
+    table = torch.randperm(blocks + 2, device="cuda")[:blocks].to(torch.int32)[None]
+    kw = dict(table=rope_table(T, rope_dim), norm_dim=512, weight=w[:512], interleaved=not half, q_norm_dim=D, q_weight=w)
+    row = dict(device="cuda", dtype=torch.uint8 if fp8 else DT[dt])
+
+    def append(cache, a, b):
+        cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, b - a], [b]))
+        return append_kv_cache(kv[a:b], cache, table, cu, used, q=q[a:b], **kw)
+
+    one = torch.zeros(blocks + 2, bs, 1, 656 if fp8 else D, **row)
+    many = torch.zeros_like(one)
+    got = append(one, 0, T)
+    want = torch.cat([append(many, a, min(a + step, T)) for a in range(0, T, step)])
+    assert torch.equal(got, want) and torch.equal(one, many) and bool((one != 0).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,rope_dim,half,T", [
+    ("fp16", 576, 64, True, 2501), ("fp16", 512, 64, False, 8001), ("bf16", 576, 64, True, 7001), ("bf16", 640, 32, False, 2501),
+    ("fp16", 128, 64, True, 16001)])
+def test_gpu_forward_past_the_caches(dt, D, rope_dim, half, T):
+    """The same bits as the tokens in calls that stay within them; 512 MB and more are
+    written past the caches too."""
+    from dsv4_amd.rope import norm_rope, rope_table
+    H, step = 64, 800
+    assert T * (H + 1) * D * 4 >= 256e6 > step * (H + 1) * D * 4
+    q, kv = _randn((T, H, D), DT[dt], 43), _randn((T, D), DT[dt], 44)
+    w = 1 + 0.2 * torch.randn(D, device="cuda")
+    pos, table = torch.randint(-1, 5001, (T,), device="cuda", dtype=torch.int32), rope_table(5000, rope_dim)
+    kw = dict(table=table, q_norm_dim=512 if D > 512 else D, kv_norm_dim=D, kv_weight=w, interleaved=not half)
+    got = norm_rope(q, kv, positions=pos, **kw)
+    for a in range(0, T, step):
+        part = norm_rope(q[a:a + step], kv[a:a + step], positions=pos[a:a + step], **kw)
+        assert all(torch.equal(x[a:a + step], y) for x, y in zip(got, part))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,rope_dim,half", [("bf16", 512, 64, False), ("fp16", 576, 64, True), ("bf16", 640, 32, True)])
+def test_gpu_backward_past_the_caches(dt, D, rope_dim, half):
+    """Rows' gradients as in calls of 200 tokens; weights' against 64 bits: chains of 8 rows
+    a lane, 6 adds over the workgroup's, 12 and 64 over the workgroups: 90 e < 2^-17, and
+    2^-17 of each term."""
+    from dsv4_amd.rope import norm_rope_backward, rope_table
+    T, H, step = 1501, 64, 200
+    assert T * (H + 1) * D * 6 >= 256e6 > step * (H + 1) * D * 6
+    q, kv = _randn((T, H, D), DT[dt], 45), _randn((T, D), DT[dt], 46)
+    gq, gk = _randn((T, H, D), DT[dt], 47), _randn((T, D), DT[dt], 48)
+    w = 1 + 0.2 * torch.randn(D, device="cuda")
+    pos, table = torch.randint(0, 5000, (T,), device="cuda", dtype=torch.int32), rope_table(5000, rope_dim)
+    kw = dict(table=table, q_norm_dim=512, q_weight=w[:512], kv_weight=w, interleaved=not half)
+    dq, dkv, dqw, dkw = norm_rope_backward(gq, q, gk, kv, positions=pos, **kw)
+    for a in range(0, T, step):
+        s = slice(a, a + step)
+        part = norm_rope_backward(gq[s], q[s], gk[s], kv[s], positions=pos[s], **kw)
+        assert torch.equal(dq[s], part[0]) and torch.equal(dkv[s], part[1])
+    cs = table[pos.long()]
+    for dw, dy, x, n, c in ((dqw, gq, q, 512, cs[:, None]), (dkw, gk, kv, D, cs)):
+        _, want, total = R.norm_rope_grad(dy, x, n, w[:n], c, half)
+        assert bool(((dw.double() - want).abs() <= 2.0 ** -16 * total).all())
