@@ -825,7 +825,7 @@ def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, 
         else:
             rc = _tree_bytes()(packed + _TREE.pack(tree_mask.data_ptr(), tree_mask.shape[-1]), stream)
         if rc:
-            _lib.check(rc, "sparse_attn_sharedkv")
+            _lib.check(rc, "sparse_attn_sharedkv" if tree_mask is None else "sparse_attn_sharedkv_tree")
     finally:
         if staged is not None:
             ring.release(staged[1], stream)

@@ -116,6 +116,20 @@ def test_python_refuses():
         sparse_attn_sharedkv_tree(q, tree_mask=torch.zeros(3, 1, dtype=torch.int64), **kw)
 
 
+def test_failed_call_of_a_kept_resolution_is_named(monkeypatch):
+    from dsv4_amd import api
+    r = api._Cached.__new__(api._Cached)
+    r.out_shape, r.lse_shape, r.tail, r.ws_bytes, r.host_names = (1, 16, 512), (1, 16), b"", 0, []
+    monkeypatch.setattr(api, "_tree_raw", lambda packed, stream: _lib.SAS_EINVAL)
+    monkeypatch.setattr(api, "_fwd_raw", lambda packed, stream: _lib.SAS_EINVAL)
+    t = torch.zeros(1, dtype=torch.int32)
+    args = (r, None, t.device, t, t, None, None, t, None, t, t, torch.zeros(16), False)
+    with pytest.raises(ValueError, match="^sparse_attn_sharedkv_tree"):
+        api._run_cached(*args, torch.zeros(1, 1, dtype=torch.int64))
+    with pytest.raises(ValueError, match="^sparse_attn_sharedkv[^_]"):
+        api._run_cached(*args)
+
+
 # ---------------------------------------------------------------------------
 # GPU
 # ---------------------------------------------------------------------------
