@@ -664,7 +664,9 @@ int check_rope(const SasNormRopeArgs* a, const char* what) {
   if (!(a->eps >= 0.f)) return set_error(SAS_EINVAL, "%s: eps must not be negative", what);
   // (a launch has fewer than 2^32 threads, sixteen of them a row)
   const double rows = (double)a->T * ((double)a->H + (a->kv ? 1 : 0));
-  if (rows > kMostRows) return set_error(SAS_EINVAL, "%s: more than 2^%d rows", what, rows >= 2147483648.0 ? 31 : 28);
+  if (rows > kMostRows)
+    return set_error(SAS_EINVAL, "%s: %s rows, a call takes at most 2^28 - %d", what,
+                     rows >= 2147483648.0 ? "2^31 or more" : "too many", 2 * kRopeRows);
   if (a->T == 0) return SAS_OK;
   if ((a->H > 0) != (a->q != nullptr)) return set_error(SAS_EINVAL, "%s: q and H go together", what);
   if (!a->q && !a->kv) return set_error(SAS_EINVAL, "%s: null device pointer", what);

@@ -338,8 +338,8 @@ int sas_cache_write_v1(const SasCacheWriteArgs* a, void* stream);
  * [0, table_rows) is padding: its output rows are zeros.
  * D a multiple of 8 in [8, 1024], rope_dim a multiple of 8 (SAS_ROPE_HALF: 16)
  * in [0, D], norm dims multiples of 8 in [0, D] (0: no norm); strides multiples
- * of 8 elements, every tensor 16-byte aligned, fewer than 2^28 rows in all. Outputs
- * must not overlap inputs.
+ * of 8 elements, every tensor 16-byte aligned, at most 2^28 - 32 rows in all.
+ * Outputs must not overlap inputs.
  */
 typedef struct SasNormRopeArgs {
   const void* q;                 /* [T, H, D], or NULL with H = 0 */

@@ -987,3 +987,14 @@ def test_gpu_backward_past_the_caches(dt, D, rope_dim, half):
     for dw, dy, x, n, c in ((dqw, gq, q, 512, cs[:, None]), (dkw, gk, kv, D, cs)):
         _, want, total = R.norm_rope_grad(dy, x, n, w[:n], c, half)
         assert bool(((dw.double() - want).abs() <= 2.0 ** -16 * total).all())
+
+
+def test_abi_names_the_most_rows_of_a_call():
+    L = _lib.lib()
+    n = C.c_size_t(0)
+    for T, ok in (((1 << 28) - 32, True), ((1 << 28) - 31, False), (1 << 28, False), (1 << 31, False), (1 << 40, False)):
+        a = _args(T=T, H=0, q=None, q_out=None, D=8, kv_stride_t=8, rope_dim=0, kv_norm_dim=8, q_norm_dim=0)
+        rc = L.sas_norm_rope_bwd_plan(C.byref(_lib.SasNormRopeBwdArgs(fwd=a)), C.byref(n))   # (launches nothing)
+        assert rc == (_lib.SAS_OK if ok else _lib.SAS_EINVAL)
+        if not ok:
+            assert "at most 2^28 - 32" in L.sas_last_error().decode()
