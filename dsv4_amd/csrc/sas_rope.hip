@@ -46,7 +46,7 @@ struct RopeParams {
   const int32_t* pos;          // [T]; any readable address where there are none
   int has_pos;                 // 0: none (append: the cache positions)
   const float* table;          // [table_rows, R / 2, 2]
-  int table_rows, D, R, T;
+  int table_rows, D, R;
   int wf32;                    // weights are fp32 (else the rows' type)
   float eps, sign;             // sign of the rotation
   int nt_load, nt_store;       // rows are read / written non-temporally
@@ -229,9 +229,6 @@ struct Row {
   }
   __device__ __forceinline__ int partner(int c) const { return c - rc0 < hc ? c + hc : c - hc; }
 
-  __device__ __forceinline__ static uint4 ld(const uint8_t* x, int c) {
-    return gld16(reinterpret_cast<uint64_t>(x) + 16u * (uint32_t)c);
-  }
   // every lane loads; chunks past the row's (normed: past its normed ones, whose
   // lines are then not fetched) are clamped to the last of them
   template <bool NT>
@@ -687,7 +684,7 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
   p->pos = p->has_pos ? a->positions : (const int32_t*)(a->kv ? a->kv : a->q);
   p->table = a->table;
   p->table_rows = (int)a->table_rows;
-  p->D = (int)a->D; p->R = a->rope_dim; p->T = (int)a->T;
+  p->D = (int)a->D; p->R = a->rope_dim;
   p->wf32 = a->weight_dtype == SAS_DT_FP32;
   p->eps = a->eps;
   p->sign = a->flags & SAS_ROPE_INVERSE ? -1.f : 1.f;
