@@ -865,11 +865,14 @@ def sparse_attn_sharedkv_tree(
     node ``j`` of its sequence, one bit for each of its ancestors and one for itself.
     With ``c`` bits set the token stands at position ``n + c - 1``: its window is the last
     ``ori_win_left + 1`` of the committed rows and its attended nodes, and compressed
-    rows count from that position as ever (indices below ``(n + c) // cmp_ratio``;
-    pass -1 for rows that hold tokens of another branch). Bits past a sequence's
-    nodes, and of rows before position 0, are ignored; a token without any attends
-    the committed and compressed rows alone, and nodes past ``64 W`` are attended
-    by none.
+    rows count from that position as ever, those below ``(n + c) // cmp_ratio``. Rows
+    from ``n // cmp_ratio`` on cover draft positions, and each is one row for all
+    branches. With ``cmp_sparse_indices`` pass -1 where such a row holds tokens of
+    another branch. The dense form attends them all: it is for trees that stay below
+    the next multiple of ``cmp_ratio`` (or whose branches share what lies beyond);
+    for others list the rows as indices. Bits past a sequence's nodes, and of rows
+    before position 0, are ignored; a token without any attends the committed and
+    compressed rows alone, and nodes past ``64 W`` are attended by none.
 
     The other arguments and the result are :func:`sparse_attn_sharedkv`'s; a chain
     (bits ``0 .. i`` of node ``i``) gives what that function gives, up to rounding where

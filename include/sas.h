@@ -202,7 +202,11 @@ int sas_fwd_v1(const SasFwdArgs* a, void* stream);
  * attends node j of its sequence: its ancestors and itself. With c such nodes,
  * token t stands at position n + c - 1; its window is the last win_left + 1 of
  * (committed rows, attended nodes in query order), and compressed rows are
- * attended as by sas_fwd_v1 from that position (below (n + c) / cmp_ratio). A
+ * attended as by sas_fwd_v1 from that position (below (n + c) / cmp_ratio). Rows
+ * from n / cmp_ratio on cover draft positions, one row for all branches: SAS_SCFA
+ * indices can leave out those of another branch (-1), SAS_CFA attends them all,
+ * so it is right only for trees that stay below the next multiple of cmp_ratio
+ * or whose branches share what lies beyond. A
  * chain (bits 0 .. i for node i) is sas_fwd_v1's own mask. Bits past the
  * sequence's tokens, or of rows before position 0 (act_kv < act_q; n counts as 0
  * then), are ignored; a row without bits attends committed and compressed rows

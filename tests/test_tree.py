@@ -528,3 +528,36 @@ def test_gpu_tree_heads_short_of_a_workgroup(name):
     guard = _run(c)
     c.check(*guard)
     assert all(torch.equal(a, b) for a, b in zip(guard, _run(c)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,H", [("bf16", 64), ("fp8", 32)])
+def test_gpu_branches_across_a_compression_boundary(dt, H):
+    """Nodes on both sides of a multiple of the ratio, two branches: rows listed as
+    indices keep each node to the committed compressed rows and those of its own
+    branch; the dense form attends the shared row beyond the boundary too, as
+    documented."""
+    ratio, ql, kl = 8, [14, 9], [59 + 14, 121 + 9]
+    trees = []
+    for m in ql:   # node 0, then branches of odd and even nodes
+        t = [[0]]
+        for i in range(1, m):
+            t.append(t[max(0, i - 2)] + [i] if i > 2 else [0, i])
+        trees.append(t)
+    c = Case(kind="cfa", dt=dt, H=H, D=576, ql=ql, kl=kl, ratio=ratio, trees=trees)
+    deep = [(k - m + len(t)) // ratio > (k - m) // ratio for m, k, ts in zip(ql, kl, trees) for t in ts]
+    assert any(deep) and not all(deep)
+    out, lse = _run(c)
+    c.check(out, lse)
+    # the first branch's nodes alone have rows past the boundary
+    top = max(kl) // ratio
+    rows = []
+    for m, k, ts in zip(ql, kl, trees):
+        for t in ts:
+            limit = (k - m + len(t)) // ratio if 1 in t else (k - m) // ratio
+            rows.append([j if j < limit else -1 for j in range(top)])
+    c.kind, c.idx = "scfa", torch.tensor(rows, dtype=torch.int32)[:, None]
+    out2, lse2 = _run(c)
+    c.check(out2, lse2)
+    other = torch.tensor([d and 1 not in t for d, t in zip(deep, [t for ts in trees for t in ts])])
+    assert bool(other.any()) and bool((lse2[other] < lse[other]).all())
