@@ -998,3 +998,46 @@ def test_abi_names_the_most_rows_of_a_call():
         assert rc == (_lib.SAS_OK if ok else _lib.SAS_EINVAL)
         if not ok:
             assert "at most 2^28 - 32" in L.sas_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [16, 32, 48, 64, 128])
+@pytest.mark.parametrize("T", [9, 300])
+def test_gpu_fp8_rows_of_nan_reach_every_kernel(T, H):
+    """As above over the kernels that head and token counts choose, compressed rows among
+    the keys: one NaN row of each cache; tokens that attend neither as without them."""
+    from dsv4_amd.api import sparse_attn_sharedkv, sparse_attn_sharedkv_tree
+    from dsv4_amd.cache import append_kv_cache
+    g = torch.Generator().manual_seed(34)
+    q = torch.randn(T, H, 576, generator=g).to(torch.bfloat16).cuda()
+    blocks = -(-T // 64) + 1
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda")[None]
+    cu, used = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, T], [T]))
+    idx = torch.full((T, 1, 40), -1, dtype=torch.int32)
+    for t in range(T):
+        n = min((t + 1) // 4, 40)
+        idx[t, 0, :n] = torch.randperm((t + 1) // 4, generator=g)[:n]
+    words = -(-T // 64)
+    mask = [[(1 << min(64, t + 1 - 64 * w)) - 1 if t >= 64 * w else 0 for w in range(words)] for t in range(T)]
+    mask = torch.tensor([[x - (1 << 64) if x >> 63 else x for x in m] for m in mask], dtype=torch.int64).cuda()
+    clean, cmp_clean = (torch.randn(n, 576, generator=g).to(torch.bfloat16) for n in (T, max(T // 4, 1)))
+    kv, cmp = clean.clone(), cmp_clean.clone()
+    kv[5, 17], cmp[1, 400] = NAN, NAN
+
+    def caches(rows, cmp_rows):
+        out = []
+        for r in (rows, cmp_rows):
+            c = torch.zeros(blocks, 64, 1, 656, dtype=torch.uint8, device="cuda")
+            n = r.shape[0]
+            append_kv_cache(r.cuda(), c, table, *(torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, n], [n])), norm_dim=512)
+            out.append(c)
+        return dict(ori_kv=out[0], cmp_kv=out[1])
+
+    kw = dict(ori_block_table=table, cmp_block_table=table, cmp_sparse_indices=idx.cuda(), cmp_ratio=4, cu_seqlens_q=cu,
+              seqused_kv=used, sinks=torch.zeros(H, device="cuda"), softmax_scale=0.04, ori_win_left=31)
+    t = torch.arange(T)
+    sees = ((t >= 5) & (t - 31 <= 5)) | (idx[:, 0] == 1).any(1)
+    assert bool(sees.any()) and not bool(sees.all())
+    for call in (lambda c: sparse_attn_sharedkv(q, **kw, **c), lambda c: sparse_attn_sharedkv_tree(q, tree_mask=mask, **kw, **c)):
+        without, out = call(caches(clean, cmp_clean)), call(caches(kv, cmp))
+        assert bool(out[sees].isnan().all()) and torch.equal(out[~sees], without[~sees])
