@@ -2225,17 +2225,21 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 #if SAS_FWD_TREE
 // Whether a call takes the kernels of two workgroups a CU (sas_fwd_pair.h): all of a
 // token's slots in one workgroup, and
-//  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows, 32
-//    to 256 items of 576 channels: 13.0-15.5 us against 14.4-17.5, fp8 16.8-19.2 against
-//    17.7-34; fewer items: the same within 4%); or
+//  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows of
+//    576 channels, 32 / 64 / 128 / 256 items: 11.9 / 12.2 / 12.5 / 13.5 us against 12.3 / 14.0 /
+//    15.0 / 15.9, fp8 16.1 / 16.4 / 16.4 / 17.3 against 16.6 / 17.2 / 18.1 / 32; fewer items: the
+//    same within 4%); or
 //  - more workgroups of the other kernel than CUs, which hold one each (a second round).
-//    480 nodes, 128 + 1024 rows, 16 / 32 / 48 / 64 / 96 heads: 73 / 81 / 92 / 102 / 170 us against
-//    166 / 99 / 454 / 127 / 265 (heads that are no multiple of 32 leave it 16 a workgroup); 96
-//    nodes of 48 heads 51 against 143. With fp8 rows 97 / - / 113 / 123 / 223 against 110 / 89 /
-//    324 / 164 / 247; there the kernel of 32 heads a workgroup stays for 32 heads (it holds
-//    them all: 56 us against 64 at 640 rows), and for long rows of up to one item a CU (160 to
-//    256 items of 256 / 640 / 1152 rows 26-28 / 52-53 / 86-87 us against 31-32 / 53-55 / 83-86).
-//    (288 nodes of 96 heads, 1152 fp8 rows: 182 against 163, the one size found slower.)
+//    480 nodes, 128 + 1024 rows, 16 / 32 / 48 / 64 / 96 heads: 51 / 64 / 79 / 86 / 151 us against
+//    143 / 90 / 408 / 99 / 267 (heads that are no multiple of 32 leave it 16 a workgroup); 96
+//    nodes of 48 heads 48 against 137. With fp8 rows 95 / - / 109 / 115 / 219 against 108 / 82 /
+//    320 / 162 / 241; there the kernel of 32 heads a workgroup stays for 32 heads (it holds
+//    them all: 56 us against 64 at 640 rows), and past 640 rows for up to one item a CU: 130 to
+//    256 items of 64 heads, 256 / 512 / 640 rows 24-26 / 41-43 / 50-51 us against 29 / 44-45 /
+//    52-53, a gain that shrinks with the rows (1152: 86-87 against 83-86; it takes 58 / 66 / 73 /
+//    81 us for 768 / 896 / 1024 / 1152).
+//    One stretch lies on the wrong side: fp8 rows, 96 heads, 288 to 336 nodes (576 to 672
+//    items on 512 places) 107 against 101 us at 640 rows, 182 against 161 at 1152; 200 to 240 nodes 67 / 113 against 75 / 121, 480 130 / 219 against 151 / 241.
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
   if (pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
   const long long items = a->T * ((a->H + 63) / 64), cus = sas::device_cus();

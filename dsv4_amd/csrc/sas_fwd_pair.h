@@ -11,8 +11,8 @@
 // maximum rises by more than 2^8), P.V, in steps of 32 rows whose DMA runs a step ahead.
 //
 // us against the 8-wave kernel (window-only: the exact-window one), 64 heads, 480 nodes
-// / 960: 128-row window, D = 512 20 / 38 against 30 / 55, D = 576 21 / 39 against 31 / 59;
-// with 512 top-k rows D = 512 55 / 102 against 65 / 128, D = 576 56 / 110 against 66 / 127;
+// / 960: 128-row window, D = 512 18 / 35 against 28 / 55, D = 576 19 / 37 against 29 / 58;
+// with 512 top-k rows D = 512 50 / 94 against 63 / 122, D = 576 53 / 101 against 62 / 122;
 // over contexts of 8 K to 32 K, read from HBM, 62 / 115 against 71 / 133 and 65 / 123 against
 // 73 / 141. With lane offsets that spilled it was no faster at D = 576.
 //
@@ -61,6 +61,10 @@ __device__ __forceinline__ void put_none(uint8_t* ob, float* lse, float lse0, in
 // Online softmax of a step's scores (lane (g, c16): keys 16 mt + 4 g + j of head c16;
 // nk of the 32 keys count), in the log2 domain: P in s, the lane's sum in l, and O and l
 // rescaled in place where a row's maximum rises by more than 2^8 over the reference m.
+// The callers round P (or P x scale) once to 16 bits, which P.V's MFMAs take; l sums
+// it in fp32 before that. Half a step a key, independent over the keys: outputs are
+// 0.0021-0.0023 of their norm from 64 bits (bf16; fp16 0.00029), with P in 32 bits 0.0017
+// (0.00021), which is the output's own rounding.
 __device__ __forceinline__ void softmax_step(f32x4 (&s)[2], f32x4 (&acc)[kDV / 16], float& m, float& l, float scale,
                                              int nk, int g) {
   float mx = -INFINITY;
@@ -260,11 +264,11 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
 // rows' four scales [32][16 bytes]), and at a step's head each wave turns the latent bytes
 // that it loaded into bf16 (exactly, unscaled) in one tile of the other kernel's layout: one
 // conversion a value where a fragment converted as it is read has one in each of four
-// waves (4 trees of 64 nodes, 128 heads, 1152 rows: 115 us against 134, 729 VALU instructions a
-// step and wave against 375, 68 of them MFMAs). A scale group's four k-steps are a chain of their
-// own, folded into S with the rows' fp32 scales, and P x scale is what is rounded for P.V.
+// waves (4 trees of 64 nodes, 128 heads, 1152 rows: 115-117 us against 134, 381 VALU instructions
+// a step and wave against 729, 68 of them MFMAs). A scale group's four k-steps are a chain of
+// their own, folded into S with the rows' fp32 scales, and P x scale is what is rounded for P.V.
 // us against the 32-head kernel, which needs four rounds: 480 nodes, 64 heads, 128-row window
-// 27 against 67, with 128 / 512 / 1024 top-k rows 38 / 73 / 119 against 59 / 105 / 164.
+// 24 against 64, with 1024 top-k rows 115 against 162.
 constexpr int kPair8Slot = 21 * 1024, kPair8Rope = 16 * 1024, kPair8Scl = 20 * 1024;
 
 __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p) {

@@ -717,7 +717,12 @@ void fill_rope(const SasNormRopeArgs* a, RopeParams* p) {
 }
 
 // The kernel for a row width: 128, 512 or 576 channels with 64 rotated ones (or none) in
-// their own builds, any other in one of up to eight chunks a lane.
+// their own builds, any other in one of up to eight chunks a lane. That costs a narrow
+// forward its idle chunks (about 270 MB of rows of 64 heads, TB/s read and written: 192
+// channels 3.1, 256 3.8, 576 with 96 rotated 4.7, 512 with 32 or 128, 640 and 1024 6.3 to 6.7)
+// and the backward its registers: eight chunks of x and dy and (W) 64 sums spill 21 to
+// 151 of them. Its us with / without weights: 192 1743 / 622, 256 1342 / 484, 512 with
+// 128 rotated 727 / 274, 640 620 / 240, 1024 432 / 167; 512 in its own build 114 / 101.
 template <typename F>
 int by_width(const SasNormRopeArgs* a, F&& f) {
   const bool last = a->rope_dim == 64 || a->rope_dim == 0;
@@ -754,7 +759,9 @@ int launch_rope(const SasNormRopeArgs* a, const RopeParams& p, hipStream_t st, c
 }
 
 // Workgroups of the backward's two parts: three a CU (what the builds with weights hold, 3 waves a
-// SIMD), shared out by rows, none without rows of its own.
+// SIMD; those without hold four or five), shared out by rows, none without rows of its own.
+// A count of rows just above one round makes some walk twice: 736 tokens of 16 heads are
+// 782 groups of rows for 768 workgroups, 12-14 us.
 void grad_blocks(RopeParams* p) {
   const double all = (double)p->part[0].rows + p->part[1].rows;
   const long long most = 3LL * device_cus();
