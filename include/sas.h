@@ -310,8 +310,9 @@ int sas_bwd_plan(const SasBwdArgs* a, int32_t* dq_dtype, size_t* workspace_bytes
  * SAS_DT_FP8_E4M3_ROW656 (bf16 kv, D = 576): per 128 latent channels
  * scale = amax / 448 is stored and byte = e4m3fn(clamp(x * inv, -448, 448))
  * with inv = 448 / amax (both 1 for an all-zero group), rounded to nearest
- * even; rope channels copied as bf16. Rows written by one
- * call must be distinct (two rows to one cache row race).
+ * even; rope channels copied as bf16. A NaN stays one (0x7f or 0xff, with scale
+ * 1 for its group), an infinite channel is NaN under a scale of infinity. Rows
+ * written by one call must be distinct (two rows to one cache row race).
  */
 typedef struct SasCacheWriteArgs {
   const void* kv;                /* [N, kv_stride] kv_dtype, 16-byte aligned rows */
