@@ -26,7 +26,8 @@ SAS_ROPE_HALF = 1           # rotated pairs (i, i + rope_dim / 2)
 SAS_ROPE_INVERSE = 2        # rotation by the negative angle
 
 EXPORTED = ("sas_metadata_v1", "sas_metadata_device_v1", "sas_fwd_plan", "sas_fwd_v1", "sas_fwd_tree_v1", "sas_fwd_noalloc_v1", "sas_combine_v1",
-            "sas_cache_write_v1", "sas_cache_append_v1", "sas_norm_rope_v1", "sas_norm_rope_bwd_plan", "sas_norm_rope_bwd_v1", "sas_bwd_v1", "sas_bwd_plan", "sas_last_error", "sas_version",
+            "sas_cache_write_v1", "sas_cache_append_v1", "sas_norm_rope_v1", "sas_norm_rope_bwd_plan", "sas_norm_rope_bwd_v1", "sas_bwd_v1", "sas_bwd_plan", "sas_fwd_first_plan", "sas_fwd_first_v1", "sas_bwd_first_plan", "sas_bwd_first_v1",
+            "sas_row_weights_v1", "sas_cache_evict_v1", "sas_last_error", "sas_version",
             "sas_bench_atomic_add_v1")
 
 _i32p = C.POINTER(C.c_int32)
@@ -75,6 +76,17 @@ class SasFwdTreeArgs(C.Structure):
     _fields_ = [("fwd", SasFwdArgs), ("tree_mask", C.c_void_p), ("tree_words", C.c_int64)]
 
 
+class SasFwdFirstArgs(C.Structure):
+    _fields_ = [("fwd", SasFwdArgs), ("ori_first", C.c_int64)]
+
+
+class SasRowWeightsArgs(C.Structure):
+    _fields_ = [
+        ("fwd", SasFwdArgs), ("ori_first", C.c_int64), ("ori_weights", C.c_void_p), ("cmp_weights", C.c_void_p),
+        ("ori_rows", C.c_int64), ("cmp_rows", C.c_int64),
+    ]
+
+
 class SasCombineArgs(C.Structure):
     _fields_ = [
         ("part_o", C.c_void_p), ("part_ml", C.c_void_p), ("sinks", C.c_void_p),
@@ -88,6 +100,19 @@ class SasBwdArgs(C.Structure):
     _fields_ = [
         ("fwd", SasFwdArgs), ("dout", C.c_void_p), ("dq", C.c_void_p),
         ("d_ori_kv", C.c_void_p), ("d_cmp_kv", C.c_void_p), ("d_sinks", C.c_void_p),
+    ]
+
+
+class SasBwdFirstArgs(C.Structure):
+    _fields_ = [("bwd", SasBwdArgs), ("ori_first", C.c_int64)]
+
+
+class SasCacheEvictArgs(C.Structure):
+    _fields_ = [
+        ("cache", C.c_void_p), ("weights", C.c_void_p), ("block_table", C.c_void_p), ("act_kv", C.c_void_p),
+        ("act_kv_out", C.c_void_p), ("kept", C.c_void_p), ("B", C.c_int64), ("row_bytes", C.c_int64),
+        ("bt_stride", C.c_int64), ("block_size", C.c_int64), ("num_blocks", C.c_int64), ("weight_rows", C.c_int64),
+        ("budget", C.c_int64), ("keep_first", C.c_int64), ("keep_recent", C.c_int64),
     ]
 
 
@@ -172,6 +197,18 @@ def lib() -> C.CDLL:
                 L.sas_norm_rope_bwd_plan.restype = C.c_int
                 L.sas_norm_rope_bwd_v1.argtypes = [C.POINTER(SasNormRopeBwdArgs), C.c_void_p]
                 L.sas_norm_rope_bwd_v1.restype = C.c_int
+                L.sas_fwd_first_plan.argtypes = [C.POINTER(SasFwdFirstArgs), _i32p, C.POINTER(C.c_size_t)]
+                L.sas_fwd_first_plan.restype = C.c_int
+                L.sas_fwd_first_v1.argtypes = [C.POINTER(SasFwdFirstArgs), C.c_void_p]
+                L.sas_fwd_first_v1.restype = C.c_int
+                L.sas_bwd_first_plan.argtypes = [C.POINTER(SasBwdFirstArgs), _i32p, C.POINTER(C.c_size_t)]
+                L.sas_bwd_first_plan.restype = C.c_int
+                L.sas_bwd_first_v1.argtypes = [C.POINTER(SasBwdFirstArgs), C.c_void_p]
+                L.sas_bwd_first_v1.restype = C.c_int
+                L.sas_row_weights_v1.argtypes = [C.POINTER(SasRowWeightsArgs), C.c_void_p]
+                L.sas_row_weights_v1.restype = C.c_int
+                L.sas_cache_evict_v1.argtypes = [C.POINTER(SasCacheEvictArgs), C.c_void_p]
+                L.sas_cache_evict_v1.restype = C.c_int
                 L.sas_bench_atomic_add_v1.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                                       C.c_void_p]
                 L.sas_bench_atomic_add_v1.restype = C.c_int

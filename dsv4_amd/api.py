@@ -262,7 +262,9 @@ class _Resolved:
 def _resolve(q, *, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
              seqused_q, seqused_kv, sinks, metadata, softmax_scale, cmp_ratio, ori_mask_mode, cmp_mask_mode,
              ori_win_left, ori_win_right, layout_q, layout_kv, core_num, topk_cmp, num_splits, head_waves,
-             waves) -> _Resolved:
+             waves, ori_first=None, attends=True) -> _Resolved:
+    """``ori_first``: first rows that stay visible (None: a call without them); ``attends``
+    False: no forward, so no sinks and no split plan."""
     del seqused_q  # API-parity placeholder, as in the reference (api.py:186)
     assert ori_mask_mode == 4, "only ori_mask_mode=4 supported"
     assert cmp_mask_mode == 3 or cmp_kv is None, "only cmp_mask_mode=3 supported"
@@ -400,8 +402,8 @@ def _resolve(q, *, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_bloc
     ckv = d(cmp_kv) if scenario >= _lib.SAS_CFA else None
     cbt = d(cmp_block_table, torch.int32) if scenario >= _lib.SAS_CFA else None
     cidx = d(idx_flat, torch.int32) if scenario == _lib.SAS_SCFA else None
-    snk = d(sinks, torch.float32)
-    if snk.numel() != N1:
+    snk = d(sinks, torch.float32) if attends else None
+    if attends and snk.numel() != N1:
         raise ValueError(f"sinks must have {N1} entries (got {snk.numel()})")
 
     a = _lib.SasFwdArgs()
@@ -424,7 +426,7 @@ def _resolve(q, *, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_bloc
     a.cmp_kv = ckv.data_ptr() if ckv is not None else None
     a.cmp_block_table = cbt.data_ptr() if cbt is not None else None
     a.cmp_indices = cidx.data_ptr() if cidx is not None else None
-    a.sinks = snk.data_ptr()
+    a.sinks = snk.data_ptr() if attends else None
     a.T, a.B, a.H, a.D, a.DV = T1, B, N1, D, 512
     a.ori_block_size, a.ori_bt_stride, a.ori_num_blocks = okv.shape[1], obt.shape[1], okv.shape[0]
     if ckv is not None:
@@ -441,7 +443,11 @@ def _resolve(q, *, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_bloc
     a.waves = int(waves)
     ns = C.c_int32(0)
     ws = C.c_size_t(0)
-    _lib.check(_lib.lib().sas_fwd_plan(C.byref(a), C.byref(ns), C.byref(ws)), "sparse_attn_sharedkv")
+    if attends and ori_first is None:
+        _lib.check(_lib.lib().sas_fwd_plan(C.byref(a), C.byref(ns), C.byref(ws)), "sparse_attn_sharedkv")
+    elif attends:
+        _lib.check(_lib.lib().sas_fwd_first_plan(C.byref(_lib.SasFwdFirstArgs(a, ori_first)), C.byref(ns), C.byref(ws)),
+                   "sparse_attn_sharedkv_first")
     a.num_splits = ns.value
     r.args, r.keep, r.device, r.dtype = a, keep, dev, q.dtype
     r.T1, r.N1, r.layout_q, r.B, r.S_max = T1, N1, layout_q, B, S_max
@@ -649,6 +655,25 @@ def _fwd_bytes():
     return _fwd_raw
 
 
+# what SasFwdFirstArgs and SasRowWeightsArgs put behind them
+_INT = struct.Struct("@q")
+assert C.sizeof(_lib.SasFwdFirstArgs) == C.sizeof(_lib.SasFwdArgs) + _INT.size
+_WEIGHTS = struct.Struct("@q2Q2q")
+assert C.sizeof(_lib.SasRowWeightsArgs) == C.sizeof(_lib.SasFwdArgs) + _WEIGHTS.size
+_raw_fns = {}
+
+
+def _bytes_fn(name: str):
+    """An entry point taking its arguments as packed bytes."""
+    f = _raw_fns.get(name)
+    if f is None:
+        f = _lib.lib()[name]   # a function object of its own: other argument types
+        f.argtypes = [C.c_char_p, C.c_void_p]
+        f.restype = C.c_int
+        _raw_fns[name] = f
+    return f
+
+
 def _tree_bytes():
     """sas_fwd_tree_v1 taking its arguments as packed bytes."""
     global _tree_raw
@@ -735,14 +760,19 @@ def sparse_attn_sharedkv(
     return _run_first(r, key, stream, dev, return_softmax_lse)
 
 
-def _run_first(r: _Resolved, key, stream, dev, return_softmax_lse, tree_mask=None):
-    """Run a call from its resolution, kept for the signature's later calls where it holds for them."""
+def _keep(r: _Resolved, key) -> None:
+    """Keep a resolution for the signature's later calls where it holds for them."""
     if r.cacheable:
         kept = _Cached(r)
         with _cache_lock:
             _cache[key] = kept
             if len(_cache) > _CACHE_MAX:
                 del _cache[min(_cache.items(), key=lambda kv: kv[1].used)[0]]
+
+
+def _run_first(r: _Resolved, key, stream, dev, return_softmax_lse, tree_mask=None, ori_first=None):
+    """Run a call from its resolution."""
+    _keep(r, key)
     out = torch.empty((r.T1, r.N1, 512), dtype=r.dtype, device=dev)
     lse = torch.empty((r.T1, r.N1), dtype=torch.float32, device=dev)
     a = _lib.SasFwdArgs.from_buffer_copy(r.args)
@@ -761,7 +791,10 @@ def _run_first(r: _Resolved, key, stream, dev, return_softmax_lse, tree_mask=Non
         if r.ws_bytes:
             ws = _workspace(dev, stream, r.ws_bytes)
             a.workspace, a.workspace_bytes = ws.data_ptr(), r.ws_bytes
-        if tree_mask is None:
+        if ori_first is not None:
+            fa = _lib.SasFwdFirstArgs(a, ori_first)
+            _lib.check(_lib.lib().sas_fwd_first_v1(C.byref(fa), C.c_void_p(stream)), "sparse_attn_sharedkv_first")
+        elif tree_mask is None:
             _lib.check(_lib.lib().sas_fwd_v1(C.byref(a), C.c_void_p(stream)), "sparse_attn_sharedkv")
         else:
             ta = _lib.SasFwdTreeArgs(fwd=a, tree_mask=tree_mask.data_ptr(), tree_words=tree_mask.shape[-1])
@@ -788,7 +821,7 @@ class _Cached:
 
 
 def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table,
-                cu_seqlens_q, seqused_kv, sinks, return_softmax_lse, tree_mask=None):
+                cu_seqlens_q, seqused_kv, sinks, return_softmax_lse, tree_mask=None, ori_first=None):
     out = q.new_empty(r.out_shape)
     lse = sinks.new_empty(r.lse_shape)   # fp32 on the device, or the call would not be cached
     cu, kv = cu_seqlens_q.data_ptr(), seqused_kv.data_ptr()
@@ -820,12 +853,15 @@ def _run_cached(r: _Cached, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, 
                             cmp_sparse_indices.data_ptr() if cmp_ and cmp_sparse_indices is not None else 0,
                             cu, 0, kv, sinks.data_ptr(), out.data_ptr(), lse.data_ptr(),
                             0 if ws is None else ws.data_ptr(), r.ws_bytes) + r.tail
-        if tree_mask is None:
+        if ori_first is not None:
+            rc = _bytes_fn("sas_fwd_first_v1")(packed + _INT.pack(ori_first), stream)
+        elif tree_mask is None:
             rc = _fwd_bytes()(packed, stream)
         else:
             rc = _tree_bytes()(packed + _TREE.pack(tree_mask.data_ptr(), tree_mask.shape[-1]), stream)
         if rc:
-            _lib.check(rc, "sparse_attn_sharedkv" if tree_mask is None else "sparse_attn_sharedkv_tree")
+            _lib.check(rc, "sparse_attn_sharedkv_first" if ori_first is not None else
+                       "sparse_attn_sharedkv" if tree_mask is None else "sparse_attn_sharedkv_tree")
     finally:
         if staged is not None:
             ring.release(staged[1], stream)
@@ -929,16 +965,230 @@ _TREE_DEFAULTS = {k: v for k, v in _FWD_DEFAULTS.items() if k not in (
     "cmp_kv", "cmp_sparse_indices", "cmp_block_table", "cu_seqlens_q")}
 
 
+def _first_rows(ori_first) -> int:
+    if isinstance(ori_first, bool) or not isinstance(ori_first, int) or ori_first < 0:
+        raise ValueError(f"ori_first must be an integer of at least 0 (got {ori_first!r})")
+    return ori_first
+
+
+def _signature(kind, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q, seqused_kv,
+               softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q):
+    """The key of a call with first rows, less its sinks: geometries spelt out, as in
+    :func:`sparse_attn_sharedkv`."""
+    cfa_k = None
+    if cmp_kv is not None and cmp_sparse_indices is None and seqused_kv.numel():
+        cfa_k = int(seqused_kv.max().item())
+    return (kind, q.shape, q.dtype, q.get_device(), q.is_contiguous(),
+            ori_kv.shape, ori_kv.dtype, ori_kv.get_device(), ori_kv.is_contiguous(),
+            ori_block_table.shape, ori_block_table.dtype, ori_block_table.get_device(), ori_block_table.is_contiguous(),
+            seqused_kv.shape, seqused_kv.dtype, seqused_kv.get_device(), seqused_kv.is_contiguous(),
+            None if cu_seqlens_q is None else
+            (cu_seqlens_q.shape, cu_seqlens_q.dtype, cu_seqlens_q.get_device(), cu_seqlens_q.is_contiguous()),
+            None if cmp_kv is None else (cmp_kv.shape, cmp_kv.dtype, cmp_kv.get_device(), cmp_kv.is_contiguous()),
+            None if cmp_block_table is None else
+            (cmp_block_table.shape, cmp_block_table.dtype, cmp_block_table.get_device(), cmp_block_table.is_contiguous()),
+            None if cmp_sparse_indices is None else
+            (cmp_sparse_indices.shape, cmp_sparse_indices.dtype, cmp_sparse_indices.get_device(),
+             cmp_sparse_indices.is_contiguous()),
+            float(softmax_scale), cmp_ratio, ori_win_left, ori_first, layout_q, cfa_k)
+
+
+def sparse_attn_sharedkv_first(
+    q: torch.Tensor,
+    *,
+    ori_first: int,
+    ori_kv: torch.Tensor,
+    cmp_kv: Optional[torch.Tensor] = None,
+    cmp_sparse_indices: Optional[torch.Tensor] = None,
+    ori_block_table: torch.Tensor,
+    cmp_block_table: Optional[torch.Tensor] = None,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    seqused_kv: torch.Tensor,
+    sinks: torch.Tensor,
+    softmax_scale: float,
+    cmp_ratio: Optional[int] = None,
+    ori_win_left: int = 127,
+    layout_q: str = "TND",
+    return_softmax_lse: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """:func:`sparse_attn_sharedkv` whose first rows stay visible (the reference's window
+    drops them, golden.py:128-131).
+
+    A token at position ``s`` attends the raw rows ``j <= s`` with ``j >= s -
+    ori_win_left`` or ``j < ori_first``, each once, and the compressed rows as ever. So a
+    sequence can run on without end with a window's blocks and those of its first rows: the
+    blocks between may be given back and their entries of ``ori_block_table`` be -1.
+    ``ori_first`` 0 gives :func:`sparse_attn_sharedkv`'s mask. Draft trees, and rows whose
+    gradients are wanted in fp8, are not served; the other arguments and the result are that
+    function's. Its gradients: :func:`sparse_attn_sharedkv_first_backward`.
+    """
+    ori_first = _first_rows(ori_first)
+    key = _signature("first", q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
+                     seqused_kv, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q) + (
+        sinks.shape, sinks.dtype, sinks.get_device(), sinks.is_contiguous())
+    dev = q.device
+    if q.is_cuda and dev.index != _device():
+        with torch.cuda.device(dev):
+            return sparse_attn_sharedkv_first(
+                q, ori_first=ori_first, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices,
+                ori_block_table=ori_block_table, cmp_block_table=cmp_block_table, cu_seqlens_q=cu_seqlens_q,
+                seqused_kv=seqused_kv, sinks=sinks, softmax_scale=softmax_scale, cmp_ratio=cmp_ratio,
+                ori_win_left=ori_win_left, layout_q=layout_q, return_softmax_lse=return_softmax_lse)
+    stream = _raw_stream(dev) if q.is_cuda else None
+    r = _cache.get(key)
+    if r is not None:
+        r.used = next(_uses)
+        return _run_cached(r, stream, dev, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table,
+                           cu_seqlens_q, seqused_kv, sinks, return_softmax_lse, None, ori_first)
+    r = _resolve(q, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices, ori_block_table=ori_block_table,
+                 cmp_block_table=cmp_block_table, cu_seqlens_q=cu_seqlens_q, seqused_kv=seqused_kv, sinks=sinks,
+                 softmax_scale=softmax_scale, ori_first=ori_first,
+                 **dict(_TREE_DEFAULTS, cmp_ratio=cmp_ratio, ori_win_left=ori_win_left, layout_q=layout_q))
+    return _run_first(r, key, stream, dev, return_softmax_lse, None, ori_first)
+
+
+def add_row_weights(
+    q: torch.Tensor,
+    lse: torch.Tensor,
+    *,
+    ori_weights: Optional[torch.Tensor] = None,
+    cmp_weights: Optional[torch.Tensor] = None,
+    ori_kv: torch.Tensor,
+    cmp_kv: Optional[torch.Tensor] = None,
+    cmp_sparse_indices: Optional[torch.Tensor] = None,
+    ori_block_table: torch.Tensor,
+    cmp_block_table: Optional[torch.Tensor] = None,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    seqused_kv: torch.Tensor,
+    softmax_scale: float,
+    cmp_ratio: Optional[int] = None,
+    ori_win_left: int = 127,
+    ori_first: int = 0,
+    layout_q: str = "TND",
+    sinks: Optional[torch.Tensor] = None,
+) -> None:
+    """Add the attention weight that a call's tokens give each cache row to
+    ``ori_weights`` and ``cmp_weights`` (no counterpart in the reference), what
+    :func:`dsv4_amd.cache.evict_kv_cache` chooses rows by.
+
+    ``lse`` is what :func:`sparse_attn_sharedkv` or :func:`sparse_attn_sharedkv_first`
+    returned for ``q`` and the same keyword arguments. ``ori_weights`` float64 ``[B, R]``,
+    row ``b`` beside row ``b`` of the block table, gets at ``[b, j]`` the mean over heads
+    of the sum over sequence ``b``'s tokens of ``exp(softmax_scale q . k_j - lse)`` for every raw
+    row ``j`` that they attend (the window and the first ``ori_first`` rows), and
+    ``cmp_weights`` likewise for compressed rows; either may be left out, rows past ``R`` are. A
+    weight starts as 0 and grows by at most 1 a token. The sums are multiples of 2^-36:
+    below 2^17 they are exact, so the same whatever order calls, tokens and workgroups
+    add in. A row listed twice counts twice; NaN and infinities propagate. ``sinks`` is
+    taken so that the attention's keyword arguments fit, and not read (``lse`` holds
+    them). No host sync, but for the dense compressed form's as in the attention.
+    """
+    ori_first = _first_rows(ori_first)
+    if ori_weights is None and cmp_weights is None:
+        raise ValueError("add_row_weights needs ori_weights or cmp_weights")
+    if cmp_weights is not None and cmp_kv is None:
+        raise ValueError("cmp_weights without cmp_kv")
+    dev = q.device
+    B = seqused_kv.numel()
+    for name, w in (("ori_weights", ori_weights), ("cmp_weights", cmp_weights)):
+        if w is not None and (w.dtype is not torch.float64 or w.dim() != 2 or w.shape[0] != B or w.device != dev
+                              or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float64 [{B}, rows] tensor on {dev}, got {w.dtype} "
+                             f"{tuple(w.shape)} on {w.device}")
+    if lse.dtype is not torch.float32 or lse.shape != q.shape[:-1] or lse.device != dev:
+        raise ValueError(f"lse must be float32 {tuple(q.shape[:-1])} on {dev}, got {lse.dtype} {tuple(lse.shape)} "
+                         f"on {lse.device}")
+    if q.is_cuda and dev.index != _device():
+        with torch.cuda.device(dev):
+            return add_row_weights(
+                q, lse, ori_weights=ori_weights, cmp_weights=cmp_weights, ori_kv=ori_kv, cmp_kv=cmp_kv,
+                cmp_sparse_indices=cmp_sparse_indices, ori_block_table=ori_block_table, cmp_block_table=cmp_block_table,
+                cu_seqlens_q=cu_seqlens_q, seqused_kv=seqused_kv, softmax_scale=softmax_scale, cmp_ratio=cmp_ratio,
+                ori_win_left=ori_win_left, ori_first=ori_first, layout_q=layout_q)
+    # (weights without rows have no address)
+    if ori_weights is not None and ori_weights.shape[1] == 0:
+        ori_weights = None
+    if cmp_weights is not None and cmp_weights.shape[1] == 0:
+        cmp_weights = None
+    if ori_weights is None and cmp_weights is None:
+        return
+    lse = lse.contiguous()
+    behind = _WEIGHTS.pack(ori_first, 0 if ori_weights is None else ori_weights.data_ptr(),
+                           0 if cmp_weights is None else cmp_weights.data_ptr(),
+                           0 if ori_weights is None else ori_weights.shape[1],
+                           0 if cmp_weights is None else cmp_weights.shape[1])
+    key = _signature("weights", q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
+                     seqused_kv, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q)
+    stream = _raw_stream(dev) if q.is_cuda else None
+    r = _cache.get(key)
+    staged = keep = None
+    try:
+        if r is not None:
+            r.used = next(_uses)
+            cu, kv = cu_seqlens_q.data_ptr(), seqused_kv.data_ptr()
+            if r.host_names:
+                cur = {"cu": cu_seqlens_q, "kv": seqused_kv}
+                parts = [_host_i32(cur[name]) for name in r.host_names]
+                if not torch.cuda.is_current_stream_capturing():
+                    ring = _seqlen_ring(dev)
+                    staged = ring.stage([(t.data_ptr(), t.numel()) for t in parts], stream)
+                if staged is not None:
+                    base = staged[0]
+                else:
+                    keep = _stage(parts, dev, torch.cuda.current_stream(dev))
+                    base = keep.data_ptr()
+                for name, t in zip(r.host_names, parts):
+                    if name == "cu":
+                        cu = base
+                    else:
+                        kv = base
+                    base += 4 * t.numel()
+            packed = _PTRS.pack(q.data_ptr(), ori_kv.data_ptr(), ori_block_table.data_ptr(),
+                                0 if cmp_kv is None else cmp_kv.data_ptr(),
+                                0 if cmp_kv is None else cmp_block_table.data_ptr(),
+                                0 if cmp_sparse_indices is None or cmp_kv is None else cmp_sparse_indices.data_ptr(),
+                                cu, 0, kv, 0, 0, lse.data_ptr(), 0, 0) + r.tail
+        else:
+            r = _resolve(q, ori_kv=ori_kv, cmp_kv=cmp_kv, cmp_sparse_indices=cmp_sparse_indices,
+                         ori_block_table=ori_block_table, cmp_block_table=cmp_block_table, cu_seqlens_q=cu_seqlens_q,
+                         seqused_kv=seqused_kv, sinks=None, softmax_scale=softmax_scale, attends=False,
+                         **dict(_TREE_DEFAULTS, cmp_ratio=cmp_ratio, ori_win_left=ori_win_left, layout_q=layout_q))
+            _keep(r, key)
+            a = _lib.SasFwdArgs.from_buffer_copy(r.args)
+            a.lse = lse.data_ptr()
+            keep = []
+            if r.host_parts:
+                if not torch.cuda.is_current_stream_capturing():
+                    ring = _seqlen_ring(dev)
+                    staged = ring.stage([(t.data_ptr(), t.numel()) for _, t in r.host_parts], stream)
+                if staged is not None:
+                    _point_seqlens(r.host_parts, a, staged[0])
+                else:
+                    _bind_seqlens(r, r.host_parts, a, torch.cuda.current_stream(dev), keep)
+            packed = bytes(a)
+        rc = _bytes_fn("sas_row_weights_v1")(packed + behind, stream)
+        if rc:
+            _lib.check(rc, "add_row_weights")
+    finally:
+        if staged is not None:
+            ring.release(staged[1], stream)
+
+
 class PreparedBackward:
     """Arguments and gradient buffers of one backward, resolved once;
     :meth:`launch` enqueues the kernel (the gradients accumulate:
     :meth:`zero_grads` clears them), :meth:`result` returns them."""
 
-    def __init__(self, call: PreparedCall, ba, keep, q, dq, d_ori, d_cmp, d_sinks):
+    def __init__(self, call: PreparedCall, ba, keep, q, dq, d_ori, d_cmp, d_sinks, ori_first=None):
         self._call, self.args, self._keep, self._q = call, ba, keep, q
+        self._first = None if ori_first is None else _lib.SasBwdFirstArgs(ba, ori_first)
         self.dq, self.d_ori_kv, self.d_cmp_kv, self.d_sinks = dq, d_ori, d_cmp, d_sinks
 
     def launch(self, stream: Optional[torch.cuda.Stream] = None) -> None:
+        if self._first is not None:
+            _lib.check(_lib.lib().sas_bwd_first_v1(C.byref(self._first), self._call._stream(stream)),
+                       "sparse_attn_sharedkv_first_backward")
+            return
         _lib.check(_lib.lib().sas_bwd_v1(C.byref(self.args), self._call._stream(stream)),
                    "sparse_attn_sharedkv_backward")
 
@@ -972,7 +1222,11 @@ def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBack
     and convert)."""
     kwargs.pop("return_softmax_lse", None)
     window_pass = kwargs.pop("window_pass", None)
-    call = prepare_sparse_attn_sharedkv(q, **kwargs)
+    ori_first = kwargs.pop("ori_first", None)
+    if ori_first is None:
+        call = prepare_sparse_attn_sharedkv(q, **kwargs)
+    else:
+        call = PreparedCall(_resolve(q, ori_first=ori_first, **dict(_FWD_DEFAULTS, **kwargs)))
     # a copy: the forward's resolved split count stays with the forward. The
     # backward takes the caller's count, or plans its own (0); the forward's
     # plan (C2: 4 splits, 128 workgroups of 64 heads) would leave half the
@@ -996,8 +1250,12 @@ def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBack
     cmp_kv = kwargs.get("cmp_kv")
     keep = [dout_f, out_f, lse_f]
     direct, ws = C.c_int32(0), C.c_size_t(0)
-    _lib.check(_lib.lib().sas_bwd_plan(C.byref(_lib.SasBwdArgs(fwd=a, dout=dout_f.data_ptr())), C.byref(direct),
-                                       C.byref(ws)), "sparse_attn_sharedkv_backward")
+    plan = _lib.SasBwdArgs(fwd=a, dout=dout_f.data_ptr())
+    if ori_first is None:
+        _lib.check(_lib.lib().sas_bwd_plan(C.byref(plan), C.byref(direct), C.byref(ws)), "sparse_attn_sharedkv_backward")
+    else:
+        _lib.check(_lib.lib().sas_bwd_first_plan(C.byref(_lib.SasBwdFirstArgs(plan, ori_first)), C.byref(direct),
+                                                 C.byref(ws)), "sparse_attn_sharedkv_first_backward")
     if ws.value:
         work = torch.empty(ws.value, dtype=torch.uint8, device=dev)
         keep.append(work)
@@ -1015,7 +1273,7 @@ def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBack
     ba = _lib.SasBwdArgs(fwd=a, dout=dout_f.data_ptr(), dq=dq.data_ptr(), d_ori_kv=d_ori.data_ptr(),
                          d_cmp_kv=d_cmp.data_ptr() if d_cmp is not None else None,
                          d_sinks=d_sinks.data_ptr())
-    return PreparedBackward(call, ba, keep, q, dq, d_ori, d_cmp, d_sinks)
+    return PreparedBackward(call, ba, keep, q, dq, d_ori, d_cmp, d_sinks, ori_first)
 
 
 def sparse_attn_sharedkv_backward(
@@ -1042,14 +1300,37 @@ def sparse_attn_sharedkv_backward(
     return pb.result()
 
 
+def sparse_attn_sharedkv_first_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    *,
+    ori_first: int,
+    **kwargs,
+) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], torch.Tensor]:
+    """Gradients of :func:`sparse_attn_sharedkv_first`: as
+    :func:`sparse_attn_sharedkv_backward`, over that forward's keys; ``kwargs`` are
+    its keyword arguments."""
+    ori_first = _first_rows(ori_first)
+    if q.is_cuda and q.device.index != _device():
+        with torch.cuda.device(q.device):
+            return sparse_attn_sharedkv_first_backward(dout, q, out, lse, ori_first=ori_first, **kwargs)
+    pb = _prepare_backward(dout, q, out, lse, True, ori_first=ori_first, **kwargs)
+    pb.launch()
+    return pb.result()
+
+
 class _SparseAttnSharedkvFn(torch.autograd.Function):
     """Autograd binding: forward = :func:`sparse_attn_sharedkv` (keeping
-    out / LSE), backward = :func:`sparse_attn_sharedkv_backward`."""
+    out / LSE), backward = :func:`sparse_attn_sharedkv_backward`; with
+    ``ori_first`` among the arguments, those with first rows."""
 
     @staticmethod
     def forward(ctx, q, ori_kv, cmp_kv, sinks, kw):
         kwargs = dict(kw, ori_kv=ori_kv, cmp_kv=cmp_kv, sinks=sinks)
-        out, lse = sparse_attn_sharedkv(q, return_softmax_lse=True, **kwargs)
+        fwd = sparse_attn_sharedkv_first if "ori_first" in kw else sparse_attn_sharedkv
+        out, lse = fwd(q, return_softmax_lse=True, **kwargs)
         ctx.save_for_backward(q, ori_kv, cmp_kv if cmp_kv is not None else torch.empty(0), sinks, out, lse)
         ctx.kw = kw
         ctx.has_cmp = cmp_kv is not None
@@ -1060,7 +1341,8 @@ class _SparseAttnSharedkvFn(torch.autograd.Function):
     def backward(ctx, dout, dlse):
         q, ori_kv, cmp_kv, sinks, out, lse = ctx.saved_tensors
         kwargs = dict(ctx.kw, ori_kv=ori_kv, cmp_kv=cmp_kv if ctx.has_cmp else None, sinks=sinks)
-        dq, d_ori, d_cmp, d_sinks = sparse_attn_sharedkv_backward(
+        bwd = sparse_attn_sharedkv_first_backward if "ori_first" in ctx.kw else sparse_attn_sharedkv_backward
+        dq, d_ori, d_cmp, d_sinks = bwd(
             dout.to(q.dtype).contiguous(), q, out, lse, **kwargs)
         return (dq, d_ori.to(ori_kv.dtype), d_cmp.to(cmp_kv.dtype) if ctx.has_cmp else None,
                 d_sinks.to(sinks.dtype), None)
@@ -1074,4 +1356,13 @@ def sparse_attn_sharedkv_autograd(q: torch.Tensor, *, ori_kv: torch.Tensor,
     :func:`sparse_attn_sharedkv_backward`; the LSE output is not
     differentiable). Other arguments as for :func:`sparse_attn_sharedkv`."""
     out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, kwargs)
+    return (out, lse) if return_softmax_lse else out
+
+
+def sparse_attn_sharedkv_first_autograd(q: torch.Tensor, *, ori_first: int, ori_kv: torch.Tensor,
+                                        cmp_kv: Optional[torch.Tensor] = None, sinks: torch.Tensor,
+                                        return_softmax_lse: bool = False, **kwargs):
+    """:func:`sparse_attn_sharedkv_first` recorded for autograd, as
+    :func:`sparse_attn_sharedkv_autograd` records the attention without first rows."""
+    out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, dict(kwargs, ori_first=ori_first))
     return (out, lse) if return_softmax_lse else out

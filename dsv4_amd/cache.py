@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -226,3 +226,69 @@ def append_kv_cache(
     rope._launch("sas_cache_append_v1", b.ptrs(out, None) + b.dims + _APPEND_PTRS.pack(
         cu.data_ptr(), used.data_ptr(), bt.data_ptr(), cache.data_ptr()) + b.extra, dev, "append_kv_cache")
     return out
+
+
+# SasCacheEvictArgs as packed bytes: six pointers, nine int64
+_EVICT = struct.Struct("@6Q9q")
+assert _EVICT.size == C.sizeof(_lib.SasCacheEvictArgs)
+
+
+def evict_kv_cache(
+    cache: torch.Tensor,
+    weights: torch.Tensor,
+    block_table: torch.Tensor,
+    seqused_kv: torch.Tensor,
+    *,
+    budget: int,
+    keep_first: int = 0,
+    keep_recent: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cut every sequence of more than ``budget`` cache rows down to that many, in place:
+    its first ``keep_first`` rows stay, its last ``keep_recent`` ones, and of the others
+    the heaviest by ``weights`` (of equal ones those at the lowest positions; NaN counts
+    as the least). Returns ``(seqused_kv, kept)``.
+
+    ``cache [num_blocks, block_size, 1, row]`` holds rows of any type whose size is a
+    multiple of 16 bytes; ``weights`` float64 ``[B, R]``
+    (:func:`dsv4_amd.api.add_row_weights`), row ``b`` beside row ``b`` of ``block_table``;
+    a cache row past ``R`` weighs 0. The rows that stay move together, in their order, to the
+    sequence's first ``budget`` positions, their weights with them, and the weights behind
+    become 0, ready for the rows that come next; the cache's bytes behind stay as they are. So
+    the next step appends at position ``budget`` (:func:`append_kv_cache` with the
+    ``positions`` that the tokens' angles belong to) and the attention reads the rows as
+    one run (``ori_win_left`` at least the longest sequence), and blocks past the last
+    row can be given back.
+
+    ``seqused_kv`` int32 ``[B]`` is the new lengths, ``kept`` int32 ``[B, budget]`` the old
+    positions of the rows that stay (-1 past the last): what else is kept by row moves by it.
+    A row whose old or new place has no block is not moved. Sequences that share a block (a
+    common prefix) must not be evicted from. No host sync.
+    """
+    if cache.dim() != 4 or cache.shape[2] != 1 or not cache.is_contiguous():
+        raise ValueError(f"cache must be contiguous [num_blocks, block_size, 1, row], got {tuple(cache.shape)}")
+    row = cache.shape[3] * cache.element_size()
+    B = seqused_kv.numel()
+    if seqused_kv.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise ValueError(f"seqused_kv [B] and block_table [B, max_blocks] must agree, got {tuple(seqused_kv.shape)}, "
+                         f"{tuple(block_table.shape)}")
+    if weights.dtype is not torch.float64 or weights.dim() != 2 or weights.shape[0] != B or not weights.is_contiguous():
+        raise ValueError(f"weights must be contiguous float64 [{B}, rows], got {weights.dtype} {tuple(weights.shape)}")
+    for name, v in (("budget", budget), ("keep_first", keep_first), ("keep_recent", keep_recent)):
+        if isinstance(v, bool) or not isinstance(v, int):
+            raise ValueError(f"{name} must be an integer (got {v!r})")
+    if budget < 1 or keep_first < 0 or keep_recent < 0 or keep_first + keep_recent > budget:
+        raise ValueError(f"budget must be at least 1 and hold keep_first and keep_recent (got {budget}, {keep_first}, "
+                         f"{keep_recent})")
+    dev = cache.device
+    if weights.device != dev or block_table.device != dev or seqused_kv.device != dev:
+        raise ValueError("all tensors must be on cache's device")
+    if not cache.is_cuda:
+        raise ValueError("evict_kv_cache runs on the GPU: cache must be a device tensor")
+    bt, used = _i32(block_table), _i32(seqused_kv)
+    left = torch.empty_like(used)
+    kept = used.new_empty((B, budget))
+    rope._launch("sas_cache_evict_v1", _EVICT.pack(
+        cache.data_ptr(), weights.data_ptr(), bt.data_ptr(), used.data_ptr(), left.data_ptr(), kept.data_ptr(), B, row,
+        bt.shape[1], cache.shape[1], cache.shape[0], weights.shape[1], budget, keep_first, keep_recent), dev,
+        "evict_kv_cache")
+    return left, kept

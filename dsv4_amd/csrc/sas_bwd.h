@@ -7,7 +7,13 @@
 
 #include "sas_kern.h"
 
+#ifndef SAS_BWD_FIRST
+#define SAS_BWD_FIRST 0   // 1 (sas_bwd_first.hip, sas_bwd_pre_first.hip): with first rows that stay visible
+#endif
+
 namespace sas {
+
+constexpr bool kBwdFirst = SAS_BWD_FIRST;
 
 struct BwdParams {
   FwdParams f;
@@ -31,6 +37,7 @@ struct BwdParams {
   int seg_groups;       // key-major pass: (batch, segment) slots of the grid
   int cmp_tiles;        // key-major pass: compressed row tiles per segment
   int win_tiles_seg;    // key-major pass: window row tiles per segment
+  int first_tiles;      // key-major pass: tiles of first rows per segment (as far as the window leaves them behind)
 };
 
 // f(integral_constant<int, j>) for j = 0 .. N-1, with no loop: arrays
@@ -81,6 +88,8 @@ __device__ __forceinline__ float sum16(float x) {
 // The prefill path: dq by sas_bwd_dq_kernel (one workgroup per token and head
 // group), then every cache row's gradient by sas_bwd_keys_kernel.
 int launch_bwd_prefill(const BwdParams& bp, int D, int q_dtype, hipStream_t st);
+// the same with first rows (sas_bwd_pre_first.hip)
+int launch_bwd_prefill_first(const BwdParams& bp, int D, int q_dtype, hipStream_t st);
 // heads per workgroup of sas_bwd_dq_kernel
 inline int bwd_dq_heads(int H) { return H % 64 == 0 ? 64 : 32; }
 constexpr int kKeyRows = 64;   // rows per tile of the key-major pass

@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256 * NG) sas_bwd_kernel(const BwdParams bp) {
   const int item = item_index(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
-  resolve<256, D * 2>(p, k, tid, lane, wave, [] {});
+  resolve<256, D * 2, false, false, kBwdFirst>(p, k, tid, lane, wave, [] {});
   const int hgw = wave >> 2, wl = wave & 3;    // head group in the workgroup, wave in the group
   const int h = (tid & 255) >> 4, part = tid & 15;
   const int hw = hgw * 16 + h;                 // head in the workgroup
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(512) sas_bwd64_kernel(const BwdParams bp) {
   const int item = item_index(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
-  resolve<256, D * 2>(p, k, tid, lane, wave, [] {});
+  resolve<256, D * 2, false, false, kBwdFirst>(p, k, tid, lane, wave, [] {});
   const int g = wave >> 1, hh = wave & 1;
   const int c16 = lane & 15, g4 = lane >> 4;
   const int t = k.t, h0 = k.hg * NHD;
@@ -881,16 +881,16 @@ int launch_tokens(const BwdParams& bp, const SasFwdArgs* a, bool b64, int ng, in
 struct PrePlan {
   bool on, sparse;   // sparse: some tokens may need per-token adds for their compressed rows
   int dense_thr, key_seg;
-  long long seg_groups, cmp_tiles, win_tiles;
+  long long seg_groups, cmp_tiles, win_tiles, first_tiles;
   size_t ws;
 };
-PrePlan plan_prefill(const SasBwdArgs* ba) {
+PrePlan plan_prefill(const SasBwdArgs* ba, long long first) {
   const SasFwdArgs* a = &ba->fwd;
   PrePlan r{};
   // q and dO reach LDS by DMA, 16 bytes a lane; the per-token kernels and the
   // window pass load them through registers, at any alignment
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(ba->dout)) & 15) return r;
-  const long long nslots = (long long)a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
+  const long long nslots = first + a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
   r.on = a->H % 32 == 0 && !(a->flags & SAS_BWD_WINDOW_TOKENS) && a->num_splits <= 0 &&
          ((a->flags & SAS_BWD_WINDOW_KEYS) || a->T >= 64 * a->B);
   if (!r.on) return r;
@@ -926,20 +926,16 @@ PrePlan plan_prefill(const SasBwdArgs* ba) {
   r.seg_groups = a->T / r.key_seg + a->B;
   r.win_tiles = std::min<long long>(((long long)a->win_left + r.key_seg + 2 * (kKeyRows - 1)) / kKeyRows,
                                     (a->ori_bt_stride * a->ori_block_size + kKeyRows - 1) / kKeyRows);
+  r.first_tiles = (std::min<long long>(first, a->ori_bt_stride * a->ori_block_size) + kKeyRows - 1) / kKeyRows;
   r.ws = (size_t)a->T * a->H * sizeof(float) + (size_t)a->T * (a->H / 8);   // Delta, non-finite marks
   if ((r.sparse && nslots > kMaxSlots) || r.ws == 0 ||
-      (double)(r.cmp_tiles + r.win_tiles) * (r.seg_groups + 64) * (a->H / 32) > 2e9)
+      (double)(r.cmp_tiles + r.win_tiles + r.first_tiles) * (r.seg_groups + 64) * (a->H / 32) > 2e9)
     return PrePlan{};
   return r;
 }
 
-}  // namespace
-}  // namespace sas
-
-extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
-  using namespace sas;
-  clear_error();
-  if (!ba) return set_error(SAS_EINVAL, "bwd: null args");
+// sas_bwd_v1, or (kBwdFirst) sas_bwd_first_v1
+int bwd_impl(const SasBwdArgs* ba, long long first, void* stream) {
   const SasFwdArgs* a = &ba->fwd;
   if (a->T < 0 || a->B < 1 || a->H < 1 || a->H % 16) return set_error(SAS_EINVAL, "bwd: bad T/B/H (H a multiple of 16)");
   if (a->D != 512 && a->D != 576) return set_error(SAS_EINVAL, "bwd: D must be 512 or 576");
@@ -948,8 +944,9 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
   if (a->q_dtype != SAS_DT_BF16 && a->q_dtype != SAS_DT_FP16) return set_error(SAS_EINVAL, "bwd: q dtype");
   if (a->kv_dtype != a->q_dtype) return set_error(SAS_EINVAL, "bwd: the cache must be in the query dtype (no fp8 rows)");
   if (a->win_left < 0) return set_error(SAS_EINVAL, "bwd: win_left out of range");
+  if (first < 0 || first > INT_MAX) return set_error(SAS_EINVAL, "bwd: ori_first out of range (got %lld)", first);
   if (a->scenario >= SAS_CFA && (a->cmp_ratio < 1 || a->K < 0)) return set_error(SAS_EINVAL, "bwd: bad cmp_ratio/K");
-  const long long nslots = (long long)a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
+  const long long nslots = first + a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
   if (a->T == 0) return SAS_OK;
   if (!a->q || !a->ori_kv || !a->ori_block_table || !a->q_prefix || !a->act_kv || !a->sinks ||
       !a->out || !a->lse || !ba->dout || !ba->dq || !ba->d_ori_kv || !ba->d_sinks)
@@ -985,7 +982,7 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
   fp.cmp_bt_stride = (int)std::max<int64_t>(a->cmp_bt_stride, 1);
   fp.cmp_nblocks = (int)a->cmp_num_blocks;
   fp.K = (int)a->K; fp.scenario = a->scenario;
-  fp.cmp_ratio = std::max(1, a->cmp_ratio); fp.win_left = a->win_left;
+  fp.cmp_ratio = std::max(1, a->cmp_ratio); fp.win_left = a->win_left; fp.first = (int)first;
   fp.scale_log2 = a->softmax_scale * kLog2e;
   // KV splits: the caller's count, else enough (token, head group, split)
   // workgroups to fill the CUs, each split at least 128 slots (C2, 640 slots
@@ -1045,7 +1042,7 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
   if ((a->flags & SAS_BWD_WINDOW_TOKENS) && (a->flags & SAS_BWD_WINDOW_KEYS))
     return set_error(SAS_EINVAL, "bwd: SAS_BWD_WINDOW_TOKENS and SAS_BWD_WINDOW_KEYS together");
   const bool direct = a->flags & SAS_BWD_DQ_DTYPE, have_ws = a->flags & SAS_BWD_WORKSPACE;
-  const PrePlan pre = plan_prefill(ba);
+  const PrePlan pre = plan_prefill(ba, first);
   if (direct && !(pre.on && have_ws))
     return set_error(SAS_EINVAL, "bwd: SAS_BWD_DQ_DTYPE without SAS_BWD_WORKSPACE or where sas_bwd_plan does not allow it");
   if (have_ws && pre.on && (!a->workspace || a->workspace_bytes < pre.ws))
@@ -1069,6 +1066,7 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
     bp.seg_groups = (int)pre.seg_groups;
     bp.cmp_tiles = (int)pre.cmp_tiles;
     bp.win_tiles_seg = (int)pre.win_tiles;
+    bp.first_tiles = (int)pre.first_tiles;
     if (pre.sparse) {
       // one split: every token's dq is written by one workgroup
       BwdParams sb = bp;
@@ -1080,8 +1078,12 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
       if (rc) return rc;
     }
     fp.slots_per_split = (int)((nslots + bp.npass - 1) / bp.npass);
-    return launch_bwd_prefill(bp, (int)a->D, a->q_dtype, (hipStream_t)stream);
+    return (kBwdFirst ? launch_bwd_prefill_first : launch_bwd_prefill)(bp, (int)a->D, a->q_dtype, (hipStream_t)stream);
   }
+#if SAS_BWD_FIRST
+  // (no window pass: first rows' adds would have to be told from window rows')
+  return launch_tokens(bp, a, b64, ng, nblocks, (hipStream_t)stream);
+#else
   const bool win = (a->flags & SAS_BWD_WINDOW_KEYS) ||
                    (!(a->flags & SAS_BWD_WINDOW_TOKENS) && !capturing && a->T >= 64 * a->B);
   long long win_blocks = 0;
@@ -1127,14 +1129,47 @@ extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
     }
   }
   return rc;
+#endif
 }
 
-extern "C" int sas_bwd_plan(const SasBwdArgs* ba, int32_t* dq_dtype, size_t* workspace_bytes) {
-  using namespace sas;
-  clear_error();
-  if (!ba) return set_error(SAS_EINVAL, "bwd: null args");
-  const PrePlan pre = ba->fwd.T >= 0 && ba->fwd.B >= 1 && ba->fwd.H >= 1 ? plan_prefill(ba) : PrePlan{};
+int plan_impl(const SasBwdArgs* ba, long long first, int32_t* dq_dtype, size_t* workspace_bytes) {
+  const PrePlan pre = ba->fwd.T >= 0 && ba->fwd.B >= 1 && ba->fwd.H >= 1 ? plan_prefill(ba, first) : PrePlan{};
   if (dq_dtype) *dq_dtype = pre.on;
   if (workspace_bytes) *workspace_bytes = pre.ws;
   return SAS_OK;
 }
+
+}  // namespace
+}  // namespace sas
+
+#if SAS_BWD_FIRST
+
+extern "C" int sas_bwd_first_v1(const SasBwdFirstArgs* a, void* stream) {
+  sas::clear_error();
+  if (!a) return sas::set_error(SAS_EINVAL, "bwd: null args");
+  return sas::bwd_impl(&a->bwd, a->ori_first, stream);
+}
+
+extern "C" int sas_bwd_first_plan(const SasBwdFirstArgs* a, int32_t* dq_dtype, size_t* workspace_bytes) {
+  sas::clear_error();
+  if (!a) return sas::set_error(SAS_EINVAL, "bwd: null args");
+  if (a->ori_first < 0 || a->ori_first > INT_MAX)
+    return sas::set_error(SAS_EINVAL, "bwd: ori_first out of range (got %lld)", (long long)a->ori_first);
+  return sas::plan_impl(&a->bwd, a->ori_first, dq_dtype, workspace_bytes);
+}
+
+#else
+
+extern "C" int sas_bwd_v1(const SasBwdArgs* ba, void* stream) {
+  sas::clear_error();
+  if (!ba) return sas::set_error(SAS_EINVAL, "bwd: null args");
+  return sas::bwd_impl(ba, 0, stream);
+}
+
+extern "C" int sas_bwd_plan(const SasBwdArgs* ba, int32_t* dq_dtype, size_t* workspace_bytes) {
+  sas::clear_error();
+  if (!ba) return sas::set_error(SAS_EINVAL, "bwd: null args");
+  return sas::plan_impl(ba, 0, dq_dtype, workspace_bytes);
+}
+
+#endif

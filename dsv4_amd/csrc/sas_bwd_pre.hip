@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
 
   for (int pass = 0; pass < bp.npass; ++pass) {
     k.sp = pass;
-    resolve<256, D * 2>(p, k, tid, lane, wave, [] {});
+    resolve<256, D * 2, false, false, kBwdFirst>(p, k, tid, lane, wave, [] {});
     if (pass == 0) {
       dl = lds_dl[16 * g + c16];   // behind resolve()'s barriers
       if (k.thr > bp.dense_thr) {         // the per-token kernel's token
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
   const FwdParams& p = bp.f;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c16 = lane & 15, g4 = lane >> 4;
-  const int nhg = p.H / 32, ntile = bp.cmp_tiles + bp.win_tiles_seg;
+  const int nhg = p.H / 32, ntile = bp.cmp_tiles + bp.win_tiles_seg + (kBwdFirst ? bp.first_tiles : 0);
   // (batch, segment) group gi on XCD (gi nhg + hg) % nxcd, its tiles adjacent there
   const unsigned nx = (unsigned)p.nxcd;
   const int x = (int)(blockIdx.x % nx), l = (int)(blockIdx.x / nx);
@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
   int a0 = seg * bp.key_seg, a1 = min(a0 + bp.key_seg, aqe);
   if (a0 + sg0 < 0) a0 = min(a1, -sg0);         // tokens before position 0 attend no row
   const bool cmp = tile < bp.cmp_tiles;
+  const bool head = kBwdFirst && tile >= bp.cmp_tiles + bp.win_tiles_seg;   // a tile of first rows
   int p0;                                       // the tile's first position
   if (cmp) {
     p0 = tile * kKeyRows;
@@ -388,6 +389,11 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
     if (lo > a0) a0 = (int)min(lo, (long long)a1);
     if (hi < a1) a1 = (int)max(hi, (long long)a0);
     if (p.scenario == SAS_CFA && p0 >= p.K) return;
+  } else if (head) {
+    p0 = (tile - bp.cmp_tiles - bp.win_tiles_seg) * kKeyRows;
+    // tokens whose window starts behind the tile's first row
+    const long long lo = (long long)p0 + p.win_left + 1 - sg0;
+    if (lo > a0) a0 = (int)min(lo, (long long)a1);
   } else {
     const int first = max(0, sg0 + a0 - p.win_left) / kKeyRows;
     p0 = (first + tile - bp.cmp_tiles) * kKeyRows;
@@ -571,6 +577,7 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
       int n = cnt;
       if (list) {}
       else if (cmp) n = pos < (sg + 1) / p.cmp_ratio && pos < p.K;
+      else if (head) n = pos < p.first && pos < sg - p.win_left;
       else n = pos <= sg && pos >= sg - p.win_left;
       if (!rok) n = 0;
       float pr[4], ds[4];
@@ -699,7 +706,8 @@ int launch(const BwdParams& bp, hipStream_t st) {
   b.f.nhg = nhg;
   b.f.nsplit = 1;
   const long long nb = (p.T + nx - 1) / nx * nx * nhg;
-  const long long kb = ((long long)bp.seg_groups * (p.H / 32) + nx - 1) / nx * nx * (bp.cmp_tiles + bp.win_tiles_seg);
+  const long long kb = ((long long)bp.seg_groups * (p.H / 32) + nx - 1) / nx * nx *
+                       (bp.cmp_tiles + bp.win_tiles_seg + (kBwdFirst ? bp.first_tiles : 0));
   if (nb > INT_MAX || kb > INT_MAX) return set_error(SAS_EINVAL, "bwd: %lld workgroups beyond one launch", std::max(nb, kb));
   if (bwd_dq_heads(p.H) == 64) hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 4>), dim3((unsigned)nb), dim3(512), 0, st, b);
   else hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 2>), dim3((unsigned)nb), dim3(256), 0, st, b);
@@ -712,7 +720,11 @@ int launch(const BwdParams& bp, hipStream_t st) {
 
 }  // namespace
 
+#if SAS_BWD_FIRST
+int launch_bwd_prefill_first(const BwdParams& bp, int D, int q_dtype, hipStream_t st) {
+#else
 int launch_bwd_prefill(const BwdParams& bp, int D, int q_dtype, hipStream_t st) {
+#endif
   if (q_dtype == SAS_DT_BF16) return D == 576 ? launch<576, __bf16>(bp, st) : launch<512, __bf16>(bp, st);
   return D == 576 ? launch<576, _Float16>(bp, st) : launch<512, _Float16>(bp, st);
 }

@@ -49,6 +49,9 @@
 #ifndef SAS_FWD_TREE
 #define SAS_FWD_TREE 0   // 1 (sas_fwd_tree.hip): the same kernels over draft trees
 #endif
+#ifndef SAS_FWD_FIRST
+#define SAS_FWD_FIRST 0  // 1 (sas_fwd_first.hip): the same kernels with first rows that stay visible
+#endif
 #ifndef SAS_PFK
 #define SAS_PFK 3   // K operand k-steps read ahead (32-row steps)
 #endif
@@ -76,6 +79,7 @@ namespace sas {
 namespace {
 
 constexpr bool kTree = SAS_FWD_TREE;
+constexpr bool kFirst = SAS_FWD_FIRST;
 
 // ---------------------------------------------------------------------------
 // forward kernel
@@ -1673,7 +1677,7 @@ sas_fwd_kernel(const FwdParams p) {
   if constexpr (C::QL) {
     if (wave >= 4) f.q_dma(k, wave);
   }
-  resolve<256, C::ROWB, kTree>(p, k, tid, lane, wave, [&] {
+  resolve<256, C::ROWB, kTree, false, kFirst>(p, k, tid, lane, wave, [&] {
     if constexpr (C::QL) return;
     const uint4* qp = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq) * D * 2);
 #pragma unroll
@@ -1887,7 +1891,7 @@ sas_dec_kernel(const FwdParams p) {
   if (item < 0) return;
   Tok k = item_of(p, item);
   C f(p, lane);
-  resolve<256, C::ROWB, kTree>(p, k, tid, lane, wave, [] {});
+  resolve<256, C::ROWB, kTree, false, kFirst>(p, k, tid, lane, wave, [] {});
   const int nvalid = __builtin_amdgcn_readfirstlane(k.nvalid);
   const int hq = k.hg * 16 + f.c16;
   // key-group share of wave `wave`: whole 16-row steps, wave 0 first
@@ -1961,7 +1965,7 @@ struct Plan {
   size_t ws;
 };
 
-int make_plan(const SasFwdArgs* a, Plan* pl) {
+int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   if (!a) return sas::set_error(SAS_EINVAL, "null args");
   if (a->T < 0 || a->B < 1 || a->H < 1) return sas::set_error(SAS_EINVAL, "bad T/B/H");
   if (a->D != 512 && a->D != 576) return sas::set_error(SAS_EINVAL, "D must be 512 or 576 (got %lld)", (long long)a->D);
@@ -1971,10 +1975,11 @@ int make_plan(const SasFwdArgs* a, Plan* pl) {
   if (a->flags & ~SAS_FWD_NO_COMBINE) return sas::set_error(SAS_EINVAL, "unknown flags 0x%x", a->flags);
   if (a->win_left < 0) return sas::set_error(SAS_EINVAL, "win_left out of range");
   if (a->scenario >= SAS_CFA && (a->cmp_ratio < 1 || a->K < 0)) return sas::set_error(SAS_EINVAL, "bad cmp_ratio/K");
-  const long long nslots_ll = (long long)a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
+  if (first < 0 || first > INT_MAX) return sas::set_error(SAS_EINVAL, "ori_first out of range (got %lld)", first);
+  const long long nslots_ll = first + a->win_left + 1 + (a->scenario >= SAS_CFA ? a->K : 0);
   if (nslots_ll > kMaxTokenSlots)
-    return sas::set_error(SAS_EINVAL, "%lld key slots per token (win_left + 1 + K) beyond %lld", nslots_ll,
-                          kMaxTokenSlots);
+    return sas::set_error(SAS_EINVAL, "%lld key slots per token (%swin_left + 1 + K) beyond %lld", nslots_ll,
+                          kFirst ? "ori_first + " : "", kMaxTokenSlots);
   pl->nslots = (int)nslots_ll;
   const long long T = std::max<long long>(a->T, 1);
   int hw = a->head_waves;
@@ -2250,10 +2255,10 @@ bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
 }
 #endif
 
-// sas_fwd_v1, or (kTree) sas_fwd_tree_v1
-int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, void* stream) {
+// sas_fwd_v1, or (kTree) sas_fwd_tree_v1, or (kFirst) sas_fwd_first_v1
+int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, long long first, void* stream) {
   Plan pl;
-  int rc = make_plan(a, &pl);
+  int rc = make_plan(a, first, &pl);
   if (rc) return rc;
   if (a->T == 0) return SAS_OK;
   if (!a->q || !a->ori_kv || !a->ori_block_table || !a->q_prefix || !a->act_kv ||
@@ -2321,9 +2326,10 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, voi
   fp.out_nt = pl.nsplit == 1 && (size_t)a->T * a->H * kDV * 2 >= (size_t(16) << 20);
   fp.tree = tree_mask;
   fp.tree_words = tree_words;
+  fp.first = (int)first;
   hipStream_t st = (hipStream_t)stream;
 
-  if constexpr (!kTree) {   // (runs of tokens are chains)
+  if constexpr (!kTree && !kFirst) {   // (runs of tokens are chains)
     if (const int run = win_run(a, pl)) return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
     if (const int run = dense_run(a, pl)) {
       fp.nhg = (int)a->H / 64;
@@ -2361,7 +2367,26 @@ extern "C" int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream) {
     return sas::set_error(SAS_EINVAL, "tree_words must be 1 to 64 (got %lld)", (long long)a->tree_words);
   if (a->fwd.T > 0 && (!a->tree_mask || (uintptr_t)a->tree_mask % 8))
     return sas::set_error(SAS_EINVAL, "tree_mask must be an 8-byte aligned device pointer");
-  return fwd_impl(&a->fwd, a->tree_mask, (int)a->tree_words, stream);
+  return fwd_impl(&a->fwd, a->tree_mask, (int)a->tree_words, 0, stream);
+}
+
+#elif SAS_FWD_FIRST
+
+extern "C" int sas_fwd_first_plan(const SasFwdFirstArgs* a, int32_t* num_splits, size_t* workspace_bytes) {
+  sas::clear_error();
+  if (!a) return sas::set_error(SAS_EINVAL, "null args");
+  Plan pl;
+  const int rc = make_plan(&a->fwd, a->ori_first, &pl);
+  if (rc) return rc;
+  if (num_splits) *num_splits = pl.nsplit;
+  if (workspace_bytes) *workspace_bytes = pl.ws;
+  return SAS_OK;
+}
+
+extern "C" int sas_fwd_first_v1(const SasFwdFirstArgs* a, void* stream) {
+  sas::clear_error();
+  if (!a) return sas::set_error(SAS_EINVAL, "null args");
+  return fwd_impl(&a->fwd, nullptr, 0, a->ori_first, stream);
 }
 
 #else
@@ -2369,7 +2394,7 @@ extern "C" int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream) {
 extern "C" int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* workspace_bytes) {
   sas::clear_error();
   Plan pl;
-  const int rc = make_plan(a, &pl);
+  const int rc = make_plan(a, 0, &pl);
   if (rc) return rc;
   if (num_splits) *num_splits = pl.nsplit;
   if (workspace_bytes) *workspace_bytes = pl.ws;
@@ -2378,7 +2403,7 @@ extern "C" int sas_fwd_plan(const SasFwdArgs* a, int32_t* num_splits, size_t* wo
 
 extern "C" int sas_fwd_v1(const SasFwdArgs* a, void* stream) {
   sas::clear_error();
-  return fwd_impl(a, nullptr, 0, stream);
+  return fwd_impl(a, nullptr, 0, 0, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -2430,7 +2455,7 @@ int scratch_ptr(hipStream_t st, void** out) {
 extern "C" int sas_fwd_noalloc_v1(const SasFwdArgs* a, void* stream) {
   sas::clear_error();
   Plan pl;
-  const int rc = make_plan(a, &pl);
+  const int rc = make_plan(a, 0, &pl);
   if (rc) return rc;
   if (a->flags & SAS_FWD_NO_COMBINE)
     return sas::set_error(SAS_EINVAL, "no-alloc forward: SAS_FWD_NO_COMBINE would leave the partials in the "

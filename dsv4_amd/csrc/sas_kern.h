@@ -132,6 +132,7 @@ struct FwdParams {
   int out_nt;    // 1: the output (one split) goes out with non-temporal stores
   const uint64_t* tree;   // draft trees: [T, tree_words] attended slots of the token's sequence
   int tree_words;         // 64-slot words a token, at most 64
+  int first;              // first rows that stay visible (sas_fwd_first.hip): slots before the window's
 };
 
 // ---------------------------------------------------------------------------
@@ -477,8 +478,9 @@ struct Tree {
 // block-table loads are issued (a caller can put its own loads behind them
 // there).
 // With LIST the rows go to `list` instead, as 32-bit cache row indices (bit 31: a
-// compressed row).
-template <int NT, int ROWB, bool TREE = false, bool LIST = false, typename Mid>
+// compressed row). With FIRST the first p.first slots are the cache's first rows,
+// as far as the window starts behind them; the window's slots follow.
+template <int NT, int ROWB, bool TREE = false, bool LIST = false, bool FIRST = false, typename Mid>
 __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int lane, int wave, Mid&& mid,
                                         uint32_t* list = nullptr) {
   constexpr int NWV = NT / 64;
@@ -486,7 +488,8 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
   static_assert(kRounds <= kRoundsMax && NWV <= kMaxWaves, "resolve geometry");
   const bool worker = tid < NT;   // wave-uniform
   const int t = k.t;
-  const int wincap = p.win_left + 1;
+  const int nfirst = FIRST ? p.first : 0;
+  const int wincap = p.win_left + 1 + nfirst;
   const int nslots = wincap + (p.scenario >= SAS_CFA ? p.K : 0);
   const int s0 = k.sp * p.slots_per_split;
   const int s1 = min(s0 + p.slots_per_split, nslots);
@@ -562,10 +565,11 @@ __device__ __forceinline__ void resolve(const FwdParams& p, Tok& k, int tid, int
       if (TREE && s0 + r * NT < wincap) draft = tree.slot(tree.count - nwin + j);   // wave-uniform
       int blk;
       if (j < wincap) {
-        const int pos = TREE && j >= nwin - path ? max(akv - aq + draft, 0) : wlo + j;
+        const int w = j - nfirst;   // window slot (below 0: first row j)
+        const int pos = TREE && j >= nwin - path ? max(akv - aq + draft, 0) : FIRST && w < 0 ? j : wlo + w;
         blk = pos / p.ori_bs;
         off[r] = pos - blk * p.ori_bs;
-        ok[r] = live && j < nwin && blk < p.ori_bt_stride;
+        ok[r] = live && (FIRST && w < 0 ? j < wlo : w < nwin) && blk < p.ori_bt_stride;
       } else {
         const int idx = p.scenario == SAS_SCFA ? idxv[r] : j - wincap;
         const int ic = max(idx, 0);

@@ -222,6 +222,22 @@ typedef struct SasFwdTreeArgs {
 int sas_fwd_tree_v1(const SasFwdTreeArgs* a, void* stream);
 
 /*
+ * The forward with first rows that stay visible beside the window (no counterpart in
+ * the reference, whose window drops them): a token at position s attends the rows j <= s
+ * of the raw cache with j >= s - win_left or j < ori_first, each once, and compressed
+ * rows as ever. Blocks of rows that are neither may be missing (-1). ori_first 0 is
+ * sas_fwd_v1's own mask. Plan and workspace are sas_fwd_first_plan's; win_left + 1 +
+ * ori_first takes win_left + 1's place in what SasFwdArgs says of slots.
+ */
+typedef struct SasFwdFirstArgs {
+  SasFwdArgs fwd;
+  int64_t ori_first;
+} SasFwdFirstArgs;
+
+int sas_fwd_first_plan(const SasFwdFirstArgs* a, int32_t* num_splits, size_t* workspace_bytes);
+int sas_fwd_first_v1(const SasFwdFirstArgs* a, void* stream);
+
+/*
  * sas_fwd_v1 without any allocation by caller or library, for callers that
  * cannot allocate device memory (code under HIP graph capture, tight serving
  * loops, harnesses that forbid hipMalloc). No counterpart in the reference.
@@ -297,6 +313,69 @@ int sas_bwd_v1(const SasBwdArgs* a, void* stream);
    window flags and whether q and dout are 16-byte aligned (the prefill path
    takes no others). */
 int sas_bwd_plan(const SasBwdArgs* a, int32_t* dq_dtype, size_t* workspace_bytes);
+
+/*
+ * Backward of sas_fwd_first_v1: sas_bwd_v1's contract over that forward's keys. The
+ * first rows' gradients are summed with the window rows': key-major where sas_bwd_v1
+ * takes its prefill path (sas_bwd_first_plan reports its workspace), else one add per
+ * (token, row, head group, channel); SAS_BWD_WINDOW_KEYS means the former alone.
+ */
+typedef struct SasBwdFirstArgs {
+  SasBwdArgs bwd;
+  int64_t ori_first;
+} SasBwdFirstArgs;
+
+int sas_bwd_first_plan(const SasBwdFirstArgs* a, int32_t* dq_dtype, size_t* workspace_bytes);
+int sas_bwd_first_v1(const SasBwdFirstArgs* a, void* stream);
+
+/*
+ * The weight that a call's tokens give each cache row (no counterpart in the
+ * reference), added to what the caller holds:
+ *   ori_weights[b][j] += mean over heads h of sum over tokens t of b of
+ *                        exp(softmax_scale q[t][h] . k_j - lse[t][h])
+ * over the raw rows j of sequence b that token t attends (window, and rows below
+ * ori_first, as in sas_fwd_first_v1), and cmp_weights[b][j] over its compressed rows. fwd
+ * holds the forward's arguments, its lse an input (q and lse 16-byte aligned); sinks, out,
+ * workspace, num_splits, head_waves, waves and flags are ignored, and of a cache whose
+ * weights are NULL everything. A row listed twice counts twice. Rows without a block, and
+ * those past the weights' rows, are skipped. Every added value is a multiple of 2^-36 (the
+ * fp32 sum rounded to it): weights below 2^17 are exact sums, the same bits in any order of
+ * calls and tokens. NaN and infinities propagate.
+ */
+typedef struct SasRowWeightsArgs {
+  SasFwdArgs fwd;
+  int64_t ori_first;
+  double* ori_weights;           /* [B, ori_rows] or NULL */
+  double* cmp_weights;           /* [B, cmp_rows] or NULL */
+  int64_t ori_rows, cmp_rows;
+} SasRowWeightsArgs;
+
+int sas_row_weights_v1(const SasRowWeightsArgs* a, void* stream);
+
+/*
+ * Eviction (no counterpart in the reference): of each sequence b with more than `budget`
+ * rows stay rows [0, keep_first), the last keep_recent ones and, of the others, the
+ * heaviest (of equal weights those at the lowest positions; NaN counts as the least, a
+ * row past weight_rows as 0), `budget` rows in all. They move together in their order, in
+ * place through the block table, their weights with them; the weights of rows [budget,
+ * act_kv[b]) become 0, cache rows there keep their bytes. kept[b] lists the old positions
+ * of the rows that stay, -1 past them; act_kv_out[b] is min(act_kv[b], budget) (act_kv_out
+ * may be act_kv). Sequences of at most `budget` rows stay as they are. A row whose source
+ * or destination has no block is not moved. No two sequences may share a block.
+ */
+typedef struct SasCacheEvictArgs {
+  void* cache;                   /* [num_blocks, block_size, row_bytes] bytes */
+  double* weights;               /* [B, weight_rows] */
+  const int32_t* block_table;    /* [B, bt_stride] */
+  const int32_t* act_kv;         /* [B] */
+  int32_t* act_kv_out;           /* [B] */
+  int32_t* kept;                 /* [B, budget] */
+  int64_t B, row_bytes;          /* row_bytes: a multiple of 16 */
+  int64_t bt_stride, block_size, num_blocks;
+  int64_t weight_rows, budget, keep_first, keep_recent;
+} SasCacheEvictArgs;
+
+int sas_cache_evict_v1(const SasCacheEvictArgs* a, void* stream);
 
 /*
  * Paged-KV cache writer (no counterpart in the reference, whose tests build
