@@ -359,8 +359,8 @@ int sas_row_weights_v1(const SasRowWeightsArgs* a, void* stream);
  * row past weight_rows as 0), `budget` rows in all. They move together in their order, in
  * place through the block table, their weights with them; the weights of rows [budget,
  * act_kv[b]) become 0, cache rows there keep their bytes. kept[b] lists the old positions
- * of the rows that stay, -1 past them; act_kv_out[b] is min(act_kv[b], budget) (act_kv_out
- * may be act_kv). Sequences of at most `budget` rows stay as they are. A row whose source
+ * of the rows that stay, -1 past them; act_kv_out[b] is min(act_kv[b], budget), in memory of
+ * its own. Sequences of at most `budget` rows stay as they are. A row whose source
  * or destination has no block is not moved. No two sequences may share a block.
  */
 typedef struct SasCacheEvictArgs {

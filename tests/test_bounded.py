@@ -812,6 +812,41 @@ def test_gpu_evict_odd_weights():
 
 
 @pytest.mark.gpu
+def test_gpu_evict_nan_beside_equal_weights():
+    """Whole waves of NaN, others of one weight each side of them in the order."""
+    for other in (-float("inf"), 5e-324, float("inf")):
+        a = _evict_case([2000], 1200, 2, 3)
+        a[1][:] = float("nan")
+        a[1][0, 500:1300] = other
+        _same(_evict(*a), R.evict(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [4096, 4097, 32768, 32769, 40000])
+def test_gpu_evict_long(n):
+    """Each side of the lengths that the selection keeps in registers."""
+    for budget, zero in ((n - 1, 0.3), (1000, 0.3), (n // 2, 0.9)):
+        a = _evict_case([n, 50], budget, 4, 64, bs=64, row=8, zero=zero)
+        _same(_evict(*a), R.evict(*a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3000, 9000, 33000])
+@pytest.mark.parametrize("spread", [50, 1 << 20, 1 << 45])
+def test_gpu_evict_close_weights(n, spread):
+    """Weights that differ in their last bits only, or in those and a few above, with NaN,
+    zeros and infinities around them; the edge at each end and in the middle."""
+    a = _evict_case([n], 10, 2, 3, bs=64, row=8)
+    g = torch.Generator().manual_seed(2)
+    a[1][:] = 1.0 + torch.randint(0, spread, a[1].shape, generator=g).double() * 2.0 ** -52
+    a[1][0, 40:80], a[1][0, 100:300], a[1][0, 350:360] = float("nan"), 0.0, float("inf")
+    a[1][0, 400:500] = -a[1][0, 400:500]
+    for budget in (12, 16, 200, n // 2, n - 400, n - 200, n - 45, n - 20):
+        b = a[:4] + (budget, 2, 3)
+        _same(_evict(*b), R.evict(*b))
+
+
+@pytest.mark.gpu
 def test_gpu_evict_rows_without_blocks():
     """A moved row needs both blocks; entries out of range count as none, nothing is
     read or written through them."""
