@@ -6,12 +6,11 @@
 // are exact: whatever order the adds of workgroups, tokens and calls come in, the bits
 // are the same. Products, exponentials and a workgroup's own sums are fp32.
 //
-// A workgroup (4 waves) owns 64 RT slots of one token, slots being its first rows, its
-// window and its compressed rows without gaps. A wave holds the K fragments of its 16 RT
-// rows in registers, loaded straight from the cache (16 bytes a lane: the MFMA's B
-// operand), and the queries, 16 heads at a time, reach LDS by DMA, four tiles deep, one
-// barrier a tile: S[head][row] = Q . K^T (16x16x32 MFMA), P = 2^(S - lse), summed over
-// the lane's four heads, over tiles, and last over the four lane groups.
+// Rows stay with a wave, as K fragments in registers loaded straight from the cache (16
+// bytes a lane: the MFMA's B operand), and queries reach LDS by DMA, 16 heads of one token at
+// a time, one barrier a tile: S[head][row] = Q . K^T (16x16x32 MFMA), P = 2^(S - lse), summed
+// over the lane's four heads, over tiles, and last over the four lane groups. One kernel
+// for the slots of single tokens, one for rows that several tokens attend.
 
 #include "sas_kern.h"
 
@@ -60,15 +59,140 @@ __device__ __forceinline__ void add_weight(double* at, float sum, double units) 
   unsafeAtomicAdd(at, rint((double)sum * units) * (1. / kGrid));
 }
 
-template <int D, typename QT, bool F8, int RT>
-__global__ void __launch_bounds__(256, 2) sas_weights_kernel(const WeightParams wp) {
-  constexpr int CH = D / 8, KS = D / 32, SG = kSwzGroup<CH>;
-  constexpr int NI = 16 * CH / 64, OPS = (NI + 3) / 4;   // DMA instructions a query tile, and a wave's most
-  constexpr int NB = 4;                                  // query tiles in LDS
-  constexpr int ROWS = 64 * RT;
-  static_assert(NI * 64 == 16 * CH, "whole instructions");
-  __shared__ __attribute__((aligned(1024))) uint4 lq[NB][16 * CH];
-  __shared__ __attribute__((aligned(16))) float ll[NB][256];   // a tile's 16 lse (written 16 times over)
+// A row's K fragments: lane group g holds channels 32 ks + 8 g .. of k-step ks; of fp8 rows the
+// latent values of two k-steps from one 16-byte load (the queries' fragments follow), and
+// the row's scales.
+template <int D, bool F8>
+__device__ __forceinline__ void load_row(uint64_t row, int g, uint4 (&k)[D / 32], float (&sc)[F8 ? 4 : 1]) {
+  if constexpr (F8) {
+    uint4 raw[8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m) raw[m] = gld16(row + (4 * m + g) * 16);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) k[16 + m] = gld16(row + 528 + (4 * m + g) * 16);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) sc[m] = gldf(row + 512 + 4 * m);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      e4m3x4_to_bf16(raw[m].x, k[2 * m].x, k[2 * m].y);
+      e4m3x4_to_bf16(raw[m].y, k[2 * m].z, k[2 * m].w);
+      e4m3x4_to_bf16(raw[m].z, k[2 * m + 1].x, k[2 * m + 1].y);
+      e4m3x4_to_bf16(raw[m].w, k[2 * m + 1].z, k[2 * m + 1].w);
+    }
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) k[ks] = gld16(row + (4 * ks + g) * 16);
+  }
+}
+
+// The queries' way into LDS: tiles of 16 heads of one token, D channels each and their 16
+// lse, by DMA of a workgroup's four waves.
+template <int D>
+struct Queries {
+  static constexpr int CH = D / 8, SG = kSwzGroup<CH>;
+  static constexpr int NI = 16 * CH / 64, OPS = (NI + 3) / 4;   // instructions a tile, and a wave's most
+  static_assert(NI * 64 == 16 * CH && NI / 4 == 4 && NI % 4 < 3, "four instructions a wave; the left-over ones and the lse make five");
+  struct Tile {
+    uint4 q[16 * CH];      // chunk c of head r at c ^ swz(r), in its swizzle group
+    float lse[256];        // 16 of them, 16 times over
+  };
+  const uint8_t* q;
+  const float* lse;
+  int wave, lane;
+  uint32_t off[OPS];
+  bool wide;               // five instructions a tile, else four
+  __device__ __forceinline__ Queries(const FwdParams& p, size_t token, int wave_, int lane_)
+      : q(p.q + token * p.H * D * 2), lse(p.lse + token * p.H), wave(wave_), lane(lane_),
+        wide(wave_ == 3 || wave_ < NI % 4) {
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) {
+      const int P = (o * 4 + wave) * 64 + lane, r = P / CH;
+      off[o] = (uint32_t)(r * CH + ((P - r * CH) ^ swz<CH>(r))) * 16;
+    }
+  }
+  // tile i, counted from the first token's first
+  __device__ __forceinline__ void issue(Tile& to, int i) const {
+    const uint32_t dst = lds_addr_of(to.q);
+#pragma unroll
+    for (int o = 0; o < OPS; ++o)
+      if (o * 4 + wave < NI)   // uniform
+        dma16s(off[o], q + (size_t)i * 16 * D * 2, __builtin_amdgcn_readfirstlane(dst + (o * 4 + wave) * 1024));
+    if (wave == 3) dma16s((uint32_t)(lane & 3) * 16, lse + (size_t)i * 16, __builtin_amdgcn_readfirstlane(lds_addr_of(to.lse)));
+  }
+  // all but the `n` newest tiles are here
+  __device__ __forceinline__ void wait(int n) const {
+    if (wide) n == 2 ? wait_vm<10>() : n == 1 ? wait_vm<5>() : wait_vm<0>();
+    else n == 2 ? wait_vm<8>() : n == 1 ? wait_vm<4>() : wait_vm<0>();
+  }
+  // a tile's fragment of k-step ks for lane group g, head c16; of fp8 rows as load_row() has them
+  template <bool F8>
+  static __device__ __forceinline__ uint4 frag(const Tile& t, int ks, int g, int c16) {
+    const int L = F8 && ks < 16 ? 8 * (ks >> 1) + 2 * g + (ks & 1) : 4 * ks + g;
+    return t.q[c16 * CH + ((L & -SG) | ((L & (SG - 1)) ^ swz<CH>(c16)))];
+  }
+};
+
+// S[head][row] of a tile against RT row tiles. PF fragments are read ahead; work(), VALU
+// work of another tile, goes between the MFMAs.
+template <int D, typename QT, bool F8, int RT, int PF, typename Work>
+__device__ __forceinline__ void tile_scores(const typename Queries<D>::Tile& t, const uint4 (&k)[RT][D / 32],
+                                            const float (&sc)[RT][F8 ? 4 : 1], int g, int c16, f32x4 (&s)[RT], Work&& work) {
+  constexpr int KS = D / 32;
+  f32x4 part[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint4 a[PF];
+#pragma unroll
+  for (int ks = 0; ks < PF; ++ks) a[ks] = Queries<D>::template frag<F8>(t, ks, g, c16);
+  work();
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const uint4 q = a[ks % PF];
+    if (ks + PF < KS) a[ks % PF] = Queries<D>::template frag<F8>(t, ks + PF, g, c16);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (F8 && ks < 16) {
+        // one scale's 128 channels at a time, unscaled e4m3 values (exact in bf16)
+        part[rt] = mfma32k<QT>(q, k[rt][ks], ks % 4 == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[rt]);
+        if (ks % 4 == 3) s[rt] += part[rt] * sc[rt][F8 ? ks / 4 : 0];
+      } else {
+        s[rt] = mfma32k<QT>(q, k[rt][ks], s[rt]);
+      }
+    }
+  }
+  if constexpr (!F8 && RT > 1) {
+    __builtin_amdgcn_sched_group_barrier(0x100, PF + 1, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x008, RT, 0);
+      if (ks + PF < KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, RT, 0);
+    }
+  }
+}
+
+// The sum over the lane's four heads of 2^(scale S - lse).
+__device__ __forceinline__ float shares(const f32x4& s, const f32x4& lse2, float scale_log2) {
+  float x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_exp2f(s[j] * scale_log2 - lse2[j]);
+  return (x[0] + x[1]) + (x[2] + x[3]);
+}
+
+// ---------------------------------------------------------------------------
+// slots of one token
+// ---------------------------------------------------------------------------
+//
+// A workgroup owns 64 slots of one token, slots being its first rows, its window and its
+// compressed rows without gaps, 16 to a wave. HBM-bound where the rows are many; short
+// workgroups, four to a CU, keep the last round of a grid short (32 tokens of 64 heads over
+// 2000 rows, 576 channels: 26.2 us a call with 128 slots, two to a CU, 23.7 with 64; one
+// token 13.9 and 10.9).
+template <int D, typename QT, bool F8>
+__global__ void __launch_bounds__(256, 4) sas_weights_kernel(const WeightParams wp) {
+  using Q = Queries<D>;
+  constexpr int NB = 2, ROWS = 64;
+  __shared__ __attribute__((aligned(1024))) typename Q::Tile tiles[NB];
 
   const FwdParams& p = wp.f;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -99,135 +223,299 @@ __global__ void __launch_bounds__(256, 2) sas_weights_kernel(const WeightParams 
     thr = (sg + 1) / p.cmp_ratio;
     ns = nr + (p.scenario == SAS_SCFA ? p.K : min(min(thr, p.K), wp.cmp_cap));
   }
-  const int s0 = chunk * ROWS + wave * 16 * RT;
   if (chunk * ROWS >= ns) return;                        // uniform
 
-  // queries: tile i of the token's H / 16 goes to buffer i % NB
   const int ntile = p.H / 16;
-  const uint8_t* qb = p.q + (size_t)t * p.H * D * 2;
-  const float* lb = p.lse + (size_t)t * p.H;
-  uint32_t qoff[OPS];
-#pragma unroll
-  for (int o = 0; o < OPS; ++o) {
-    const int P = (o * 4 + wave) * 64 + lane, r = P / CH;
-    qoff[o] = (uint32_t)(r * CH + ((P - r * CH) ^ swz<CH>(r))) * 16;
+  const Q queries(p, (size_t)t, wave, lane);
+  queries.issue(tiles[0], 0);
+
+  // lane (g, c16) holds slot 16 wave + c16 of the chunk (all four g)
+  const int s = chunk * ROWS + wave * 16 + c16;
+  const bool ori = s < nr;
+  int pos = s < nf ? s : wlo + s - nf;
+  bool ok = s < ns;
+  if (!ori) {
+    pos = s - nr;
+    if (p.scenario == SAS_SCFA && ok) pos = p.cmp_idx[(size_t)t * p.K + pos];
+    ok = ok && pos >= 0 && pos < thr;
   }
-  const bool wide = wave == 3 || (NI % 4 != 0 && wave < NI % 4);   // five instructions a tile, else four
-  static_assert(NI / 4 == 4 && NI % 4 < 3 && NB == 4, "instructions a tile: four, the left-over ones, wave 3's lse");
-  auto issue = [&](int i) {
-    const uint32_t dst = lds_addr_of(lq[i % NB]);
+  const int bs = ori ? p.ori_bs : p.cmp_bs, blk = max(pos, 0) / bs;
+  const int stride = ori ? p.ori_bt_stride : p.cmp_bt_stride;
+  ok = ok && blk < stride && pos < (ori ? wp.ori_rows : wp.cmp_rows);
+  const int32_t* bt = ori ? p.ori_bt : p.cmp_bt;
+  const int phys = ok ? bt[(size_t)at.b * stride + blk] : -1;
+  ok = ok && phys >= 0 && phys < (ori ? p.ori_nblocks : p.cmp_nblocks);
+  constexpr int ROWB = F8 ? kRow656 : D * 2;
+  // (a row that is not there: the query's bytes, masked out)
+  const uint64_t row = ok ? reinterpret_cast<uint64_t>(ori ? p.ori_kv : p.cmp_kv) +
+                                (uint64_t)(uint32_t)(phys * bs + pos - blk * bs) * ROWB
+                          : reinterpret_cast<uint64_t>(queries.q);
+  uint4 k[1][D / 32];
+  float sc[1][F8 ? 4 : 1];
+  load_row<D, F8>(row, g, k[0], sc[0]);
+
+  float acc = 0.f;
+  // the K fragments and the first tile's DMA: known to the compiler to be done, so none
+  // of its waits falls into the loop
+  __builtin_amdgcn_s_waitcnt(0);
+  for (int i = 0; i < ntile; ++i) {
+    if (i > 0) queries.wait(0);
+    lds_barrier();   // every wave's part of tile i is here, and tile i - 1 is read
+    if (i + 1 < ntile) queries.issue(tiles[(i + 1) % NB], i + 1);
+    const typename Q::Tile& tile = tiles[i % NB];
+    const f32x4 l2 = *reinterpret_cast<const f32x4*>(&tile.lse[4 * g]) * kLog2e;
+    f32x4 x[1];
+    tile_scores<D, QT, F8, 1, 4>(tile, k, sc, g, c16, x, [] {});
+    acc += shares(x[0], l2, p.scale_log2);
+  }
+  const float w = rows_sum(acc);
+  if (g == 0 && ok)
+    add_weight((ori ? wp.ori_w + (size_t)at.b * wp.ori_rows : wp.cmp_w + (size_t)at.b * wp.cmp_rows) + pos, w, wp.units);
+}
+
+// ---------------------------------------------------------------------------
+// rows of several tokens
+// ---------------------------------------------------------------------------
+//
+// A prompt's end, a chunk, drafts: the rows are keys of many tokens, so a workgroup keeps
+// 128 consecutive rows of a sequence (raw ones of the windows, first ones that a window
+// has left behind, or compressed ones), 32 to a wave, and streams a segment of the tokens
+// that attend any of them, a tile of 16 heads at a time; the exponentials of one tile stand
+// between the MFMAs of the next. Two workgroups a CU: 64 tokens of 64 heads over 20000 and
+// 32768 rows of 512 channels at 1.05 PFLOP/s, the rate of a large matrix product; a wave
+// with 64 rows (half the LDS reads, but alone on its SIMD) 297 us for 228, with 48 rows 295.
+// Tiles of at most 32 rows (a few first rows: keys of every token behind them) are held by
+// all four waves, which take four tiles of queries at once.
+
+struct RowParts {
+  int seg;                        // tokens a segment
+  int win_blocks, first_blocks;   // workgroups of window tiles, then of first rows' tiles; compressed ones follow
+};
+
+// Part, sequence, tile and segment of a workgroup: tiles x segments of the part's sequences one
+// after the other.
+struct RowItem {
+  int part;                  // 0 window, 1 first rows, 2 compressed
+  int b, p0, rows;           // sequence; the tile's first position and how many
+  int a0, a1;                // its tokens, offsets in the sequence
+  int qp, sg0;               // packed index of the sequence's first token, its position
+};
+
+template <int ROWS>
+__device__ __forceinline__ bool find_item(const WeightParams& wp, const RowParts& rp, int blk, int lane, RowItem& o) {
+  const FwdParams& p = wp.f;
+  o.part = blk < rp.win_blocks ? 0 : blk < rp.win_blocks + rp.first_blocks ? 1 : 2;
+  const int at = blk - (o.part == 0 ? 0 : o.part == 1 ? rp.win_blocks : rp.win_blocks + rp.first_blocks);
+  const bool cu = p.act_q == nullptr;
+  long long base = 0;
+  for (int c = 0; c < p.B; c += 64) {
+    const int i = c + lane;
+    int qp = 0, aq = 0, sg0 = 0, lo = 0, hi = 0, nseg = 0;
+    if (i < p.B) {
+      qp = p.q_prefix[i];
+      const int next = i + 1 < p.B ? p.q_prefix[i + 1] : p.T;
+      const int len = cu ? p.q_prefix[i + 1] - qp : p.act_q[i];
+      sg0 = p.act_kv[i] - len;
+      // tokens up to the next sequence's first, as batch_of() tells them apart
+      aq = qp < 0 ? 0 : max(0, min(len, min(next, p.T) - qp));
+      const int last = sg0 + aq - 1;                     // last position
+      if (aq > 0 && last >= 0) {
+        int most = aq;                                   // tokens of a tile
+        if (o.part == 0) {
+          lo = max(max(sg0, 0) - p.win_left, 0);
+          hi = min(last + 1, wp.ori_cap);
+          most = (int)min((long long)aq, (long long)p.win_left + ROWS);
+        } else if (o.part == 1) {
+          hi = min(min(p.first, wp.ori_cap), last - p.win_left);
+        } else {
+          hi = min(min((last + 1) / p.cmp_ratio, p.K), wp.cmp_cap);
+        }
+        nseg = (most + rp.seg - 1) / rp.seg;
+      }
+    }
+    const int n = max(hi - lo, 0);
+    const long long items = (long long)((n + ROWS - 1) / ROWS) * nseg;
+    long long x = items;
 #pragma unroll
-    for (int o = 0; o < OPS; ++o)
-      if (o * 4 + wave < NI)   // uniform
-        dma16s(qoff[o], qb + (size_t)i * 16 * D * 2, __builtin_amdgcn_readfirstlane(dst + (o * 4 + wave) * 1024));
-    if (wave == 3) dma16s((uint32_t)(lane & 3) * 16, lb + i * 16, __builtin_amdgcn_readfirstlane(lds_addr_of(ll[i % NB])));
-  };
+    for (int d = 1; d < 64; d <<= 1) { const long long v = __shfl_up(x, d); x += lane >= d ? v : 0; }
+    const uint64_t m = __ballot(base + x > at);
+    if (m) {
+      const int j = __ffsll((unsigned long long)m) - 1;
+      const int k = __builtin_amdgcn_readfirstlane((int)(at - base - (__shfl(x, j) - __shfl(items, j))));
+      nseg = __builtin_amdgcn_readfirstlane(__shfl(nseg, j));
+      lo = __builtin_amdgcn_readfirstlane(__shfl(lo, j));
+      hi = __builtin_amdgcn_readfirstlane(__shfl(hi, j));
+      aq = __builtin_amdgcn_readfirstlane(__shfl(aq, j));
+      o.b = c + j;
+      o.qp = __builtin_amdgcn_readfirstlane(__shfl(qp, j));
+      o.sg0 = __builtin_amdgcn_readfirstlane(__shfl(sg0, j));
+      o.p0 = lo + k / nseg * ROWS;
+      o.rows = min(ROWS, hi - o.p0);
+      // tokens [a0, a1) that attend any row of the tile, of which this segment
+      long long a0 = max(0, -o.sg0), a1 = aq;
+      if (o.part == 0) {
+        a0 = max(a0, (long long)o.p0 - o.sg0);
+        a1 = min(a1, (long long)o.p0 + o.rows + p.win_left - o.sg0);
+      } else if (o.part == 1) {
+        a0 = max(a0, (long long)o.p0 + p.win_left + 1 - o.sg0);
+      } else {
+        a0 = max(a0, ((long long)o.p0 + 1) * p.cmp_ratio - 1 - o.sg0);
+      }
+      a0 += (long long)(k % nseg) * rp.seg;
+      o.a0 = (int)min(a0, a1);
+      o.a1 = (int)min(a1, a0 + rp.seg);
+      return o.a0 < o.a1;
+    }
+    base += __shfl(x, 63);
+  }
+  return false;
+}
+
+template <int D, typename QT, bool F8, int RT>
+__global__ void __launch_bounds__(256, 2) sas_weights_rows_kernel(const WeightParams wp, const RowParts rp) {
+  using Q = Queries<D>;
+  constexpr int NB = 4, ROWS = 64 * RT, PF = 5;
+  __shared__ __attribute__((aligned(1024))) typename Q::Tile tiles[NB];
+  __shared__ float joined[4][16 * RT];
+
+  const FwdParams& p = wp.f;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int c16 = lane & 15, g = lane >> 4;
+  RowItem it;
+  if (!find_item<ROWS>(wp, rp, (int)blockIdx.x, lane, it)) return;
+  const bool few = it.rows <= 16 * RT;      // every wave holds all rows
+  const int ntile = p.H / 16, units = (it.a1 - it.a0) * ntile;
+  const Q queries(p, (size_t)it.qp + it.a0, wave, lane);
 #pragma unroll
   for (int i = 0; i < NB - 1; ++i)
-    if (i < ntile) issue(i);
+    if (i < units) queries.issue(tiles[i], i);
 
-  // rows: lane (g, c16) holds slot s0 + 16 rt + c16 (all four g), channels 32 ks + 8 g ..
+  // lane (g, c16) holds rows r0 + 16 rt + c16 of the tile, attended from position `from` to `to`
+  const int r0 = few ? 0 : 16 * RT * wave;
+  const bool cmp = it.part == 2;
+  const int bs = cmp ? p.cmp_bs : p.ori_bs, stride = cmp ? p.cmp_bt_stride : p.ori_bt_stride;
+  const int32_t* bt = (cmp ? p.cmp_bt : p.ori_bt) + (size_t)it.b * stride;
+  double* const wrow = cmp ? wp.cmp_w + (size_t)it.b * wp.cmp_rows : wp.ori_w + (size_t)it.b * wp.ori_rows;
   bool ok[RT];
-  double* dest[RT];
-  uint4 k[RT][KS];
+  int from[RT], to[RT];
+  uint4 k[RT][D / 32];
   float sc[RT][F8 ? 4 : 1];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int s = s0 + 16 * rt + c16;
-    const bool ori = s < nr;
-    int pos = s < nf ? s : wlo + s - nf;
-    ok[rt] = s < ns;
-    if (!ori) {
-      pos = s - nr;
-      if (p.scenario == SAS_SCFA && ok[rt]) pos = p.cmp_idx[(size_t)t * p.K + pos];
-      ok[rt] = ok[rt] && pos >= 0 && pos < thr;
-    }
-    const int bs = ori ? p.ori_bs : p.cmp_bs, blk = max(pos, 0) / bs;
-    const int stride = ori ? p.ori_bt_stride : p.cmp_bt_stride;
-    ok[rt] = ok[rt] && blk < stride && pos < (ori ? wp.ori_rows : wp.cmp_rows);
-    const int32_t* bt = ori ? p.ori_bt : p.cmp_bt;
-    const int phys = ok[rt] ? bt[(size_t)at.b * stride + blk] : -1;
-    ok[rt] = ok[rt] && phys >= 0 && phys < (ori ? p.ori_nblocks : p.cmp_nblocks);
+    const int r = r0 + 16 * rt + c16, pos = it.p0 + r, blk = pos / bs;
+    ok[rt] = r < it.rows && blk < stride && pos < (cmp ? wp.cmp_rows : wp.ori_rows);
+    const int phys = ok[rt] ? bt[blk] : -1;
+    ok[rt] = ok[rt] && phys >= 0 && phys < (cmp ? p.cmp_nblocks : p.ori_nblocks);
+    from[rt] = it.part == 0 ? pos : it.part == 1 ? (int)min((long long)pos + p.win_left + 1, (long long)INT_MAX)
+                                                 : (int)min(((long long)pos + 1) * p.cmp_ratio - 1, (long long)INT_MAX);
+    to[rt] = it.part == 0 ? (int)min((long long)pos + p.win_left, (long long)INT_MAX) : INT_MAX;
     constexpr int ROWB = F8 ? kRow656 : D * 2;
     // (a row that is not there: the query's bytes, masked out)
-    const uint64_t row = ok[rt] ? reinterpret_cast<uint64_t>(ori ? p.ori_kv : p.cmp_kv) +
+    const uint64_t row = ok[rt] ? reinterpret_cast<uint64_t>(cmp ? p.cmp_kv : p.ori_kv) +
                                       (uint64_t)(uint32_t)(phys * bs + pos - blk * bs) * ROWB
-                                : reinterpret_cast<uint64_t>(qb);
-    dest[rt] = ok[rt] ? (ori ? wp.ori_w + (size_t)at.b * wp.ori_rows : wp.cmp_w + (size_t)at.b * wp.cmp_rows) + pos
-                      : nullptr;
-    if constexpr (F8) {
-      // 16 latent values of a lane are its channels of two k-steps
-      uint4 raw[8];
-#pragma unroll
-      for (int m = 0; m < 8; ++m) raw[m] = gld16(row + (4 * m + g) * 16);
-#pragma unroll
-      for (int m = 0; m < 2; ++m) k[rt][16 + m] = gld16(row + 528 + (4 * m + g) * 16);
-#pragma unroll
-      for (int m = 0; m < 4; ++m) sc[rt][m] = gldf(row + 512 + 4 * m);
-#pragma unroll
-      for (int m = 0; m < 8; ++m) {
-        e4m3x4_to_bf16(raw[m].x, k[rt][2 * m].x, k[rt][2 * m].y);
-        e4m3x4_to_bf16(raw[m].y, k[rt][2 * m].z, k[rt][2 * m].w);
-        e4m3x4_to_bf16(raw[m].z, k[rt][2 * m + 1].x, k[rt][2 * m + 1].y);
-        e4m3x4_to_bf16(raw[m].w, k[rt][2 * m + 1].z, k[rt][2 * m + 1].w);
-      }
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k[rt][ks] = gld16(row + (4 * ks + g) * 16);
-    }
+                                : reinterpret_cast<uint64_t>(queries.q);
+    load_row<D, F8>(row, g, k[rt], sc[rt]);
   }
+  const int sg1 = it.sg0 + it.a0;           // position of the first token
 
   float acc[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) acc[rt] = 0.f;
-  const int qsw = swz<CH>(c16);
-  // the K fragments and the first tiles' DMA: known to the compiler to be done, so none
-  // of its waits falls into the loop
   __builtin_amdgcn_s_waitcnt(0);
-  for (int i = 0; i < ntile; ++i) {
-    // tile i is here once only the tiles behind it, at most NB - 2 of them, are under way
-    if (i >= NB - 1) {
-      const int m = min(NB - 2, ntile - 1 - i);
-      if (wide) m == 2 ? wait_vm<10>() : m == 1 ? wait_vm<5>() : wait_vm<0>();
-      else m == 2 ? wait_vm<8>() : m == 1 ? wait_vm<4>() : wait_vm<0>();
-    }
-    lds_barrier();   // every wave's part of tile i is here, and tile i - 1 is read
-    if (i + NB - 1 < ntile) issue(i + NB - 1);
-    const uint4* qt = lq[i % NB] + c16 * CH;
-    f32x4 s[RT], part[RT];
+  if (few) {
+    for (int i0 = 0; i0 < units; i0 += NB) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NB; ++j)          // (of the first four, three are under way)
+        if (i0 + j < units && (i0 > 0 || j == NB - 1)) queries.issue(tiles[j], i0 + j);
+      queries.wait(0);
+      lds_barrier();
+      const int i = i0 + wave;
+      if (i < units) {
+        const typename Q::Tile& tile = tiles[wave];
+        const int sg = sg1 + i / ntile;
+        const f32x4 l2 = *reinterpret_cast<const f32x4*>(&tile.lse[4 * g]) * kLog2e;
+        f32x4 s[RT];
+        tile_scores<D, QT, F8, RT, PF>(tile, k, sc, g, c16, s, [] {});
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int L = F8 && ks < 16 ? 8 * (ks >> 1) + 2 * g + (ks & 1) : 4 * ks + g;
-      const uint4 a = qt[(L & -SG) | ((L & (SG - 1)) ^ qsw)];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        if (F8 && ks < 16) {
-          part[rt] = mfma32k<QT>(a, k[rt][ks], ks % 4 == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[rt]);
-          if (ks % 4 == 3) s[rt] += part[rt] * sc[rt][F8 ? ks / 4 : 0];
-        } else {
-          s[rt] = mfma32k<QT>(a, k[rt][ks], s[rt]);
+        for (int rt = 0; rt < RT; ++rt) {
+          const float x = shares(s[rt], l2, p.scale_log2);
+          acc[rt] += sg >= from[rt] && sg <= to[rt] ? x : 0.f;
         }
       }
+      lds_barrier();                        // the four are read
     }
-    // lane (g, c16): heads 4 g + j of the tile, row c16
-    const f32x4 l2 = *reinterpret_cast<const f32x4*>(&ll[i % NB][4 * g]) * kLog2e;
+    // the waves' sums meet in wave 0
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
+      const float w = rows_sum(acc[rt]);
+      if (g == 0) joined[wave][16 * rt + c16] = w;
+    }
+    __syncthreads();
+    if (wave == 0 && g == 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[rt] += __builtin_amdgcn_exp2f(s[rt][j] * p.scale_log2 - l2[j]);
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = 16 * rt + c16;
+        if (ok[rt]) add_weight(wrow + it.p0 + r, (joined[0][r] + joined[1][r]) + (joined[2][r] + joined[3][r]), wp.units);
+      }
+    }
+    return;
   }
+  // unit i's scores are computed while unit i - 1's become weights
+  f32x4 so[RT], lse2 = f32x4{0.f, 0.f, 0.f, 0.f};
+  int tok = 0, head = 0;                    // unit i's token and head tile
+  bool use[RT], uso[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) { so[rt] = lse2; uso[rt] = false; use[rt] = false; }
+  auto weigh = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float x = shares(so[rt], lse2, p.scale_log2);
+      acc[rt] += uso[rt] ? x : 0.f;
+    }
+  };
+  for (int i = 0; i < units; ++i) {
+    // unit i is here once only the units behind it, at most NB - 2 of them, are under way
+    if (i >= NB - 1) queries.wait(min(NB - 2, units - 1 - i));
+    lds_barrier();   // every wave's part of unit i is here, and unit i - 1 is read
+    if (i + NB - 1 < units) queries.issue(tiles[(i + NB - 1) % NB], i + NB - 1);
+    if (head == 0) {
+      const int sg = sg1 + tok;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) use[rt] = sg >= from[rt] && sg <= to[rt];
+    }
+    const typename Q::Tile& tile = tiles[i % NB];
+    const f32x4 l2 = *reinterpret_cast<const f32x4*>(&tile.lse[4 * g]) * kLog2e;
+    f32x4 s[RT];
+    tile_scores<D, QT, F8, RT, PF>(tile, k, sc, g, c16, s, weigh);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) { so[rt] = s[rt]; uso[rt] = use[rt]; }
+    lse2 = l2;
+    if (++head == ntile) { head = 0; ++tok; }
+  }
+  weigh();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float w = rows_sum(acc[rt]);
-    if (g == 0 && ok[rt]) add_weight(dest[rt], w, wp.units);
+    if (g == 0 && ok[rt]) add_weight(wrow + it.p0 + r0 + 16 * rt + c16, w, wp.units);
   }
 }
 
+struct WeightPlan {
+  long long slots;       // workgroups of sas_weights_kernel, 0: none
+  long long rows;        // workgroups of sas_weights_rows_kernel, 0: none
+  RowParts parts;
+  WeightParams by_slot;  // what the former covers
+};
+
+constexpr int kRowTiles = 2;     // 16-row tiles a wave in sas_weights_rows_kernel
+constexpr int kSegMax = 64, kSegMin = 4;   // its tokens a segment
+
 template <int D, typename QT, bool F8>
-int launch_weights(const WeightParams& wp, long long blocks, hipStream_t st) {
-  hipLaunchKernelGGL((sas_weights_kernel<D, QT, F8, 2>), dim3((unsigned)blocks), dim3(256), 0, st, wp);
+int launch_weights(const WeightParams& wp, const WeightPlan& pl, hipStream_t st) {
+  if (pl.rows)
+    hipLaunchKernelGGL((sas_weights_rows_kernel<D, QT, F8, kRowTiles>), dim3((unsigned)pl.rows), dim3(256), 0, st, wp, pl.parts);
+  if (pl.slots)
+    hipLaunchKernelGGL((sas_weights_kernel<D, QT, F8>), dim3((unsigned)pl.slots), dim3(256), 0, st, pl.by_slot);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(SAS_ELAUNCH, "row weights launch: %s", hipGetErrorString(e));
   return SAS_OK;
@@ -305,19 +593,52 @@ int weights_impl(const SasRowWeightsArgs* ra, hipStream_t st) {
   // rows past a table's end are not there
   wp.ori_cap = ra->ori_weights ? (int)std::min<long long>(INT_MAX / 2, (long long)a->ori_bt_stride * a->ori_block_size) : 0;
   wp.cmp_cap = cmp ? (int)std::min<long long>(INT_MAX / 2, (long long)a->cmp_bt_stride * a->cmp_block_size) : 0;
-  constexpr int ROWS = 128;
-  const long long nori = std::min<long long>(wp.ori_cap, ra->ori_first + a->win_left + 1);
-  const long long ncmp = !cmp ? 0 : a->scenario == SAS_SCFA ? a->K : std::min<long long>(wp.cmp_cap, a->K);
+  WeightPlan pl{};
+  pl.by_slot = wp;
+  // tokens of a sequence that share its rows: by rows, but for the top-k ones
+  const bool by_rows = a->T >= 4 * a->B;
+  if (by_rows) {
+    constexpr long long R = 64 * kRowTiles;
+    // segments: as long as the tiles then still give most CUs their two workgroups
+    auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+    const long long mean = std::max<long long>(1, a->T / a->B), before = std::min<long long>(a->win_left, wp.ori_cap);
+    const long long ncmp = cmp && a->scenario == SAS_CFA ? std::min<long long>(wp.cmp_cap, a->K) : 0;
+    const long long all = a->B * ((wp.ori_w ? up(std::min<long long>(wp.ori_cap, mean + before), R) : 0) + up(ncmp, R));
+    int& seg = pl.parts.seg;
+    seg = kSegMax;
+    while (seg > kSegMin && 2 * all * up(std::min<long long>(mean, a->win_left + R), seg) < 3LL * device_cus()) seg /= 2;
+    // A grid that holds any lengths. Of one sequence with m tokens: up(m, seg) segments for each
+    // of its first or compressed rows' tiles; (before + m) / R + 1 tiles of window rows, each
+    // with up(min(m, win_left + R), seg) segments.
+    const long long segs = a->T / seg + a->B;
+    if (wp.ori_w) {
+      const long long w = (before / R + 2) * segs +
+                          up(a->T, R) * (std::min<long long>(a->T, a->win_left + R) / seg + 1);
+      const long long f = up(std::min<long long>(ra->ori_first, wp.ori_cap), R) * segs;
+      if (w + f > INT_MAX) return set_error(SAS_EINVAL, "row weights: %lld workgroups beyond one launch", w + f);
+      pl.parts.win_blocks = (int)w;
+      pl.parts.first_blocks = (int)f;
+      pl.rows = w + f;
+      pl.by_slot.ori_w = nullptr;
+    }
+    if (ncmp) {
+      pl.rows += up(ncmp, R) * segs;
+      pl.by_slot.cmp_w = nullptr;
+    }
+    if (pl.rows > INT_MAX) return set_error(SAS_EINVAL, "row weights: %lld workgroups beyond one launch", pl.rows);
+  }
+  constexpr int ROWS = 64;
+  const long long nori = pl.by_slot.ori_w ? std::min<long long>(wp.ori_cap, ra->ori_first + a->win_left + 1) : 0;
+  const long long ncmp = !pl.by_slot.cmp_w ? 0 : a->scenario == SAS_SCFA ? a->K : std::min<long long>(wp.cmp_cap, a->K);
   const long long chunks = (nori + ncmp + ROWS - 1) / ROWS;
-  if (chunks == 0) return SAS_OK;
-  wp.spread = a->T >= 2 * fp.nxcd;
-  const long long blocks = (wp.spread ? (a->T + fp.nxcd - 1) / fp.nxcd * fp.nxcd : a->T) * chunks;
-  if (blocks > INT_MAX) return set_error(SAS_EINVAL, "row weights: %lld workgroups beyond one launch", blocks);
-  wp.chunks = (int)chunks;
-  if (fp8) return launch_weights<576, __bf16, true>(wp, blocks, st);
+  pl.by_slot.spread = a->T >= 2 * fp.nxcd;
+  pl.slots = (pl.by_slot.spread ? (a->T + fp.nxcd - 1) / fp.nxcd * fp.nxcd : a->T) * chunks;
+  if (pl.slots > INT_MAX) return set_error(SAS_EINVAL, "row weights: %lld workgroups beyond one launch", pl.slots);
+  pl.by_slot.chunks = (int)chunks;
+  if (fp8) return launch_weights<576, __bf16, true>(wp, pl, st);
   if (a->q_dtype == SAS_DT_BF16)
-    return a->D == 576 ? launch_weights<576, __bf16, false>(wp, blocks, st) : launch_weights<512, __bf16, false>(wp, blocks, st);
-  return a->D == 576 ? launch_weights<576, _Float16, false>(wp, blocks, st) : launch_weights<512, _Float16, false>(wp, blocks, st);
+    return a->D == 576 ? launch_weights<576, __bf16, false>(wp, pl, st) : launch_weights<512, __bf16, false>(wp, pl, st);
+  return a->D == 576 ? launch_weights<576, _Float16, false>(wp, pl, st) : launch_weights<512, _Float16, false>(wp, pl, st);
 }
 
 }  // namespace
