@@ -40,7 +40,7 @@
 // :877 (P cast), :1135-1145 (LSE), and golden.py:69-204.
 
 #include "sas_fwd_win.h"
-#if SAS_FWD_TREE
+#if SAS_FWD_TREE || SAS_FWD_FIRST
 #include "sas_fwd_pair.h"
 #endif
 
@@ -1962,8 +1962,13 @@ int part_bytes(int q_dtype) { return q_dtype == SAS_DT_FP16 ? 4 : 2; }
 struct Plan {
   int hw, nw, nhg, nslots, nsplit, sps;
   bool exact;   // exact-window schedule (Fwd::run_exact)
+  bool window;  // (kFirst) a window and its first rows in at most kPairWindow slots, one split
   size_t ws;
 };
+
+// With first rows a 128-row window no longer fits the exact schedule: up to so many slots,
+// from 32 (token, 64 heads) items on, it is one split of the kernels of two workgroups a CU.
+constexpr int kPairWindow = 192;
 
 int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   if (!a) return sas::set_error(SAS_EINVAL, "null args");
@@ -2034,11 +2039,13 @@ int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   // spills (the staging registers beside the scale groups): 4 waves there.
   if (nw <= 0) nw = (hw == 2 || (hw == 4 && !fp8)) ? 8 : 4;
   if (nw != 4 && nw != 8) return sas::set_error(SAS_EINVAL, "waves must be 4 or 8");
+  pl->window = kFirst && a->scenario == SAS_SWA && pl->nslots <= kPairWindow && a->num_splits <= 0 &&
+               a->head_waves == 0 && a->waves == 0 && T * ((a->H + 63) / 64) >= 32;
   if (hw == 1 || pl->exact) nw = 4;
   pl->nw = nw;
   pl->hw = hw;
   pl->nhg = (int)a->H / (16 * hw);
-  if (pl->exact) ns = 1;
+  if (pl->exact || pl->window) ns = 1;
   if (ns <= 0) {
     // as many splits as fill each XCD's CUs in one round, each split at
     // least min_sps slots (1-token, 16-head decode: 15.5 µs at 4 splits of
@@ -2227,7 +2234,7 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
   return launch_combine(fp, a->out_dtype, st);
 }
 
-#if SAS_FWD_TREE
+#if SAS_FWD_TREE || SAS_FWD_FIRST
 // Whether a call takes the kernels of two workgroups a CU (sas_fwd_pair.h): all of a
 // token's slots in one workgroup, and
 //  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows of
@@ -2248,7 +2255,7 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
   if (pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
   const long long items = a->T * ((a->H + 63) / 64), cus = sas::device_cus();
-  if (pl.exact) return items >= 32;
+  if (pl.exact || (kFirst && pl.window)) return items >= 32;
   if (a->T * pl.nhg <= cus) return false;
   if (a->kv_dtype != a->q_dtype && pl.hw == 2) return a->H > 32 && (items > cus || pl.nslots <= 640);
   return true;
@@ -2336,7 +2343,7 @@ int fwd_impl(const SasFwdArgs* a, const uint64_t* tree_mask, int tree_words, lon
       return launch_fwd_win(fp, (int)a->D, a->q_dtype, run, st);
     }
   }
-#if SAS_FWD_TREE
+#if SAS_FWD_TREE || SAS_FWD_FIRST
   if (use_pairs(a, pl)) {
     fp.nhg = (int)(a->H + 63) / 64;
     const long long nb = (a->T + fp.nxcd - 1) / fp.nxcd * fp.nhg * fp.nxcd;

@@ -1,5 +1,5 @@
-// Draft trees of more (token, 64 heads) items than compute units, and windows of fewer
-// (use_pairs() has the rule): one item a workgroup of 4 waves, two workgroups on a CU,
+// Draft trees, and calls with first rows, of more (token, 64 heads) items than compute units,
+// and windows of fewer (use_pairs() has the rule): one item a workgroup of 4 waves, two workgroups on a CU,
 // MI355X (gfx950). Where heads are no multiple of 64, waves without heads only move rows.
 //
 // The 8-wave kernel has a CU to itself: its ring fills the LDS, and nothing runs
@@ -24,9 +24,17 @@
 
 #include "sas_kern.h"
 
+#ifndef SAS_FWD_TREE
+#define SAS_FWD_TREE 0
+#endif
+#ifndef SAS_FWD_FIRST
+#define SAS_FWD_FIRST 0
+#endif
+
 namespace sas {
 namespace {
 
+constexpr bool kPairTree = SAS_FWD_TREE, kPairFirst = SAS_FWD_FIRST;
 constexpr int kPairPT = 4, kPairSRB = kPairPT * 32 + 16, kPairStage = 16 * kPairSRB;   // output staging of a wave
 
 // 16 heads x 512 channels (lane (g, c16): channels 16 i + 4 g .. + 3 of head c16) scaled
@@ -110,14 +118,14 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair_kernel(const FwdParams p)
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c16 = lane & 15, g = lane >> 4;
-  const int item = item_index<true>(p);
+  const int item = item_index<kPairTree>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
   // (heads past the last: a wave without heads only moves rows; its addresses stay valid)
   const bool mine = k.hg * 64 + wave * 16 < p.H;
   const int hq = mine ? k.hg * 64 + wave * 16 : p.H - 16;
   uint4 qf[KS];
-  resolve<256, D * 2, true, true>(p, k, tid, lane, wave, [&] {
+  resolve<256, D * 2, kPairTree, true, kPairFirst>(p, k, tid, lane, wave, [&] {
     const uint4* q = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq + c16) * D * 2) + g;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = q[ks * 4];
@@ -281,14 +289,14 @@ __global__ void __launch_bounds__(256, 2) sas_fwd_pair8_kernel(const FwdParams p
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int c16 = lane & 15, g = lane >> 4;
-  const int item = item_index<true>(p);
+  const int item = item_index<kPairTree>(p);
   if (item < 0) return;
   Tok k = item_of(p, item);
   // (heads past the last: a wave without heads only moves rows; its addresses stay valid)
   const bool mine = k.hg * 64 + wave * 16 < p.H;
   const int hq = mine ? k.hg * 64 + wave * 16 : p.H - 16;
   uint4 qf[KS];
-  resolve<256, kRow656, true, true>(p, k, tid, lane, wave, [&] {
+  resolve<256, kRow656, kPairTree, true, kPairFirst>(p, k, tid, lane, wave, [&] {
     const uint4* q = reinterpret_cast<const uint4*>(p.q + ((size_t)k.t * p.H + hq + c16) * D * 2) + g;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = q[ks * 4];
