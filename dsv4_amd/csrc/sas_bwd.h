@@ -38,6 +38,7 @@ struct BwdParams {
   int cmp_tiles;        // key-major pass: compressed row tiles per segment
   int win_tiles_seg;    // key-major pass: window row tiles per segment
   int first_tiles;      // key-major pass: tiles of first rows per segment (as far as the window leaves them behind)
+  int first_rows;       // and rows per such tile: kFirstRows or kKeyRows
 };
 
 // f(integral_constant<int, j>) for j = 0 .. N-1, with no loop: arrays
@@ -93,5 +94,6 @@ int launch_bwd_prefill_first(const BwdParams& bp, int D, int q_dtype, hipStream_
 // heads per workgroup of sas_bwd_dq_kernel
 inline int bwd_dq_heads(int H) { return H % 64 == 0 ? 64 : 32; }
 constexpr int kKeyRows = 64;   // rows per tile of the key-major pass
+constexpr int kFirstRows = 16; // of a narrow tile of first rows (sas_bwd_head.h)
 
 }  // namespace sas

@@ -882,6 +882,7 @@ struct PrePlan {
   bool on, sparse;   // sparse: some tokens may need per-token adds for their compressed rows
   int dense_thr, key_seg;
   long long seg_groups, cmp_tiles, win_tiles, first_tiles;
+  int first_rows;
   size_t ws;
 };
 PrePlan plan_prefill(const SasBwdArgs* ba, long long first) {
@@ -926,7 +927,11 @@ PrePlan plan_prefill(const SasBwdArgs* ba, long long first) {
   r.seg_groups = a->T / r.key_seg + a->B;
   r.win_tiles = std::min<long long>(((long long)a->win_left + r.key_seg + 2 * (kKeyRows - 1)) / kKeyRows,
                                     (a->ori_bt_stride * a->ori_block_size + kKeyRows - 1) / kKeyRows);
-  r.first_tiles = (std::min<long long>(first, a->ori_bt_stride * a->ori_block_size) + kKeyRows - 1) / kKeyRows;
+  // Narrow tiles up to two of them: a narrow tile adds 37 us to a 64-head, 576-wide call of 4096
+  // tokens, a wide one 100 (64 first rows: 985 us in narrow tiles, 842 in a wide one; 4: 755, 819).
+  const long long nfirst = std::min<long long>(first, a->ori_bt_stride * a->ori_block_size);
+  r.first_rows = nfirst <= 2 * kFirstRows ? kFirstRows : kKeyRows;
+  r.first_tiles = (nfirst + r.first_rows - 1) / r.first_rows;
   r.ws = (size_t)a->T * a->H * sizeof(float) + (size_t)a->T * (a->H / 8);   // Delta, non-finite marks
   if ((r.sparse && nslots > kMaxSlots) || r.ws == 0 ||
       (double)(r.cmp_tiles + r.win_tiles + r.first_tiles) * (r.seg_groups + 64) * (a->H / 32) > 2e9)
@@ -1067,6 +1072,7 @@ int bwd_impl(const SasBwdArgs* ba, long long first, void* stream) {
     bp.cmp_tiles = (int)pre.cmp_tiles;
     bp.win_tiles_seg = (int)pre.win_tiles;
     bp.first_tiles = (int)pre.first_tiles;
+    bp.first_rows = pre.first_rows;
     if (pre.sparse) {
       // one split: every token's dq is written by one workgroup
       BwdParams sb = bp;

@@ -311,6 +311,10 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {   // two packed values
   return w;
 }
 
+#if SAS_BWD_FIRST
+#include "sas_bwd_head.h"
+#endif
+
 template <int D, typename QT>
 __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
   constexpr int CH = D / 8, OCH = kDV / 8;     // 16-byte chunks per q / dO row
@@ -380,6 +384,16 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
   if (a0 + sg0 < 0) a0 = min(a1, -sg0);         // tokens before position 0 attend no row
   const bool cmp = tile < bp.cmp_tiles;
   const bool head = kBwdFirst && tile >= bp.cmp_tiles + bp.win_tiles_seg;   // a tile of first rows
+#if SAS_BWD_FIRST
+  if (head && bp.first_rows == kFirstRows) {
+    const int at = (tile - bp.cmp_tiles - bp.win_tiles_seg) * kFirstRows;
+    // tokens whose window starts behind the tile's first row
+    const long long lo = (long long)at + p.win_left + 1 - sg0;
+    if (lo > a0) a0 = (int)min(lo, (long long)a1);
+    if (a0 < a1) first_rows_tile<D, QT>(bp, lds_q, lds_o, lds_t[0], lds_t[1], lds_h, lds_r, b, qp, sg0, a0, a1, at, hg);
+    return;   // uniform
+  }
+#endif
   int p0;                                       // the tile's first position
   if (cmp) {
     p0 = tile * kKeyRows;
@@ -391,7 +405,6 @@ __global__ void __launch_bounds__(512) sas_bwd_keys_kernel(const BwdParams bp) {
     if (p.scenario == SAS_CFA && p0 >= p.K) return;
   } else if (head) {
     p0 = (tile - bp.cmp_tiles - bp.win_tiles_seg) * kKeyRows;
-    // tokens whose window starts behind the tile's first row
     const long long lo = (long long)p0 + p.win_left + 1 - sg0;
     if (lo > a0) a0 = (int)min(lo, (long long)a1);
   } else {

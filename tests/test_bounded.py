@@ -509,6 +509,9 @@ GRAD = {
     "prompt_cfa": dict(kind="cfa", H=64, D=576, ql=[100], kl=[700], ratio=16, F=130, win=30, bs=16),
     "prompt_no_first": dict(H=32, D=576, ql=[100], kl=[150], F=0, win=64),
     "prompt_first_beyond": dict(H=32, D=512, ql=[100], kl=[100], F=1000, win=5),
+    "prompt_two_tiles": dict(H=32, D=576, ql=[90, 60], kl=[90, 33], F=25, win=10, bs=16, holes=True),
+    "prompt_32_rows": dict(dt="fp16", H=64, D=512, ql=[120], kl=[150], F=32, win=1),
+    "prompt_33_rows": dict(dt="fp16", H=64, D=512, ql=[120], kl=[150], F=33, win=3),
     "prompt_missing": dict(H=32, D=576, ql=[100, 80], kl=[60, 300], F=6, win=20),
     "prompt_holes": dict(H=64, D=512, ql=[100, 80], kl=[260, 300], holes=True, F=6, win=20),
     "sparse_beyond": dict(kind="scfa", H=64, D=576, ql=[90], kl=[900], K=6, F=9, win=70),   # tokens whose rows are added per token
@@ -540,6 +543,35 @@ def test_gpu_first_backward(name):
     kw = c.kwargs()
     out, lse = _run(c, **kw)
     _check_grads(c, _grads(c, out, lse, kw), out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [20, 40])
+def test_gpu_first_backward_keeps_a_tokens_nan_to_its_rows(first):
+    # a token at position 3 with a window of 2 attends rows 0 .. 3: a NaN in its query
+    # leaves the gradients of every other row as if the token had none
+    c = Case(H=32, D=512, ql=[70], kl=[70], F=first, win=2)
+    kw = c.kwargs()
+    quiet, dout = c.q.cuda().clone(), c.dout.cuda().clone()
+    quiet[3] = 0
+    dout[3] = 0
+    out, lse = _run(c, quiet, **kw)
+    want = _grads(c, out, lse, kw, dout=dout, q=quiet)[1]
+    loud = quiet.clone()
+    loud[3, 5, 7] = float("nan")
+    out, lse = _run(c, loud, **kw)
+    got = _grads(c, out, lse, kw, q=loud)[1]
+    rows = want.view(-1, c.D)
+    hit = torch.isnan(got.view(-1, c.D)).any(1)
+    bt = kw["ori_block_table"][0].long()
+    attended = torch.zeros(rows.shape[0], dtype=torch.bool, device="cuda")
+    for j in range(4):
+        attended[bt[j // c.bs] * c.bs + j % c.bs] = True
+    assert torch.equal(hit, attended)
+    # what is left differs by the order of the float32 adds: at most 69 tokens' terms, each below
+    # the largest gradient times some tens
+    err = (got.view(-1, c.D)[~hit] - rows[~hit]).abs().max()
+    assert float(err) <= 69 * 69 * 2.0 ** -24 * 16 * float(rows.abs().max())
 
 
 @pytest.mark.gpu
