@@ -918,8 +918,11 @@ PrePlan plan_prefill(const SasBwdArgs* ba, long long first) {
   // tokens: 512 tokens 150 / 211 / 274 us, 2048 tokens 765 / 789 / 776, 6000
   // tokens 3113 / 3034 / 2922; 2726 packed tokens with 128 heads 1427 / 1417 /
   // 1278; 16 tokens: 171 and 1596). Near the line it can miss: three
-  // sequences of 500 to 2000 tokens take 96 and 1240 us, with 64 1152.
-  for (int seg : {96, 64, 32}) {
+  // sequences of 500 to 2000 tokens take 96 and 1240 us, with 64 1152. With first rows there
+  // is a tile more, and short calls end sooner in segments of 24 (32 / 24: 64 heads 512
+  // tokens 133 / 125 us; top-64 lists, 32 heads 500 tokens 172 / 162, six sequences of 70 to
+  // 250 291 / 272; near the line three of 300 to 700 with 64 heads 358 / 363).
+  for (int seg : {96, 64, 32, kBwdFirst ? 24 : 32}) {
     r.key_seg = seg;
     const double wgs = (double)a->T / seg * (a->H / 32) * (((double)a->win_left + seg) / kKeyRows + 1 + r.cmp_tiles / 2.0);
     if (wgs >= 2.75 * device_cus()) break;
