@@ -40,24 +40,34 @@ namespace {
 // dP^T over the wave's channels, the pair adds the halves through LDS (own +
 // other: the same bits in both, and in sas_bwd64_kernel), dS^T packed in registers is the B operand of
 // dq^T[channel x head] += K^T . dS^T, K^T by transposed reads of the row tile.
-template <int D, typename QT, int NG>
+//
+// TR = 16, with first rows: chunks of 16 rows in three slots, two under way, and
+// 32 heads a workgroup, so that two workgroups share a CU and one loads its
+// token's q, dO and O while the other works (a call of few rows a token spends
+// over half its time on those). Delta comes from the registers that hold dO.
+// Gradients of 4096 tokens, 64 heads, 576 wide, 132 rows a token: 755 us with
+// TR = 32, 719 with 16, 674 with Delta so as well; 32 heads, 512 wide, 144 rows
+// 451 / 373 / 351; 512 + 132 rows 1749 / 1785 / 1736, 384 rows 1241 / 1262 / 1211.
+template <int D, typename QT, int NG, int TR = 32>
 __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp) {
-  constexpr int NW = 2 * NG, NT = 64 * NW, TR = 32;
+  constexpr int NW = 2 * NG, NT = 64 * NW;
+  constexpr int NM = TR / 16, NS = 4 - NM;    // 16-row tiles a chunk, chunks in LDS
+  constexpr int GR = TR / 8;                  // 8-row groups a chunk
   constexpr int CH = D / 8;                   // 16-byte chunks per row
   constexpr int KSH = D / 64;                 // S k-steps per channel half
   constexpr int VSH = kDV / 64;               // dP k-steps per channel half
   constexpr int DQT = D / 32;                 // dq tiles per wave
   constexpr int RI = CH / 8;                  // DMA instructions per 8 rows (9 or 8)
   constexpr int NP = 8 / NW;                  // of which a wave takes NP in each 8 rows
-  constexpr int OPS = 4 * NP + (RI == 9);     // and waves 0-3 one of the left-over ones
+  constexpr int OPS = GR * NP + (RI == 9);    // and the first GR waves one of the left-over ones
   constexpr int SG = kSwzGroup<CH>;
-  constexpr int kRing = 2 * TR * CH;          // chunks
-  constexpr int kX = NW * 4 * 64;             // exchange chunks
+  constexpr int kRing = NS * TR * CH;         // chunks
+  constexpr int kX = NW * 2 * NM * 64;        // exchange chunks
   constexpr int SRB = DQT * 16 * 2 + 16;      // staged dq row bytes
   static_assert(NW * 16 * SRB <= (kRing + kX) * 16, "dq staging fits");
-  static_assert(2 * TR <= kRowPad, "a chunk past the last stays in the padded row list");
+  static_assert(NS * TR <= kRowPad, "a chunk past the last stays in the padded row list");
   __shared__ __attribute__((aligned(16))) uint4 lds_b[kRing + kX];
-  __shared__ float lds_dl[16 * NG];
+  __shared__ float lds_dl[NM == 2 ? 16 * NG : 32 * NG];
 
   const FwdParams& p = bp.f;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -69,7 +79,7 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
   const size_t th = (size_t)t * p.H + h;
 
   // Delta = dO . O: 8 threads per head, 64 channels each
-  {
+  if constexpr (NM == 2) {
     const int hd = tid >> 3, part = tid & 7;
     const size_t at = ((size_t)t * p.H + k.hg * 16 * NG + hd) * kDV * 2 + part * 128;
     const uint32_t* dog = reinterpret_cast<const uint32_t*>(bp.dout + at);
@@ -90,6 +100,19 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
     for (int ks = 0; ks < KSH; ++ks) qf[ks] = qg[(hh * KSH + ks) * 4 + g4];
 #pragma unroll
     for (int ks = 0; ks < VSH; ++ks) of[ks] = dg[(hh * VSH + ks) * 4 + g4];
+    if constexpr (NM == 1) {
+      // Delta from these: 64 bytes of a head's row at a time, and dO is read once
+      const uint4* og = reinterpret_cast<const uint4*>(bp.out + th * kDV * 2);
+      uint4 ov[VSH];
+#pragma unroll
+      for (int ks = 0; ks < VSH; ++ks) ov[ks] = og[(hh * VSH + ks) * 4 + g4];
+      float d = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < VSH; ++ks)
+        d = dot2<QT>(of[ks].w, ov[ks].w, dot2<QT>(of[ks].z, ov[ks].z, dot2<QT>(of[ks].y, ov[ks].y, dot2<QT>(of[ks].x, ov[ks].x, d))));
+      d = rows_sum(d);
+      if (g4 == 0) lds_dl[wave * 16 + c16] = d;
+    }
   }
   const float lse2 = p.lse[th] * kLog2e;
   float dl = 0.f;
@@ -133,7 +156,7 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
     k.sp = pass;
     resolve<256, D * 2, false, false, kBwdFirst>(p, k, tid, lane, wave, [] {});
     if (pass == 0) {
-      dl = lds_dl[16 * g + c16];   // behind resolve()'s barriers
+      dl = NM == 2 ? lds_dl[16 * g + c16] : lds_dl[32 * g + c16] + lds_dl[32 * g + 16 + c16];   // behind resolve()'s barriers
       if (k.thr > bp.dense_thr) {         // the per-token kernel's token
         mark();
         return;
@@ -149,31 +172,39 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
     // behind it
     auto row_addr = [&](int c, int o) {
       const uint32_t rb = __builtin_amdgcn_readfirstlane(lds_addr_of(lds_rows + c * TR));
-      const int j = o < 4 * NP ? o & 3 : wave & 3;   // 8-row group
-      return *reinterpret_cast<const LDS_AS uint64_t*>((size_t)(rb + 8u * (uint32_t)(prow[o >> 2] + 8 * j)));
+      const int j = o < GR * NP ? o & (GR - 1) : wave & (GR - 1);   // 8-row group
+      return *reinterpret_cast<const LDS_AS uint64_t*>((size_t)(rb + 8u * (uint32_t)(prow[o / GR] + 8 * j)));
     };
     uint64_t ra;
+    auto slot = [](int c) { return NS == 2 ? c & 1 : (int)((unsigned)c % NS); };
     auto dma_fire = [&](int c, int o) {
-      if (o == 4 * NP && wave >= 4) return;   // wave-uniform
-      const int j = o < 4 * NP ? o & 3 : wave & 3, m = o < 4 * NP ? wave + NW * (o >> 2) : 8;
-      dma16(reinterpret_cast<const void*>(ra + pcol[o >> 2]),
-            __builtin_amdgcn_readfirstlane(lds_addr_of(lds_b + (c & 1) * TR * CH) + (j * RI + m) * 1024));
+      if (o == GR * NP && wave >= GR) return;   // wave-uniform
+      const int j = o < GR * NP ? o & (GR - 1) : wave & (GR - 1), m = o < GR * NP ? wave + NW * (o / GR) : 8;
+      dma16(reinterpret_cast<const void*>(ra + pcol[o / GR]),
+            __builtin_amdgcn_readfirstlane(lds_addr_of(lds_b + slot(c) * TR * CH) + (j * RI + m) * 1024));
       if (o + 1 < OPS) ra = row_addr(c, o + 1);
     };
     const int nch = (nvalid + TR - 1) / TR;
-    ra = row_addr(0, 0);
 #pragma unroll
-    for (int o = 0; o < OPS; ++o) dma_fire(0, o);
+    for (int c = 0; c < NS - 1; ++c) {
+      ra = row_addr(c, 0);
+#pragma unroll
+      for (int o = 0; o < OPS; ++o) dma_fire(c, o);
+    }
+    if (NS > 2) __builtin_amdgcn_s_waitcnt(0);   // every load that the compiler tracks, outside the loop
     for (int c = 0; c < nch; ++c) {
       const int nr = nvalid - c * TR;
-      const uint4* kt = lds_b + (c & 1) * TR * CH;
-      __builtin_amdgcn_s_waitcnt(0);   // known to the compiler: no wait of its own behind the DMA
+      const uint4* kt = lds_b + slot(c) * TR * CH;
+      // known to the compiler: no wait of its own behind the DMA. With NS = 3 the chunk after
+      // this one may be under way, GR NP instructions of every wave
+      static_assert(NS == 2 || GR * NP < 16, "vmcnt in the low four bits");
+      __builtin_amdgcn_s_waitcnt(NS == 2 ? 0 : GR * NP | 0x70);
       __builtin_amdgcn_s_barrier();
-      ra = row_addr(c + 1, 0);
-      // S^T and dP^T of the chunk's two 16-row tiles over this wave's channels
-      f32x4 s[2], dp[2];
+      ra = row_addr(c + NS - 1, 0);
+      // S^T and dP^T of the chunk's 16-row tiles over this wave's channels
+      f32x4 s[NM], dp[NM];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) { s[mt] = f32x4{0.f, 0.f, 0.f, 0.f}; dp[mt] = s[mt]; }
+      for (int mt = 0; mt < NM; ++mt) { s[mt] = f32x4{0.f, 0.f, 0.f, 0.f}; dp[mt] = s[mt]; }
       // channel half HH: fragments HH VSH + i; S takes k-steps HH KSH ..,
       // which start OFF fragments later
       auto half = [&](auto HHC) __attribute__((always_inline)) {
@@ -182,43 +213,45 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
           const int L = 4 * (HH * VSH + i) + g4;
           return kt[(mt * 16 + c16) * CH + ((L & -SG) | ((L & (SG - 1)) ^ ksw))];
         };
-        uint4 a[PF][2];
+        uint4 a[PF][NM];
 #pragma unroll
         for (int i = 0; i < PF; ++i)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) a[i][mt] = kfrag(i, mt);
+          for (int mt = 0; mt < NM; ++mt) a[i][mt] = kfrag(i, mt);
 #pragma unroll
         for (int i = 0; i < NF; ++i) {
-          const uint4 a0 = a[i % PF][0], a1 = a[i % PF][1];
-          if (i + PF < NF) { a[i % PF][0] = kfrag(i + PF, 0); a[i % PF][1] = kfrag(i + PF, 1); }
-          if (i >= OFF) {
-            s[0] = mfma32k<QT>(a0, qf[i - OFF], s[0]);
-            s[1] = mfma32k<QT>(a1, qf[i - OFF], s[1]);
-          }
-          if (i < VSH) {
-            dp[0] = mfma32k<QT>(a0, of[i], dp[0]);
-            dp[1] = mfma32k<QT>(a1, of[i], dp[1]);
-          }
+          uint4 at[NM];
+#pragma unroll
+          for (int mt = 0; mt < NM; ++mt) at[mt] = a[i % PF][mt];
+#pragma unroll
+          for (int mt = 0; mt < NM; ++mt)
+            if (i + PF < NF) a[i % PF][mt] = kfrag(i + PF, mt);
+#pragma unroll
+          for (int mt = 0; mt < NM; ++mt)
+            if (i >= OFF) s[mt] = mfma32k<QT>(at[mt], qf[i - OFF], s[mt]);
+#pragma unroll
+          for (int mt = 0; mt < NM; ++mt)
+            if (i < VSH) dp[mt] = mfma32k<QT>(at[mt], of[i], dp[mt]);
           // the next chunk's DMA between the MFMAs (see sas_bwd_keys_kernel)
           constexpr int EV = OPS > 5 ? 1 : 2;
-          if (i % EV == EV - 1 && i / EV < OPS) dma_fire(c + 1, i / EV);
+          if (i % EV == EV - 1 && i / EV < OPS) dma_fire(c + NS - 1, i / EV);
         }
 #pragma unroll
-        for (int o = NF / (OPS > 5 ? 1 : 2); o < OPS; ++o) dma_fire(c + 1, o);
+        for (int o = NF / (OPS > 5 ? 1 : 2); o < OPS; ++o) dma_fire(c + NS - 1, o);
       };
       if (hh) half(std::integral_constant<int, 1>{});
       else half(std::integral_constant<int, 0>{});
       f32x4* x = reinterpret_cast<f32x4*>(lds_b + kRing);
-      x[(wave * 4 + 0) * 64 + lane] = s[0];
-      x[(wave * 4 + 1) * 64 + lane] = s[1];
-      x[(wave * 4 + 2) * 64 + lane] = dp[0];
-      x[(wave * 4 + 3) * 64 + lane] = dp[1];
-      lds_barrier();
-      uint32_t pk[4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        s[mt] += x[((wave ^ 1) * 4 + mt) * 64 + lane];
-        dp[mt] += x[((wave ^ 1) * 4 + 2 + mt) * 64 + lane];
+      for (int mt = 0; mt < NM; ++mt) x[(wave * 2 * NM + mt) * 64 + lane] = s[mt];
+#pragma unroll
+      for (int mt = 0; mt < NM; ++mt) x[(wave * 2 * NM + NM + mt) * 64 + lane] = dp[mt];
+      lds_barrier();
+      uint32_t pk[2 * NM];
+#pragma unroll
+      for (int mt = 0; mt < NM; ++mt) {
+        s[mt] += x[((wave ^ 1) * 2 * NM + mt) * 64 + lane];
+        dp[mt] += x[((wave ^ 1) * 2 * NM + NM + mt) * 64 + lane];
         float ds[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -228,32 +261,38 @@ __global__ void __launch_bounds__(128 * NG) sas_bwd_dq_kernel(const BwdParams bp
         pk[2 * mt] = pack2<QT>(ds[0], ds[1]);
         pk[2 * mt + 1] = pack2<QT>(ds[2], ds[3]);
       }
-      const uint4 bds = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-      // dq^T: A = K^T of keys 4 g4 .. + 3 and 16 + 4 g4 .. + 3, the order of bds
-      auto vfrag = [&](int j) {
+      // dq^T: A = K^T of keys 4 g4 .. + 3 (and 16 + 4 g4 .. + 3), the order of pk
+      using Frag = std::conditional_t<NM == 2, uint4, uint2>;
+      Frag bds;
+      if constexpr (NM == 2) bds = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+      else bds = make_uint2(pk[0], pk[1]);
+      auto vfrag = [&](int j) -> Frag {
         const char* b0 = reinterpret_cast<const char*>(kt) + voff[j % TPG] + (j / TPG) * SG * 16;
         const uint2 u0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)(b0)));
-        const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)(b0 + 16 * CH * 16)));
-        return make_uint4(u0.x, u0.y, u1.x, u1.y);
+        if constexpr (NM == 2) {
+          const uint2 u1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)(b0 + 16 * CH * 16)));
+          return make_uint4(u0.x, u0.y, u1.x, u1.y);
+        } else return u0;
       };
       constexpr int PV = 4;
-      uint4 v[PV];
+      Frag v[PV];
 #pragma unroll
       for (int j = 0; j < PV; ++j) v[j] = vfrag(j);
 #pragma unroll
       for (int j = 0; j < DQT; ++j) {
-        const uint4 a = v[j % PV];
+        const Frag a = v[j % PV];
         if (j + PV < DQT) v[j % PV] = vfrag(j + PV);
-        acc[j] = mfma32k<QT>(a, bds, acc[j]);
+        if constexpr (NM == 2) acc[j] = mfma32k<QT>(a, bds, acc[j]);
+        else acc[j] = mfma16k<QT>(a, bds, acc[j]);
       }
-      __builtin_amdgcn_sched_group_barrier(0x100, 2 * PV, 2);
+      __builtin_amdgcn_sched_group_barrier(0x100, NM * PV, 2);
 #pragma unroll
       for (int j = 0; j < DQT; ++j) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 2);
-        if (j + PV < DQT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 2);
+        if (j + PV < DQT) __builtin_amdgcn_sched_group_barrier(0x100, NM, 2);
       }
     }
-    wait_vm<0>();      // the spare chunk's DMA
+    wait_vm<0>();      // the spare chunks' DMA
     __syncthreads();   // the row list and the slots are free
   }
   // lane (g4, c16): channels 16 ct + 4 g4 .. + 3 of head c16
@@ -714,7 +753,7 @@ template <int D, typename QT>
 int launch(const BwdParams& bp, hipStream_t st) {
   const FwdParams& p = bp.f;
   const long long nx = p.nxcd;
-  const int nhg = p.H / bwd_dq_heads(p.H);
+  const int nhg = p.H / (kBwdFirst ? 32 : bwd_dq_heads(p.H));
   BwdParams b = bp;
   b.f.nhg = nhg;
   b.f.nsplit = 1;
@@ -722,7 +761,8 @@ int launch(const BwdParams& bp, hipStream_t st) {
   const long long kb = ((long long)bp.seg_groups * (p.H / 32) + nx - 1) / nx * nx *
                        (bp.cmp_tiles + bp.win_tiles_seg + (kBwdFirst ? bp.first_tiles : 0));
   if (nb > INT_MAX || kb > INT_MAX) return set_error(SAS_EINVAL, "bwd: %lld workgroups beyond one launch", std::max(nb, kb));
-  if (bwd_dq_heads(p.H) == 64) hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 4>), dim3((unsigned)nb), dim3(512), 0, st, b);
+  if constexpr (kBwdFirst) hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 2, 16>), dim3((unsigned)nb), dim3(256), 0, st, b);
+  else if (bwd_dq_heads(p.H) == 64) hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 4>), dim3((unsigned)nb), dim3(512), 0, st, b);
   else hipLaunchKernelGGL((sas_bwd_dq_kernel<D, QT, 2>), dim3((unsigned)nb), dim3(256), 0, st, b);
   hipLaunchKernelGGL((sas_bwd_keys_kernel<D, QT>), dim3((unsigned)kb), dim3(512), 0, st, b);
   hipLaunchKernelGGL(sas_bwd_sink_kernel, dim3(std::min(256, (p.T + 15) / 16), (p.H + 63) / 64), dim3(256), 0, st, b);
