@@ -1113,6 +1113,10 @@ def add_row_weights(
     if ori_weights is None and cmp_weights is None:
         return
     lse = lse.contiguous()
+    if lse.data_ptr() % 16:
+        lse = lse.clone()
+    if q.data_ptr() % 16:
+        q = q.clone()
     behind = _WEIGHTS.pack(ori_first, 0 if ori_weights is None else ori_weights.data_ptr(),
                            0 if cmp_weights is None else cmp_weights.data_ptr(),
                            0 if ori_weights is None else ori_weights.shape[1],
@@ -1246,6 +1250,8 @@ def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBack
         if t_.dtype != dt or t_.device != dev:
             raise ValueError(f"{name} must be a {dt} tensor on {dev}")
     dout_f, out_f, lse_f = dout_f.contiguous(), out_f.contiguous(), lse_f.contiguous()
+    if ori_first is not None and out_f.data_ptr() % 16:
+        out_f = out_f.clone()
     ori_kv = kwargs["ori_kv"]
     cmp_kv = kwargs.get("cmp_kv")
     keep = [dout_f, out_f, lse_f]

@@ -1053,6 +1053,8 @@ int bwd_impl(const SasBwdArgs* ba, long long first, void* stream) {
   const PrePlan pre = plan_prefill(ba, first);
   if (direct && !(pre.on && have_ws))
     return set_error(SAS_EINVAL, "bwd: SAS_BWD_DQ_DTYPE without SAS_BWD_WORKSPACE or where sas_bwd_plan does not allow it");
+  if (kBwdFirst && have_ws && pre.on && (reinterpret_cast<uintptr_t>(a->out) & 15))
+    return set_error(SAS_EINVAL, "bwd: out must be 16-byte aligned");
   if (have_ws && pre.on && (!a->workspace || a->workspace_bytes < pre.ws))
     return set_error(SAS_ENOWS, "bwd: workspace of %zu bytes required", pre.ws);
   bool capturing = false;

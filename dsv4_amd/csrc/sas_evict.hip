@@ -148,8 +148,9 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
   // candidates [lo, hi), of which `need` stay; rows without a weight count as 0
   const int lo = p.first, hi = n - p.recent;
   int need = p.budget - p.first - p.recent;
-  const int run = ((n + kSelThreads - 1) / kSelThreads) * 64, r0 = wave * run;
+  const int run = ((n - 1) / kSelThreads + 1) * 64, r0 = wave * run;
   const int ne = E ? E : run / 64;
+  // (16 runs end at 2^31 at most; what lies past the last row of one is not looked at)
   auto load = [&](int e) {
     const int j = r0 + e * 64 + lane;
     return j < n && j < p.weight_rows ? w[j] : 0.;
@@ -318,7 +319,7 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lo = p.first, hi = n - p.recent;
   int need = p.budget - p.first - p.recent, left = hi - lo;
-  const int run = ((n + kSelThreads - 1) / kSelThreads) * 64, r0 = wave * run, r1 = min(r0 + run, n);
+  const int run = ((n - 1) / kSelThreads + 1) * 64, r0 = wave * run, r1 = min(r0 + run, n);
   auto weight = [&](int j) { return j < p.weight_rows ? w[j] : 0.; };
   // rows a lane under way: few, since what is written out for each has to be fetched
   constexpr int U = 4, UW = 2;
@@ -586,13 +587,14 @@ int launch_move(EvictParams p, hipStream_t st) {
 
 int evict_impl(const SasCacheEvictArgs* a, hipStream_t st) {
   if (a->B < 0 || a->B > 65535) return set_error(SAS_EINVAL, "evict: B must be 0..65535 (got %lld)", (long long)a->B);
-  if (a->budget < 1 || a->budget > INT_MAX) return set_error(SAS_EINVAL, "evict: budget must be at least 1 (got %lld)", (long long)a->budget);
+  if (a->budget < 1 || a->budget > 1 << 30) return set_error(SAS_EINVAL, "evict: budget must be 1..2^30 (got %lld)", (long long)a->budget);
   if (a->keep_first < 0 || a->keep_recent < 0 || a->keep_first > a->budget || a->keep_recent > a->budget - a->keep_first)
     return set_error(SAS_EINVAL, "evict: keep_first and keep_recent must not be negative and fit the budget (%lld + %lld, %lld)",
                      (long long)a->keep_first, (long long)a->keep_recent, (long long)a->budget);
   if (a->row_bytes < 16 || a->row_bytes % 16 || a->row_bytes > 1 << 20)
     return set_error(SAS_EINVAL, "evict: rows must be a multiple of 16 bytes, at most 1 MiB (got %lld)", (long long)a->row_bytes);
-  if (a->weight_rows < 0 || a->weight_rows > INT_MAX) return set_error(SAS_EINVAL, "evict: weight_rows out of range");
+  if (a->weight_rows < 0 || a->weight_rows > 1 << 30)
+    return set_error(SAS_EINVAL, "evict: weight_rows must be 0..2^30 (got %lld)", (long long)a->weight_rows);
   if (a->bt_stride < 1 || a->bt_stride > INT_MAX || a->block_size < 1 || a->num_blocks < 1 ||
       (double)a->num_blocks * a->block_size > 2147483000.0)
     return set_error(SAS_EINVAL, "evict: bad cache geometry");

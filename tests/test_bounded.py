@@ -327,7 +327,8 @@ def test_abi_evict_refuses():
                            (dict(row_bytes=1160), "16 bytes"), (dict(weight_rows=-1), "weight_rows"),
                            (dict(bt_stride=0), "geometry"), (dict(num_blocks=1 << 30), "geometry"), (dict(kept=None), "null"),
                            (dict(weights=None), "null"), (dict(cache=fake + 8), "16-byte"), (dict(weights=fake + 4), "8-byte"),
-                           (dict(B=-1), "B must"), (dict(B=65536), "B must")):
+                           (dict(B=-1), "B must"), (dict(B=65536), "B must"),
+                           (dict(budget=(1 << 30) + 1), "budget"), (dict(weight_rows=(1 << 30) + 1), "weight_rows")):
         _refused(fn, _lib.SasCacheEvictArgs(**dict(base, **change)), needle)
     assert fn(C.byref(_lib.SasCacheEvictArgs(**dict(base, B=0))), None) == _lib.SAS_OK
 
@@ -684,6 +685,37 @@ def test_gpu_weights(name):
     assert torch.equal(ori, 2 * one) and (cmp_ is None or torch.equal(cmp_, 2 * onec))
 
 
+def _odd(t):
+    # the same values two or four bytes behind a 16-byte boundary
+    room = torch.empty(t.numel() + 8, dtype=t.dtype, device="cuda")
+    out = room[1:1 + t.numel()].view(t.shape)
+    out.copy_(t)
+    assert out.data_ptr() % 16 and out.is_contiguous()
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["q", "dout", "out", "all"])
+def test_gpu_tensors_at_odd_addresses(which):
+    c = Case(kind="scfa", H=32, D=576, ql=[70, 2], kl=[300, 90], K=20, F=5, win=40)
+    kw, q, dout = c.kwargs(), c.q.cuda(), c.dout.cuda()
+    out, lse = _run(c, q, **kw)
+    ori, cmp_ = _zeros(c)
+    _weights(c, lse, ori, cmp_, q=q)
+    if which in ("q", "all"):
+        q = _odd(q)
+        got = _run(c, q, **kw)
+        assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+    if which in ("dout", "all"):
+        dout = _odd(dout)
+    if which in ("out", "all"):
+        out, lse = _odd(out), _odd(lse)
+    _check_grads(c, _grads(c, out, lse, kw, dout=dout, q=q), out, lse)
+    o, k = _zeros(c)
+    _weights(c, lse, o, k, q=q)
+    assert torch.equal(o, ori) and torch.equal(k, cmp_)
+
+
 @pytest.mark.gpu
 def test_gpu_weights_of_one_cache_alone():
     c = Case(**WEIGHTS["scfa"])
@@ -922,6 +954,40 @@ def test_gpu_evict_int64_lengths():
     ref = R.evict(*a)
     got = _evict(a[0], a[1], a[2].long(), a[3].long(), *a[4:])
     _same(got, ref)
+
+
+# ---------------------------------------------------------------------------
+# GPU: long caches
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ql", [[3, 1], [70, 40]])
+def test_gpu_rows_past_32_bit_offsets(ql):
+    """A cache of more than 2^32 bytes whose blocks at the end hold the rows: what the
+    small cache with the same blocks at its start gives."""
+    from dsv4_amd.cache import evict_kv_cache
+    c = Case(H=64, D=576, ql=ql, kl=[300, 200], F=6, win=64)
+    kw = c.kwargs()
+    small, table = kw["ori_kv"], kw["ori_block_table"]
+    nb = small.shape[0]
+    far = (5 << 30) // (c.bs * c.D * 2)
+    big = torch.zeros(far + nb, c.bs, 1, c.D, dtype=c.dt, device="cuda")
+    big[far:] = small
+    there = dict(kw, ori_kv=big, ori_block_table=torch.where(table >= 0, table + far, table))
+    (out, lse), (o2, l2) = _run(c, **kw), _run(c, **there)
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    (w, _), (w2, _) = _zeros(c), _zeros(c)
+    _weights(c, lse, w, None, kw)
+    _weights(c, lse, w2, None, there)
+    assert torch.equal(w, w2)
+    g, g2 = _grads(c, out, lse, kw), _grads(c, out, lse, there)
+    _check_grads(c, (g2[0], g2[1][far:].clone(), g2[2], g2[3]), out, lse)
+    assert torch.equal(g[0], g2[0]) and not bool(g2[1][:far].any())
+    del g2
+    left = [evict_kv_cache(k["ori_kv"], x, k["ori_block_table"], k["seqused_kv"], budget=90, keep_first=4, keep_recent=20)
+            for k, x in ((kw, w), (there, w2))]
+    assert torch.equal(left[0][0], left[1][0]) and torch.equal(left[0][1], left[1][1]) and torch.equal(w, w2)
+    assert torch.equal(small.view(torch.int16), big[far:].view(torch.int16)) and not bool(big[:far].view(torch.int16).any())
 
 
 # ---------------------------------------------------------------------------
