@@ -314,53 +314,68 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
 // A sequence of n > budget rows, at most kWordRows, with its keys' high words in LDS: many
 // rows a thread in registers are as many unrolled copies of every step, whose instructions
 // then have to be fetched (26000 rows: 52 us, 12 of them one pass of counts). Low words are
-// read from memory where they matter.
+// read from memory where they matter. One CU works here, and what a pass takes is the
+// instructions it issues for a row: so no pass looks where a wave's rows end (the words
+// behind are kNone), a weight's word takes two instructions where it is finite and not
+// below 0, and ties are counted only in steps that hold some.
 __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, SelSmall& sh, int n, const double* w, int32_t* kept) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int lo = p.first, hi = n - p.recent;
   int need = p.budget - p.first - p.recent, left = hi - lo;
-  const int run = ((n - 1) / kSelThreads + 1) * 64, r0 = wave * run, r1 = min(r0 + run, n);
+  const int run = ((n - 1) / (2 * kSelThreads) + 1) * 128, r0 = wave * run;   // 16 runs: at most kWordRows
   auto weight = [&](int j) { return j < p.weight_rows ? w[j] : 0.; };
-  // rows a lane under way: few, since what is written out for each has to be fetched
-  constexpr int U = 4, UW = 2;
-  auto each = [&](auto&& f) __attribute__((always_inline)) {   // f(row, word); UW rows at a time
-    for (int j0 = r0 + lane; j0 - lane < r1; j0 += 64 * UW) {
-      uint32_t v[UW];
-#pragma unroll
-      for (int u = 0; u < UW; ++u) v[u] = big.word[min(j0 + 64 * u, kWordRows - 1)];
-#pragma unroll
-      for (int u = 0; u < UW; ++u) f(j0 + 64 * u, j0 + 64 * u < r1 ? v[u] : kNone);
+  auto each = [&](auto&& f) __attribute__((always_inline)) {   // f(row, word)
+    for (int i = 0; i < run; i += 128) {
+      const int j = r0 + i + lane;
+      const uint32_t v0 = big.word[j], v1 = big.word[j + 64];
+      f(j, v0);
+      f(j + 64, v1);
     }
   };
   // the same with the low words of the rows whose word is `word`: f(row, low word), the
   // others' left out
   auto lows = [&](uint32_t word, auto&& f) __attribute__((always_inline)) {
-    for (int j0 = r0 + lane; j0 - lane < r1; j0 += 64 * U) {
-      bool has[U];
-      double v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) has[u] = j0 + 64 * u < r1 && big.word[min(j0 + 64 * u, kWordRows - 1)] == word;
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = has[u] ? weight(j0 + 64 * u) : 0.;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (has[u]) f(j0 + 64 * u, key_of(v[u]).lo);
+    for (int i = 0; i < run; i += 128) {
+      const int j = r0 + i + lane;
+      const bool h0 = big.word[j] == word, h1 = big.word[j + 64] == word;
+      const double v0 = h0 ? weight(j) : 0., v1 = h1 ? weight(j + 64) : 0.;
+      if (h0) f(j, key_of(v0).lo);
+      if (h1) f(j + 64, key_of(v1).lo);
     }
   };
-  if (tid == 0) { sh.nrank = 0; sh.any[0] = 0; sh.any[1] = ~0u; }
-  for (int i = tid; i < kBins; i += kSelThreads) big.hist[i] = 0;
-  __syncthreads();
-  uint32_t most = 0, least = ~0u;   // of the candidates' words above 0's
-  for (int j0 = r0 + lane; j0 - lane < r1; j0 += 64 * U) {
-    double v[U];
+  auto is_word = [](uint32_t k) { return k - 1u < kStays - 1u; };
+  auto clear = [&] {   // counts and joined words, behind a barrier; one follows
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kSelThreads) big.hist[i] = 0;
+    if (tid < 4) sh.any[tid] = tid & 1 ? ~0u : 0u;
+    __syncthreads();
+  };
+  if (tid == 0) sh.nrank = 0;
+  clear();
+  uint32_t most = 0, least = ~0u;   // the candidates' highest word, and the lowest above 0's less that and 1
+  {
+    constexpr int U = 4;   // rows a lane under way
+    const uint32_t* wh = reinterpret_cast<const uint32_t*>(w) + 1;
+    const int have = min(n, p.weight_rows);
+    for (int i = 0; i < run; i += 64 * U) {
+      uint32_t h[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = j0 + 64 * u < r1 ? weight(j0 + 64 * u) : 0.;
+      for (int u = 0; u < U; ++u) {
+        const int j = r0 + i + 64 * u + lane;
+        h[u] = i + 64 * u < run && j < have ? wh[2 * (size_t)j] : 0u;
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = j0 + 64 * u;
-      const uint32_t k = j < lo || j >= hi ? kStays : key_of(v[u]).hi;
-      if (j < r1) big.word[j] = k;
-      if (k > kZero && k < kStays) { most = max(most, k); least = min(least, k); }
+      for (int u = 0; u < U; ++u) {
+        if (i + 64 * u >= run) break;   // uniform
+        const int j = r0 + i + 64 * u + lane;
+        uint32_t k = h[u] | 0x80000000u;
+        if (h[u] >= 0x7ff00000u) k = key_of(w[j]).hi;   // below 0, -0, infinite or NaN
+        const bool cand = (unsigned)(j - lo) < (unsigned)left;
+        big.word[j] = cand ? k : j < n ? kStays : kNone;
+        k = cand ? k : 0u;
+        most = max(most, k);
+        least = min(least, k - (kZero + 1));
+      }
     }
   }
 #pragma unroll
@@ -368,46 +383,83 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   if (lane == 0) { atomicMax(&sh.any[0], most); atomicMin(&sh.any[1], least); }
 
   Key edge{kStays - 1, ~0u}, prefix{0, 0}, mask{0, 0};
-  bool done = need == 0;
+  bool done = need == 0, sorted = false;   // sorted: the rows that share the edge's high word are told apart
+  int pass = 0;
+  // the need-th of the `left` rows in rpos; `all`: no other row has one of their high words
+  auto rank_list = [&](bool all) {
+    __syncthreads();
+    if (tid < left) sh.rkey[tid] = key_of(weight(sh.rpos[tid]));
+    rank_keys(sh, left, need);
+    edge = sh.edge;
+    need = sh.need;
+    done = true;
+    if (all) {
+      if (tid < left && sh.rkey[tid].hi == edge.hi) {
+        const uint32_t l = sh.rkey[tid].lo;
+        big.word[sh.rpos[tid]] = l > edge.lo ? kStays : l == edge.lo ? edge.hi : kNone;
+      }
+      sorted = true;
+      __syncthreads();
+    }
+  };
+  // whether one low word is all that the rows of high word prefix.hi have (any is clear)
+  auto one_low = [&] {
+    uint32_t o = 0, a = ~0u;
+    bool has = false;
+    lows(prefix.hi, [&](int, uint32_t k) { o |= k; a &= k; has = true; });
+    if (one_word(sh.any + 2, o, a, has)) { edge = Key{prefix.hi, sh.any[2]}; done = true; }
+  };
   if (!done) {
-    // first over the range of the positive weights, in up to 2047 even steps of their high
-    // words (bin 0: the others); a bin of few keys ends the search here
     __syncthreads();
     most = __builtin_amdgcn_readfirstlane(sh.any[0]);
-    least = min((uint32_t)__builtin_amdgcn_readfirstlane(sh.any[1]), most);
-    const int s = max(0, 32 - __clz((int)((most - least) / (kBins - 1))));
-    auto bin_of = [&](uint32_t k) { return k > kZero ? 1 + (int)((k - least) >> s) : 0; };
-    each([&](int, uint32_t k) {
-      if (k - 1u < kStays - 1u) atomicAdd(&big.hist[bin_of(k)], 1);
-    });
-    find_bin(sh, need, [&](int i) { return big.hist[i]; });
-    const int bin = __builtin_amdgcn_readfirstlane(sh.found[0]);
-    if (sh.found[2] <= kRank) {
-      left = __builtin_amdgcn_readfirstlane(sh.found[2]);
-      each([&](int j, uint32_t k) {
-        if (k - 1u < kStays - 1u && bin_of(k) == bin) {
-          const int at = atomicAdd(&sh.nrank, 1);
-          sh.rkey[at] = key_of(weight(j));
-          sh.rpos[at] = j;
-        }
+    if (most > kZero) {
+      // first over the range of the positive weights, in up to 2047 even steps of their high
+      // words (bin 0: the others), then over 2048 steps of the bin that divides them; a bin
+      // of few keys ends the search
+      uint32_t base = kZero + 1 + (uint32_t)__builtin_amdgcn_readfirstlane(sh.any[1]);
+      int s = max(0, 32 - __clz((int)((most - base) / (kBins - 1))));
+      each([&](int, uint32_t k) {
+        if (is_word(k)) atomicAdd(&big.hist[k > kZero ? 1 + ((k - base) >> s) : 0], 1);
       });
-      rank_keys(sh, left, need - __builtin_amdgcn_readfirstlane(sh.found[1]));
-      edge = sh.edge;
-      need = sh.need;
-      done = true;
+      find_bin(sh, need, [&](int i) { return big.hist[i]; });
+      int bin = __builtin_amdgcn_readfirstlane(sh.found[0]) - 1;
+      while (bin >= 0) {
+        need -= __builtin_amdgcn_readfirstlane(sh.found[1]);
+        left = __builtin_amdgcn_readfirstlane(sh.found[2]);
+        base += (uint32_t)bin << s;
+        if (left <= kRank) {
+          each([&](int j, uint32_t k) {
+            if (is_word(k) && (k - base) >> s == 0) sh.rpos[atomicAdd(&sh.nrank, 1)] = j;
+          });
+          rank_list(true);
+          break;
+        }
+        clear();
+        if (s == 0) {   // one high word: on to the low ones
+          prefix.hi = base;
+          mask.hi = ~0u;
+          pass = 3;
+          one_low();
+          break;
+        }
+        const int t = max(0, s - 11);
+        each([&](int, uint32_t k) {
+          if (is_word(k) && (k - base) >> s == 0) atomicAdd(&big.hist[(k - base) >> t], 1);
+        });
+        find_bin(sh, need, [&](int i) { return big.hist[i]; });
+        bin = __builtin_amdgcn_readfirstlane(sh.found[0]);
+        s = t;
+      }
     }
-    __syncthreads();   // found and any are read
   }
-  for (int pass = 0; !done && pass < 6; ++pass) {
+  for (; !done && pass < 6; ++pass) {
     const bool high = pass < 3;
     const int third = pass % 3, s = third == 0 ? 21 : third == 1 ? 10 : 0;
     const uint32_t digit = third == 2 ? 1023u : 2047u;
-    for (int i = tid; i < kBins; i += kSelThreads) big.hist[i] = 0;
-    if (tid < 4) sh.any[tid] = tid & 1 ? ~0u : 0u;
-    __syncthreads();
+    clear();
     if (high)
       each([&](int, uint32_t k) {
-        if (k - 1u < kStays - 1u && (k & mask.hi) == prefix.hi) atomicAdd(&big.hist[k >> s & digit], 1);
+        if (is_word(k) && (k & mask.hi) == prefix.hi) atomicAdd(&big.hist[k >> s & digit], 1);
       });
     else
       lows(prefix.hi, [&](int, uint32_t k) {
@@ -424,44 +476,36 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
       need = 0;
       done = true;
     } else if (left <= kRank) {
-      each([&](int j, uint32_t k) {
-        if (k - 1u < kStays - 1u && (k & mask.hi) == prefix.hi) {
-          const Key key = key_of(weight(j));
-          if ((key.lo & mask.lo) == prefix.lo) {
-            const int at = atomicAdd(&sh.nrank, 1);
-            sh.rkey[at] = key;
-            sh.rpos[at] = j;
-          }
-        }
-      });
-      rank_keys(sh, left, need);
-      edge = sh.edge;
-      need = sh.need;
-      done = true;
+      auto take = [&](int j) { sh.rpos[atomicAdd(&sh.nrank, 1)] = j; };
+      if (high)
+        each([&](int j, uint32_t k) {
+          if (is_word(k) && (k & mask.hi) == prefix.hi) take(j);
+        });
+      else
+        lows(prefix.hi, [&](int j, uint32_t k) {
+          if ((k & mask.lo) == prefix.lo) take(j);
+        });
+      rank_list(high);
     } else if (high) {
       // one high word alone: on to the low ones, if those are not one as well (weights of 0)
-      uint32_t o = 0, a = ~0u;
-      bool has = false;
       if (pass < 2) {
+        uint32_t o = 0, a = ~0u;
+        bool has = false;
         each([&](int, uint32_t k) {
-          if (k - 1u < kStays - 1u && (k & mask.hi) == prefix.hi) { o |= k; a &= k; has = true; }
+          if (is_word(k) && (k & mask.hi) == prefix.hi) { o |= k; a &= k; has = true; }
         });
         if (one_word(sh.any, o, a, has)) { prefix.hi = sh.any[0]; mask.hi = ~0u; }
       }
       if (mask.hi == ~0u) {
         pass = 2;
-        o = 0, a = ~0u;
-        has = false;
-        lows(prefix.hi, [&](int, uint32_t k) { o |= k; a &= k; has = true; });
-        if (one_word(sh.any + 2, o, a, has)) { edge = Key{prefix.hi, sh.any[2]}; done = true; }
+        one_low();
       }
-      __syncthreads();   // read before the next pass clears them
     }
   }
   if (!done) edge = prefix;
 
   // among the rows that share the edge's high word: those above it stay, those below are none
-  if (need > 0 || edge.lo != ~0u)
+  if (!sorted && (need > 0 || edge.lo != ~0u))
     lows(edge.hi, [&](int j, uint32_t k) { big.word[j] = k > edge.lo ? kStays : k == edge.lo ? edge.hi : kNone; });
   // list: a wave's places follow from the runs before it
   int nk = 0, nt = 0;
@@ -475,10 +519,16 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   int pk = before(sh.wsum, wave, lane), pt = before(sh.wtie, wave, lane);
   each([&](int j, uint32_t k) {
     const uint64_t over = __ballot(k > edge.hi), tie = __ballot(k == edge.hi);
-    const int rank = pt + lanes_before(tie), at = pk + lanes_before(over) + min(rank, need);
-    if ((over >> lane & 1) || ((tie >> lane & 1) && rank < need)) kept[at] = j;
+    bool stays = k > edge.hi;
+    int at = pk + min(pt, need) + lanes_before(over);
+    if (tie) {   // uniform
+      const int rank = pt + lanes_before(tie);
+      at += min(rank, need) - min(pt, need);
+      stays |= k == edge.hi && rank < need;
+      pt += __popcll(tie);
+    }
+    if (stays) kept[at] = j;
     pk += __popcll(over);
-    pt += __popcll(tie);
   });
 }
 

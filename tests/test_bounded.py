@@ -911,6 +911,22 @@ def test_gpu_evict_close_weights(n, spread):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [4097, 20000, 32767, 32768])
+@pytest.mark.parametrize("kind", ["few", "narrow", "squares", "below"])
+def test_gpu_evict_distributions(n, kind):
+    """Weights that fill their range unevenly: five values, a few thousand neighbouring ones
+    of one binade, squares, all at or below 0."""
+    a = _evict_case([n, 5000], 10, 4, 64, bs=64, row=8)
+    g = torch.Generator().manual_seed(3)
+    u = torch.rand(a[1].shape, generator=g, dtype=torch.float64)
+    a[1][:] = {"few": (u * 5).floor() / 7, "narrow": 1 + (u * 4096).floor() * 2.0 ** -34, "squares": (u * u * 2 ** 20).round() * 2.0 ** -36,
+               "below": -(u * 3).floor()}[kind]
+    for budget in (100, n // 7, n // 2, n - 90):
+        b = a[:4] + (budget, 4, 64)
+        _same(_evict(*b), R.evict(*b))
+
+
+@pytest.mark.gpu
 def test_gpu_evict_rows_without_blocks():
     """A moved row needs both blocks; entries out of range count as none, nothing is
     read or written through them."""
