@@ -4,14 +4,19 @@
 //
 //  evict_select_kernel  one workgroup a sequence reads its weights once, as
 //     order-preserving 64-bit keys (in registers up to 4096 rows, the keys' high words in
-//     LDS up to 32768, longer sequences are read anew in each pass), and finds the key that divides the candidates: radix
-//     passes of 11 bits (counts in LDS) until the bin in question holds a wave or two of
-//     keys, which are ranked against each other, or one key alone. Then every wave lists
-//     the rows of its run that stay and puts their weights in place.
+//     LDS up to 32768; longer sequences are read anew in each pass), and finds the key that
+//     divides the candidates: passes of 2048 counts in LDS over the range of the weights or
+//     over 11 bits, until the bin in question holds at most 128 keys, which are ranked
+//     against each other, or one key alone. Then every wave lists the rows of its run that
+//     stay. 32 sequences of 2100 rows 8.5 us; four of 20000 to 32768 25 us, 6 of them one
+//     CU's load of 208 KB.
 //  evict_move_kernel    a workgroup owns one slice of the rows' bytes of one sequence
 //     and walks the list: since row i comes from a row at or behind i, the rows of a
 //     chunk are loaded before any of them is written, and later chunks read only rows
-//     behind them. Rows that stay where they are are not touched.
+//     behind them. Rows that stay where they are are not touched. One more workgroup a
+//     sequence closes up the weights. 32 sequences of 2048 rows of 1152 bytes 12.5 us (an
+//     eviction of a few rows moves those behind the first that leaves: up to 75 MB read and
+//     as much written, most of it in the Infinity Cache), four of 4096 rows of 656 bytes 13.
 
 #include <hip/hip_runtime.h>
 
@@ -354,7 +359,7 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   clear();
   uint32_t most = 0, least = ~0u;   // the candidates' highest word, and the lowest above 0's less that and 1
   {
-    constexpr int U = 4;   // rows a lane under way
+    constexpr int U = 8;   // rows a lane under way (4: 0.5 us more; 16 and 32: no less, a CU's 208 KB take 6 us)
     const uint32_t* wh = reinterpret_cast<const uint32_t*>(w) + 1;
     const int have = min(n, p.weight_rows);
     for (int i = 0; i < run; i += 64 * U) {
@@ -668,7 +673,7 @@ int evict_impl(const SasCacheEvictArgs* a, hipStream_t st) {
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)p.B), dim3(kSelThreads), 0, st, p);
   // Slices of 64 bytes, or narrower where those leave CUs without work: 32 sequences of
   // 2048 rows of 1152 bytes 64 / 32 / 16 bytes 21.9 / 25.8 / 28.7 us a call, 4 of 4096
-  // rows of 656 59.7 / 55.1 / 53.2.
+  // rows of 656 59.7 / 55.1 / 53.2 (when the selection took 10 us more).
   const long long quarters = (long long)p.B * ((p.row_bytes + 15) / 16);
   const int rc = quarters >= 4LL * device_cus() ? launch_move<4, 8>(p, st)
                : quarters >= 2LL * device_cus() ? launch_move<2, 8>(p, st) : launch_move<1, 4>(p, st);
