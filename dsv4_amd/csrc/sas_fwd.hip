@@ -1962,13 +1962,20 @@ int part_bytes(int q_dtype) { return q_dtype == SAS_DT_FP16 ? 4 : 2; }
 struct Plan {
   int hw, nw, nhg, nslots, nsplit, sps;
   bool exact;   // exact-window schedule (Fwd::run_exact)
-  bool window;  // (kFirst) a window and its first rows in at most kPairWindow slots, one split
+  bool window;  // (kFirst) a window and its first rows in one split of the kernels of two workgroups a CU
   size_t ws;
 };
 
-// With first rows a 128-row window no longer fits the exact schedule: up to so many slots,
-// from 32 (token, 64 heads) items on, it is one split of the kernels of two workgroups a CU.
-constexpr int kPairWindow = 192;
+// With first rows a 128-row window no longer fits the exact schedule. Where one round of
+// workgroups takes the call, each slot costs more in one split of the kernels of two
+// workgroups a CU than in several splits, but no combine follows: up to kPairWindow slots, and
+// from kPairItems (token, 64 heads) items on, which leave little to split, up to kPairWide.
+// 64 heads, 576 wide, splits / pairs, us: 132 slots, 1 token 13.5 / 11.5, 64 tokens 15.0 /
+// 12.6, fp8 rows 1 token 12.7 / 11.7; 184 slots, 1 token 12.9 / 12.7, 32 tokens 13.2 / 13.1;
+// 256 slots, 16 tokens 13.0 / 15.2, 64 tokens 15.2 / 15.9, 96 tokens 18.0 / 16.3, 128 tokens
+// 20.9 / 16.9; 400 slots, 96 tokens 21.2 / 21.1, 32 tokens 15.2 / 20.4. 16 heads fill a
+// quarter of a pair kernel's workgroup: 132 slots, 1 token 13.0 / 13.9.
+constexpr int kPairWindow = 192, kPairWide = 320, kPairItems = 96;
 
 int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   if (!a) return sas::set_error(SAS_EINVAL, "null args");
@@ -2039,8 +2046,9 @@ int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   // spills (the staging registers beside the scale groups): 4 waves there.
   if (nw <= 0) nw = (hw == 2 || (hw == 4 && !fp8)) ? 8 : 4;
   if (nw != 4 && nw != 8) return sas::set_error(SAS_EINVAL, "waves must be 4 or 8");
-  pl->window = kFirst && a->scenario == SAS_SWA && pl->nslots <= kPairWindow && a->num_splits <= 0 &&
-               a->head_waves == 0 && a->waves == 0 && T * ((a->H + 63) / 64) >= 32;
+  const long long items = T * ((a->H + 63) / 64);
+  pl->window = kFirst && a->scenario == SAS_SWA && a->H > 16 && a->num_splits <= 0 && a->head_waves == 0 && a->waves == 0 &&
+               (pl->nslots <= kPairWindow || (pl->nslots <= kPairWide && items >= kPairItems));
   if (hw == 1 || pl->exact) nw = 4;
   pl->nw = nw;
   pl->hw = hw;
@@ -2255,7 +2263,8 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
   if (pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
   const long long items = a->T * ((a->H + 63) / 64), cus = sas::device_cus();
-  if (pl.exact || (kFirst && pl.window)) return items >= 32;
+  if (pl.exact) return items >= 32;
+  if (kFirst && pl.window) return true;
   if (a->T * pl.nhg <= cus) return false;
   if (a->kv_dtype != a->q_dtype && pl.hw == 2) return a->H > 32 && (items > cus || pl.nslots <= 640);
   return true;
