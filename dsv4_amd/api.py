@@ -1018,9 +1018,9 @@ def sparse_attn_sharedkv_first(
     ori_win_left`` or ``j < ori_first``, each once, and the compressed rows as ever. So a
     sequence can run on without end with a window's blocks and those of its first rows: the
     blocks between may be given back and their entries of ``ori_block_table`` be -1.
-    ``ori_first`` 0 gives :func:`sparse_attn_sharedkv`'s mask. Draft trees, and rows whose
-    gradients are wanted in fp8, are not served; the other arguments and the result are that
-    function's. Its gradients: :func:`sparse_attn_sharedkv_first_backward`.
+    ``ori_first`` 0 gives :func:`sparse_attn_sharedkv`'s mask. The other arguments and the
+    result are that function's. Its gradients (of rows in q's dtype):
+    :func:`sparse_attn_sharedkv_first_backward`.
     """
     ori_first = _first_rows(ori_first)
     key = _signature("first", q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
