@@ -966,8 +966,8 @@ _TREE_DEFAULTS = {k: v for k, v in _FWD_DEFAULTS.items() if k not in (
 
 
 def _first_rows(ori_first) -> int:
-    if isinstance(ori_first, bool) or not isinstance(ori_first, int) or ori_first < 0:
-        raise ValueError(f"ori_first must be an integer of at least 0 (got {ori_first!r})")
+    if isinstance(ori_first, bool) or not isinstance(ori_first, int) or not 0 <= ori_first < 1 << 31:
+        raise ValueError(f"ori_first must be an integer of at least 0 (below 2^31, got {ori_first!r})")
     return ori_first
 
 
@@ -1230,6 +1230,7 @@ def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBack
     if ori_first is None:
         call = prepare_sparse_attn_sharedkv(q, **kwargs)
     else:
+        ori_first = _first_rows(ori_first)
         call = PreparedCall(_resolve(q, ori_first=ori_first, **dict(_FWD_DEFAULTS, **kwargs)))
     # a copy: the forward's resolved split count stays with the forward. The
     # backward takes the caller's count, or plans its own (0); the forward's

@@ -276,8 +276,8 @@ def evict_kv_cache(
     for name, v in (("budget", budget), ("keep_first", keep_first), ("keep_recent", keep_recent)):
         if isinstance(v, bool) or not isinstance(v, int):
             raise ValueError(f"{name} must be an integer (got {v!r})")
-    if budget < 1 or keep_first < 0 or keep_recent < 0 or keep_first + keep_recent > budget:
-        raise ValueError(f"budget must be at least 1 and hold keep_first and keep_recent (got {budget}, {keep_first}, "
+    if not 1 <= budget <= 1 << 30 or keep_first < 0 or keep_recent < 0 or keep_first + keep_recent > budget:
+        raise ValueError(f"budget must be at least 1, at most 2^30, and hold keep_first and keep_recent (got {budget}, {keep_first}, "
                          f"{keep_recent})")
     dev = cache.device
     if weights.device != dev or block_table.device != dev or seqused_kv.device != dev:

@@ -341,7 +341,7 @@ def test_python_refuses():
     kw = dict(ori_kv=torch.zeros(1, 16, 1, 512, dtype=torch.bfloat16), ori_block_table=i[:1, None], cu_seqlens_q=i,
               seqused_kv=i[:1], softmax_scale=1.0)
     sinks = torch.zeros(16)
-    for bad in (-1, 1.0, True, None):
+    for bad in (-1, 1.0, True, None, 1 << 31, 1 << 70):
         with pytest.raises(ValueError, match="ori_first"):
             sparse_attn_sharedkv_first(q, ori_first=bad, sinks=sinks, **kw)
         with pytest.raises(ValueError, match="ori_first"):
@@ -370,7 +370,8 @@ def test_python_refuses():
     for bad in (w.float(), w[0], torch.zeros(2, 16, dtype=torch.float64)):
         with pytest.raises(ValueError, match="weights must be"):
             evict_kv_cache(c, bad, i[:1, None], i[:1], **e)
-    for bad in (dict(budget=0), dict(budget=4, keep_first=-1), dict(budget=4, keep_first=3, keep_recent=2)):
+    for bad in (dict(budget=0), dict(budget=4, keep_first=-1), dict(budget=4, keep_first=3, keep_recent=2),
+                dict(budget=(1 << 30) + 1), dict(budget=1 << 70), dict(budget=4, keep_first=1 << 70)):
         with pytest.raises(ValueError, match="budget must be at least 1"):
             evict_kv_cache(c, w, i[:1, None], i[:1], **bad)
     with pytest.raises(ValueError, match="must be an integer"):
@@ -397,6 +398,10 @@ ATTN = {
     "fp8_h128": dict(kind="cfa", dt="fp8", H=128, D=576, ql=[5], kl=[500], ratio=8, F=17),
     "cfa": dict(kind="cfa", H=64, D=576, ql=[9, 14], kl=[800, 90], ratio=8),
     "odd_heads": dict(H=48, D=576, ql=[7, 2], kl=[400, 33], F=5, win=100),
+    "one_h32": dict(H=32, D=512, ql=[1], kl=[300]),
+    "one_h80": dict(dt="fp16", H=80, D=576, ql=[1], kl=[200], F=60),
+    "one_fp8_h48": dict(dt="fp8", H=48, D=576, ql=[1, 0, 1], kl=[300, 5, 1], F=9),
+    "many_256": dict(H=64, D=576, ql=[50, 30, 20], kl=[500, 200, 20], F=7, win=249),
     "missing_rows": dict(kind="scfa", H=64, D=576, ql=[12, 70], kl=[5, 30], K=70),
     "holes": dict(H=64, D=576, ql=[4, 4], kl=[270, 290], holes=True),
     "empty_between": dict(H=64, D=512, ql=[4, 0, 5], kl=[270, 7, 190], gap=True),
