@@ -1370,6 +1370,9 @@ def sparse_attn_sharedkv_first_autograd(q: torch.Tensor, *, ori_first: int, ori_
                                         cmp_kv: Optional[torch.Tensor] = None, sinks: torch.Tensor,
                                         return_softmax_lse: bool = False, **kwargs):
     """:func:`sparse_attn_sharedkv_first` recorded for autograd, as
-    :func:`sparse_attn_sharedkv_autograd` records the attention without first rows."""
+    :func:`sparse_attn_sharedkv_autograd` records the attention without first rows. To
+    capture a training step while an eager graph of the same leaves lives, capture
+    :func:`sparse_attn_sharedkv_first_backward`: PyTorch ends the process where a captured
+    ``backward()`` meets such a graph."""
     out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, dict(kwargs, ori_first=ori_first))
     return (out, lse) if return_softmax_lse else out

@@ -145,6 +145,9 @@ __device__ __forceinline__ int lanes_before(uint64_t m) {
   return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
+// (Weights that another stream changes meanwhile give any choice of rows, but no access out
+// of range: places are held below the lists' ends, and the moves look at what they are given.)
+
 // A sequence of n > budget rows. Wave w has the run of rows from w * run on, lane l its rows
 // l, l + 64, ..: E of them in registers, or (E = 0) read where they are needed.
 template <int E>
@@ -225,8 +228,7 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
       __syncthreads();
       scan([&](int j, Key k) {
         const int at = atomicAdd(&sh.nrank, 1);
-        sh.rkey[at] = k;
-        sh.rpos[at] = j;
+        if (at < kRank) { sh.rkey[at] = k; sh.rpos[at] = j; }
       });
       rank_keys(sh, left, need);
       edge = sh.edge;
@@ -265,7 +267,7 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
         if (lane == 63) at = atomicAdd(&sh.nlist, y);
         at = __shfl(at, 63) + y - mine;
         each([&](int j, Key k) {
-          if (is_key(k) && same(k)) { big.lkey[at] = k; big.lpos[at] = j; ++at; }
+          if (is_key(k) && same(k) && at < kList) { big.lkey[at] = k; big.lpos[at] = j; ++at; }
         });
         listed = left;
         __syncthreads();
@@ -309,7 +311,7 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
     split(k, over, tie);
     if (over | tie) {
       const int rank = pt + lanes_before(tie), at = pk + lanes_before(over) + min(rank, need);
-      if ((over >> lane & 1) || ((tie >> lane & 1) && rank < need)) kept[at] = j;
+      if (((over >> lane & 1) || ((tie >> lane & 1) && rank < need)) && (unsigned)at < (unsigned)p.budget) kept[at] = j;
       pk += __popcll(over);
       pt += __popcll(tie);
     }
@@ -328,7 +330,7 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   const int lo = p.first, hi = n - p.recent;
   int need = p.budget - p.first - p.recent, left = hi - lo;
   const int run = ((n - 1) / (2 * kSelThreads) + 1) * 128, r0 = wave * run;   // 16 runs: at most kWordRows
-  auto weight = [&](int j) { return j < p.weight_rows ? w[j] : 0.; };
+  auto weight = [&](int j) { return (unsigned)j < (unsigned)p.weight_rows ? w[j] : 0.; };
   auto each = [&](auto&& f) __attribute__((always_inline)) {   // f(row, word)
     for (int i = 0; i < run; i += 128) {
       const int j = r0 + i + lane;
@@ -390,6 +392,10 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
   Key edge{kStays - 1, ~0u}, prefix{0, 0}, mask{0, 0};
   bool done = need == 0, sorted = false;   // sorted: the rows that share the edge's high word are told apart
   int pass = 0;
+  auto take = [&](int j) {
+    const int at = atomicAdd(&sh.nrank, 1);
+    if (at < kRank) sh.rpos[at] = j;
+  };
   // the need-th of the `left` rows in rpos; `all`: no other row has one of their high words
   auto rank_list = [&](bool all) {
     __syncthreads();
@@ -434,7 +440,7 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
         base += (uint32_t)bin << s;
         if (left <= kRank) {
           each([&](int j, uint32_t k) {
-            if (is_word(k) && (k - base) >> s == 0) sh.rpos[atomicAdd(&sh.nrank, 1)] = j;
+            if (is_word(k) && (k - base) >> s == 0) take(j);
           });
           rank_list(true);
           break;
@@ -481,7 +487,6 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
       need = 0;
       done = true;
     } else if (left <= kRank) {
-      auto take = [&](int j) { sh.rpos[atomicAdd(&sh.nrank, 1)] = j; };
       if (high)
         each([&](int j, uint32_t k) {
           if (is_word(k) && (k & mask.hi) == prefix.hi) take(j);
@@ -532,7 +537,7 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
       stays |= k == edge.hi && rank < need;
       pt += __popcll(tie);
     }
-    if (stays) kept[at] = j;
+    if (stays && (unsigned)at < (unsigned)p.budget) kept[at] = j;
     pk += __popcll(over);
   });
 }
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
 #pragma unroll
       for (int u = 0; u < UW; ++u) {
         const int i = i0 + u * kMoveThreads + tid, j = i < m ? kept[i] : n;
-        v[u] = j < n && j < p.weight_rows ? w[j] : 0.;
+        v[u] = (unsigned)j < (unsigned)min(n, p.weight_rows) ? w[j] : 0.;
       }
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();   // the chunk's weights are read; later ones lie behind it
