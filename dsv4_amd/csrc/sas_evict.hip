@@ -221,6 +221,59 @@ __device__ __forceinline__ void select_rows(const EvictParams& p, SelShared& big
     }
   };
   if (tid == 0) sh.nlist = sh.nrank = 0;
+  if constexpr (E > 0) {
+    if (!done && left > kRank) {
+      // first over the range of the positive weights, in up to 2047 even steps of their high
+      // words (bin 0: the others): a bin of few keys, or of one key (0), ends the search
+      uint32_t most = 0, least = ~0u;   // the highest word, and the lowest above 0's less that and 1
+      each([&](int, Key k) {
+        const uint32_t h = is_key(k) ? k.hi : 0u;
+        most = max(most, h);
+        least = min(least, h - (kZero + 1));
+      });
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { most = max(most, __shfl_xor(most, d)); least = min(least, __shfl_xor(least, d)); }
+      for (int i = tid; i < kCopies * kBins; i += kSelThreads) (&big.hist[0][0])[i] = 0;
+      if (tid < 4) sh.any[tid] = tid & 1 ? ~0u : 0u;
+      __syncthreads();
+      if (lane == 0) { atomicMax(&sh.any[0], most); atomicMin(&sh.any[1], least); }
+      __syncthreads();
+      most = __builtin_amdgcn_readfirstlane(sh.any[0]);
+      const uint32_t base = min(kZero + 1 + (uint32_t)__builtin_amdgcn_readfirstlane(sh.any[1]), most);
+      const int s = max(0, 32 - __clz((int)((most - base) / (kBins - 1))));
+      auto bin_of = [&](Key k) { return k.hi > kZero ? 1 + (int)((k.hi - base) >> s) : 0; };
+      int* hist = big.hist[lane % kCopies];
+      each([&](int, Key k) {
+        if (is_key(k)) atomicAdd(&hist[bin_of(k)], 1);
+      });
+      find_bin(sh, need, [&](int i) { return big.hist[0][i] + big.hist[1][i] + big.hist[2][i] + big.hist[3][i]; });
+      const int bin = __builtin_amdgcn_readfirstlane(sh.found[0]), rest = need - __builtin_amdgcn_readfirstlane(sh.found[1]);
+      const int in = __builtin_amdgcn_readfirstlane(sh.found[2]);
+      if (in <= kRank) {
+        each([&](int j, Key k) {
+          if (is_key(k) && bin_of(k) == bin) {
+            const int at = atomicAdd(&sh.nrank, 1);
+            if (at < kRank) { sh.rkey[at] = k; sh.rpos[at] = j; }
+          }
+        });
+        rank_keys(sh, in, rest);
+        edge = sh.edge;
+        need = sh.need;
+        done = true;
+      } else if (bin == 0) {
+        if (tid < 4) sh.any[tid] = tid & 1 ? ~0u : 0u;
+        __syncthreads();
+        uint32_t o[4] = {0, ~0u, 0, ~0u};
+        bool has = false;
+        each([&](int, Key k) {
+          if (is_key(k) && k.hi <= kZero) { o[0] |= k.hi; o[1] &= k.hi; o[2] |= k.lo; o[3] &= k.lo; has = true; }
+        });
+        const bool hi1 = one_word(sh.any, o[0], o[1], has), lo1 = one_word(sh.any + 2, o[2], o[3], has);
+        if (hi1 && lo1) { edge = Key{sh.any[0], sh.any[2]}; need = rest; done = true; }
+      }
+      __syncthreads();   // found and any are read
+    }
+  }
   // passes: bits 21.., 10.., 0.. of the high word, then of the low one
   for (int pass = 0; !done && pass < 6; ++pass) {
     if (left <= kRank) {
@@ -434,6 +487,23 @@ __device__ __forceinline__ void select_long(const EvictParams& p, SelLong& big, 
       });
       find_bin(sh, need, [&](int i) { return big.hist[i]; });
       int bin = __builtin_amdgcn_readfirstlane(sh.found[0]) - 1;
+      if (bin < 0) {
+        // 0 and below: often one key
+        const int above = __builtin_amdgcn_readfirstlane(sh.found[1]);
+        clear();
+        uint32_t o = 0, x = ~0u;
+        bool has = false;
+        each([&](int, uint32_t k) {
+          if (is_word(k) && k <= kZero) { o |= k; x &= k; has = true; }
+        });
+        if (one_word(sh.any, o, x, has)) {
+          prefix.hi = sh.any[0];
+          mask.hi = ~0u;
+          need -= above;
+          pass = 3;
+          one_low();
+        }
+      }
       while (bin >= 0) {
         need -= __builtin_amdgcn_readfirstlane(sh.found[1]);
         left = __builtin_amdgcn_readfirstlane(sh.found[2]);
