@@ -520,6 +520,8 @@ GRAD = {
     "prompt_33_rows": dict(dt="fp16", H=64, D=512, ql=[120], kl=[150], F=33, win=3),
     "prompt_missing": dict(H=32, D=576, ql=[100, 80], kl=[60, 300], F=6, win=20),
     "prompt_holes": dict(H=64, D=512, ql=[100, 80], kl=[260, 300], holes=True, F=6, win=20),
+    "dense_32_heads": dict(kind="scfa", H=32, D=512, ql=[120], kl=[3300], K=64, F=9, win=70, ratio=4),   # 448 to 896 rows: key-major
+    "sparse_32_heads": dict(kind="scfa", H=32, D=512, ql=[70], kl=[3700], K=64, F=9, win=70, ratio=4),   # past 896 rows: per token
     "sparse_beyond": dict(kind="scfa", H=64, D=576, ql=[90], kl=[900], K=6, F=9, win=70),   # tokens whose rows are added per token
 }
 
