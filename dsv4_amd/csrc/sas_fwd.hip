@@ -2248,7 +2248,8 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 //  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows of
 //    576 channels, 32 / 64 / 128 / 256 items: 11.9 / 12.2 / 12.5 / 13.5 us against 12.3 / 14.0 /
 //    15.0 / 15.9, fp8 16.1 / 16.4 / 16.4 / 17.3 against 16.6 / 17.2 / 18.1 / 32; fewer items: the
-//    same within 4%); or
+//    same within 4%);
+//  - a window with its first rows (kPairWindow above); or
 //  - more workgroups of the other kernel than CUs, which hold one each (a second round).
 //    480 nodes, 128 + 1024 rows, 16 / 32 / 48 / 64 / 96 heads: 51 / 64 / 79 / 86 / 151 us against
 //    143 / 90 / 408 / 99 / 267 (heads that are no multiple of 32 leave it 16 a workgroup); 96
