@@ -1962,20 +1962,20 @@ int part_bytes(int q_dtype) { return q_dtype == SAS_DT_FP16 ? 4 : 2; }
 struct Plan {
   int hw, nw, nhg, nslots, nsplit, sps;
   bool exact;   // exact-window schedule (Fwd::run_exact)
-  bool window;  // (kFirst) a window and its first rows in one split of the kernels of two workgroups a CU
   size_t ws;
 };
 
-// With first rows a 128-row window no longer fits the exact schedule. Where one round of
-// workgroups takes the call, each slot costs more in one split of the kernels of two
-// workgroups a CU than in several splits, but no combine follows: up to kPairWindow slots, and
-// from kPairItems (token, 64 heads) items on, which leave little to split, up to kPairWide.
-// 64 heads, 576 wide, splits / pairs, us: 132 slots, 1 token 13.5 / 11.5, 64 tokens 15.0 /
-// 12.6, fp8 rows 1 token 12.7 / 11.7; 184 slots, 1 token 12.9 / 12.7, 32 tokens 13.2 / 13.1;
-// 256 slots, 16 tokens 13.0 / 15.2, 64 tokens 15.2 / 15.9, 96 tokens 18.0 / 16.3, 128 tokens
-// 20.9 / 16.9; 400 slots, 96 tokens 21.2 / 21.1, 32 tokens 15.2 / 20.4. 16 heads fill a
-// quarter of a pair kernel's workgroup: 132 slots, 1 token 13.0 / 13.9.
-constexpr int kPairWindow = 192, kPairWide = 320, kPairItems = 96;
+// With first rows a 128-row window no longer fits the exact schedule, and its few slots in
+// several splits are a second launch that merges them. One split takes so many slots, or more
+// where two splits would fill the CUs. 64 heads, 576 wide, splits / one, us: 132 slots, 1 / 32 /
+// 64 / 96 / 128 tokens 11.5 / 11.2, 12.3 / 11.6, 14.0 / 12.2, 16.4 / 12.6, 19.0 / 13.1, fp8 rows
+// 1 / 32 / 64 tokens 12.1 / 11.6, 13.4 / 12.0, 14.6 / 12.3; 184 slots, 1 / 32 / 96 tokens 11.1 /
+// 12.3, 12.7 / 12.8, 16.5 / 13.6, fp8 12.0 / 11.9, 13.5 / 12.4; 256 slots, 32 / 64 (four
+// splits) / 96 (two) tokens 13.1 / 15.0, 14.4 / 15.4, 17.4 / 15.6; 400 slots, 96 / 128 tokens
+// 20.9 / 20.8, 23.1 / 21.4, fp8 64 tokens 18.0 / 19.9. 16 heads a workgroup: 132 slots, 1 token
+// 12.3 / 13.7. (One split of the kernels of two workgroups a CU: 132 slots, 1 / 64 tokens 12.2 /
+// 12.8, fp8 17.1 / 17.8.)
+constexpr int kOneSplit = 160, kNotTwoSplits = 320;
 
 int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   if (!a) return sas::set_error(SAS_EINVAL, "null args");
@@ -2046,14 +2046,11 @@ int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
   // spills (the staging registers beside the scale groups): 4 waves there.
   if (nw <= 0) nw = (hw == 2 || (hw == 4 && !fp8)) ? 8 : 4;
   if (nw != 4 && nw != 8) return sas::set_error(SAS_EINVAL, "waves must be 4 or 8");
-  const long long items = T * ((a->H + 63) / 64);
-  pl->window = kFirst && a->scenario == SAS_SWA && a->H > 16 && a->num_splits <= 0 && a->head_waves == 0 && a->waves == 0 &&
-               (pl->nslots <= kPairWindow || (pl->nslots <= kPairWide && items >= kPairItems));
   if (hw == 1 || pl->exact) nw = 4;
   pl->nw = nw;
   pl->hw = hw;
   pl->nhg = (int)a->H / (16 * hw);
-  if (pl->exact || pl->window) ns = 1;
+  if (pl->exact) ns = 1;
   if (ns <= 0) {
     // as many splits as fill each XCD's CUs in one round, each split at
     // least min_sps slots (1-token, 16-head decode: 15.5 µs at 4 splits of
@@ -2078,6 +2075,9 @@ int make_plan(const SasFwdArgs* a, long long first, Plan* pl) {
     };
     while (ns > 1 && steps(ns - 1) == steps(ns)) --ns;
   }
+  if (kFirst && a->scenario == SAS_SWA && a->num_splits <= 0 && hw > 1 &&
+      pl->nslots <= (ns <= 2 ? kNotTwoSplits : kOneSplit))
+    ns = 1;
   // 16-head groups run the exact schedule when a split's rows fit the ring
   // (every row gathered at once, no per-step barriers; 1-token, 16-head
   // decode: 12.7 µs against 15.5 µs for the register-streaming decode
@@ -2248,8 +2248,7 @@ int combine_impl(const SasCombineArgs* a, hipStream_t st) {
 //  - a window that the exact schedule holds, from 32 (token, 64 heads) items on (128 rows of
 //    576 channels, 32 / 64 / 128 / 256 items: 11.9 / 12.2 / 12.5 / 13.5 us against 12.3 / 14.0 /
 //    15.0 / 15.9, fp8 16.1 / 16.4 / 16.4 / 17.3 against 16.6 / 17.2 / 18.1 / 32; fewer items: the
-//    same within 4%);
-//  - a window with its first rows (kPairWindow above); or
+//    same within 4%); or
 //  - more workgroups of the other kernel than CUs, which hold one each (a second round).
 //    480 nodes, 128 + 1024 rows, 16 / 32 / 48 / 64 / 96 heads: 51 / 64 / 79 / 86 / 151 us against
 //    143 / 90 / 408 / 99 / 267 (heads that are no multiple of 32 leave it 16 a workgroup); 96
@@ -2265,7 +2264,6 @@ bool use_pairs(const SasFwdArgs* a, const Plan& pl) {
   if (pl.nsplit != 1 || pl.nslots > kMaxSlots || a->head_waves != 0 || a->waves != 0) return false;
   const long long items = a->T * ((a->H + 63) / 64), cus = sas::device_cus();
   if (pl.exact) return items >= 32;
-  if (kFirst && pl.window) return true;
   if (a->T * pl.nhg <= cus) return false;
   if (a->kv_dtype != a->q_dtype && pl.hw == 2) return a->H > 32 && (items > cus || pl.nslots <= 640);
   return true;
