@@ -1217,20 +1217,20 @@ def prepare_sparse_attn_sharedkv_backward(dout: torch.Tensor, q: torch.Tensor, o
     aligned, the window rows alone, beside the per-token kernel on a side
     stream); False, one add per (token, row). The results agree up to fp32
     summation order."""
-    return _prepare_backward(dout, q, out, lse, False, **kwargs)
+    return _prepare_backward(dout, q, out, lse, False, kwargs)
 
 
-def _prepare_backward(dout, q, out, lse, own_dq: bool, **kwargs) -> PreparedBackward:
+def _prepare_backward(dout, q, out, lse, own_dq: bool, kwargs: dict, ori_first: Optional[int] = None) -> PreparedBackward:
     """``own_dq``: dq may be a fresh tensor in q's dtype, written whole by one
     launch, where the library's plan writes it so (no fp32 buffer to clear
-    and convert)."""
+    and convert). ``kwargs``: the caller's keyword arguments; ``ori_first``: first rows
+    that stay visible (None: a call without them)."""
+    kwargs = dict(kwargs)
     kwargs.pop("return_softmax_lse", None)
     window_pass = kwargs.pop("window_pass", None)
-    ori_first = kwargs.pop("ori_first", None)
     if ori_first is None:
         call = prepare_sparse_attn_sharedkv(q, **kwargs)
     else:
-        ori_first = _first_rows(ori_first)
         call = PreparedCall(_resolve(q, ori_first=ori_first, **dict(_FWD_DEFAULTS, **kwargs)))
     # a copy: the forward's resolved split count stays with the forward. The
     # backward takes the caller's count, or plans its own (0); the forward's
@@ -1302,7 +1302,7 @@ def sparse_attn_sharedkv_backward(
     ``[H]``. Key sets are the forward's: window rows and the valid top-k (or
     dense compressed) rows; V is the first 512 channels of each row.
     """
-    pb = _prepare_backward(dout, q, out, lse, True, **kwargs)
+    pb = _prepare_backward(dout, q, out, lse, True, kwargs)
     pb.launch()
     return pb.result()
 
@@ -1323,23 +1323,23 @@ def sparse_attn_sharedkv_first_backward(
     if q.is_cuda and q.device.index != _device():
         with torch.cuda.device(q.device):
             return sparse_attn_sharedkv_first_backward(dout, q, out, lse, ori_first=ori_first, **kwargs)
-    pb = _prepare_backward(dout, q, out, lse, True, ori_first=ori_first, **kwargs)
+    pb = _prepare_backward(dout, q, out, lse, True, kwargs, ori_first)
     pb.launch()
     return pb.result()
 
 
 class _SparseAttnSharedkvFn(torch.autograd.Function):
     """Autograd binding: forward = :func:`sparse_attn_sharedkv` (keeping
-    out / LSE), backward = :func:`sparse_attn_sharedkv_backward`; with
-    ``ori_first`` among the arguments, those with first rows."""
+    out / LSE), backward = :func:`sparse_attn_sharedkv_backward`; ``first``
+    (``dict(ori_first=..)``, else empty): those with first rows."""
 
     @staticmethod
-    def forward(ctx, q, ori_kv, cmp_kv, sinks, kw):
+    def forward(ctx, q, ori_kv, cmp_kv, sinks, first, kw):
         kwargs = dict(kw, ori_kv=ori_kv, cmp_kv=cmp_kv, sinks=sinks)
-        fwd = sparse_attn_sharedkv_first if "ori_first" in kw else sparse_attn_sharedkv
-        out, lse = fwd(q, return_softmax_lse=True, **kwargs)
+        fwd = sparse_attn_sharedkv_first if first else sparse_attn_sharedkv
+        out, lse = fwd(q, return_softmax_lse=True, **first, **kwargs)
         ctx.save_for_backward(q, ori_kv, cmp_kv if cmp_kv is not None else torch.empty(0), sinks, out, lse)
-        ctx.kw = kw
+        ctx.first, ctx.kw = first, kw
         ctx.has_cmp = cmp_kv is not None
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -1348,11 +1348,11 @@ class _SparseAttnSharedkvFn(torch.autograd.Function):
     def backward(ctx, dout, dlse):
         q, ori_kv, cmp_kv, sinks, out, lse = ctx.saved_tensors
         kwargs = dict(ctx.kw, ori_kv=ori_kv, cmp_kv=cmp_kv if ctx.has_cmp else None, sinks=sinks)
-        bwd = sparse_attn_sharedkv_first_backward if "ori_first" in ctx.kw else sparse_attn_sharedkv_backward
+        bwd = sparse_attn_sharedkv_first_backward if ctx.first else sparse_attn_sharedkv_backward
         dq, d_ori, d_cmp, d_sinks = bwd(
-            dout.to(q.dtype).contiguous(), q, out, lse, **kwargs)
+            dout.to(q.dtype).contiguous(), q, out, lse, **ctx.first, **kwargs)
         return (dq, d_ori.to(ori_kv.dtype), d_cmp.to(cmp_kv.dtype) if ctx.has_cmp else None,
-                d_sinks.to(sinks.dtype), None)
+                d_sinks.to(sinks.dtype), None, None)
 
 
 def sparse_attn_sharedkv_autograd(q: torch.Tensor, *, ori_kv: torch.Tensor,
@@ -1362,7 +1362,7 @@ def sparse_attn_sharedkv_autograd(q: torch.Tensor, *, ori_kv: torch.Tensor,
     ``q``, ``ori_kv``, ``cmp_kv`` and ``sinks`` (through
     :func:`sparse_attn_sharedkv_backward`; the LSE output is not
     differentiable). Other arguments as for :func:`sparse_attn_sharedkv`."""
-    out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, kwargs)
+    out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, {}, kwargs)
     return (out, lse) if return_softmax_lse else out
 
 
@@ -1374,5 +1374,5 @@ def sparse_attn_sharedkv_first_autograd(q: torch.Tensor, *, ori_first: int, ori_
     capture a training step while an eager graph of the same leaves lives, capture
     :func:`sparse_attn_sharedkv_first_backward`: PyTorch ends the process where a captured
     ``backward()`` meets such a graph."""
-    out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, dict(kwargs, ori_first=ori_first))
+    out, lse = _SparseAttnSharedkvFn.apply(q, ori_kv, cmp_kv, sinks, dict(ori_first=ori_first), kwargs)
     return (out, lse) if return_softmax_lse else out
