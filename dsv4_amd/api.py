@@ -1318,7 +1318,10 @@ def sparse_attn_sharedkv_first_backward(
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], torch.Tensor]:
     """Gradients of :func:`sparse_attn_sharedkv_first`: as
     :func:`sparse_attn_sharedkv_backward`, over that forward's keys; ``kwargs`` are
-    its keyword arguments."""
+    its keyword arguments, and ``window_pass`` as in
+    :func:`prepare_sparse_attn_sharedkv_backward`, but that True is refused where H is not
+    a multiple of 32 or q or dout not 16-byte aligned (raw rows' gradients are summed
+    key-major together with all others or not at all)."""
     ori_first = _first_rows(ori_first)
     if q.is_cuda and q.device.index != _device():
         with torch.cuda.device(q.device):

@@ -1062,6 +1062,10 @@ int bwd_impl(const SasBwdArgs* ba, long long first, void* stream) {
   const PrePlan pre = plan_prefill(ba, first);
   if (direct && !(pre.on && have_ws))
     return set_error(SAS_EINVAL, "bwd: SAS_BWD_DQ_DTYPE without SAS_BWD_WORKSPACE or where sas_bwd_plan does not allow it");
+  // (key-major sums of first rows are the prefill path's alone)
+  if (kBwdFirst && (a->flags & SAS_BWD_WINDOW_KEYS) && !(pre.on && have_ws))
+    return set_error(SAS_EINVAL, "bwd: SAS_BWD_WINDOW_KEYS with first rows where sas_bwd_first_plan reports no workspace "
+                     "(H %% 32, odd addresses of q or dout, num_splits), or without it");
   if (kBwdFirst && have_ws && pre.on && (reinterpret_cast<uintptr_t>(a->out) & 15))
     return set_error(SAS_EINVAL, "bwd: out must be 16-byte aligned");
   if (have_ws && pre.on && (!a->workspace || a->workspace_bytes < pre.ws))

@@ -318,8 +318,10 @@ int sas_bwd_plan(const SasBwdArgs* a, int32_t* dq_dtype, size_t* workspace_bytes
  * Backward of sas_fwd_first_v1: sas_bwd_v1's contract over that forward's keys. The
  * first rows' gradients are summed with the window rows': key-major where sas_bwd_v1
  * takes its prefill path (sas_bwd_first_plan reports its workspace), else one add per
- * (token, row, head group, channel); SAS_BWD_WINDOW_KEYS means the former alone. With a
- * workspace, out is 16-byte aligned.
+ * (token, row, head group, channel), window rows' too. SAS_BWD_WINDOW_KEYS asks for the
+ * former and is refused where that is not to be had: no workspace, or none reported (H no
+ * multiple of 32, q or dout not 16-byte aligned, num_splits given). With a workspace, out is
+ * 16-byte aligned.
  */
 typedef struct SasBwdFirstArgs {
   SasBwdArgs bwd;

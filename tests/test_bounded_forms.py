@@ -3,8 +3,13 @@ refused."""
 
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
+
+from dsv4_amd import _lib
+from test_bounded import _fwd_args, _refused
 
 
 def test_calls_without_first_rows_refuse_them():
@@ -23,3 +28,17 @@ def test_calls_without_first_rows_refuse_them():
                      lambda: api.prepare_sparse_attn_sharedkv_backward(q, q, q, lse, ori_first=first, **kw)):
             with pytest.raises(TypeError, match="ori_first"):
                 call()
+
+
+def test_abi_key_major_sums_of_first_rows_are_refused_where_there_are_none():
+    """SAS_BWD_WINDOW_KEYS with first rows: 16 and 48 heads, an odd address, a split count, no
+    workspace."""
+    L, fake = _lib.lib(), 1 << 20
+    mk = lambda dout=fake, **kw: _lib.SasBwdFirstArgs(_lib.SasBwdArgs(  # noqa: E731
+        fwd=_fwd_args(**dict(dict(T=4096, flags=_lib.SAS_BWD_WINDOW_KEYS), **kw)), dout=dout, dq=fake, d_ori_kv=fake, d_sinks=fake), 4)
+    direct, ws = C.c_int32(0), C.c_size_t(1)
+    for kw in (dict(H=16), dict(H=48), dict(q=fake + 8), dict(dout=fake + 8), dict(num_splits=2)):
+        assert L.sas_bwd_first_plan(C.byref(mk(**kw)), C.byref(direct), C.byref(ws)) == _lib.SAS_OK and ws.value == 0
+        _refused(L.sas_bwd_first_v1, mk(**kw), "SAS_BWD_WINDOW_KEYS with first rows")
+    assert L.sas_bwd_first_plan(C.byref(mk()), C.byref(direct), C.byref(ws)) == _lib.SAS_OK and ws.value > 0
+    _refused(L.sas_bwd_first_v1, mk(), "or without it")
