@@ -904,14 +904,18 @@ PrePlan plan_prefill(const SasBwdArgs* ba, long long first) {
   // 810, 1148 / 803 us. They meet between 7 K and 11 K.
   const long long cap = a->scenario >= SAS_CFA ? a->cmp_bt_stride * a->cmp_block_size : 0;
   // With first rows, where the per-token kernel's adds are one per 32 heads (H no multiple of
-  // 64) and not per 64, they meet at twice that from 64 entries on. Packed prompts, 7 K / 14 K:
-  // 32 heads, six of 70 to 250 tokens at 300 to 4000, K = 16 / 32 / 64 / 96 / 256: 203 against
-  // 204, 220 / 242, 265 / 221, 286 / 225, 243 / 242 us; four of 300 at 2000 to 5000 330 / 325,
-  // 348 / 394, 459 / 342, 455 / 346, 375 / 373; 2000 tokens 426 / 429, 463 / 496, 593 / 584,
-  // 684 / 563, 598 / 597; 96 heads, three of 100 to 400 337 / 340, 370 / 342, 381 / 401, 422 /
-  // 359, 383 / 385. 64 heads, K = 64, 4096 tokens 1616 / 1412 (at 20 K), eight of 100 to 400 at
-  // 1000 to 8000 870 / 930: as without first rows.
-  const int dense_k = kBwdFirst && a->H % 64 && a->K >= 64 ? 2 * SAS_BWD_DENSE : SAS_BWD_DENSE;
+  // 64) and not per 64, they meet at twice that for lists of 64 to 128. Packed prompts, 7 K / 14 K:
+  // 32 heads, six of 70 to 250 tokens at 300 to 4000, K = 16 / 32 / 64 / 96: 203 against 204, 220
+  // / 242, 265 / 221, 286 / 225 us; four of 300 at 2000 to 5000 330 / 325, 348 / 394, 459 / 342,
+  // 455 / 346; 2000 tokens 426 / 429, 463 / 496, 593 / 584, 684 / 563; 96 heads, three of 100 to
+  // 400 337 / 340, 370 / 342, 381 / 401, 422 / 359. Of longer ones, K = 64 / 128 / 256 / 512: 32
+  // heads, six of 70 to 250 at 4000 to 14000 382 / 355, 465 / 446, 537 / 497, 537 / 537, at 14000
+  // to 28000 347 / 317, 405 / 412, 585 / 659, 938 / 979, four of 300 there 473 / 435, 565 / 577,
+  // 832 / 1003, 1432 / 1406, 1000 tokens at 20000 331 / 305, 403 / 413, 609 / 616, 1010 / 940; 96
+  // heads, six of 70 to 250 at 4000 to 14000 930 / 895, 1195 / 1051, 1284 / 1199, 1299 / 1298, at
+  // 14000 to 28000 769 / 732, 983 / 985, 1469 / 1691, 2524 / 2953. 64 heads, K = 64, 4096 tokens
+  // 1616 / 1412 (at 20 K), eight of 100 to 400 at 1000 to 8000 870 / 930: as without first rows.
+  const int dense_k = kBwdFirst && a->H % 64 && a->K >= 64 && a->K <= 128 ? 2 * SAS_BWD_DENSE : SAS_BWD_DENSE;
   const long long dense = a->scenario == SAS_SCFA ? std::min<long long>(INT_MAX, dense_k * a->K) : INT_MAX;
   // Thresholds follow the sequences, not the table: where a table has at most
   // `dense` rows, every token is key-major, also one whose threshold lies past

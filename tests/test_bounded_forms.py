@@ -1,5 +1,6 @@
 """Bounded caches, further forms of the calls that tests/test_bounded.py covers: what is
-refused."""
+refused, lists of compressed rows each side of the planner's limits. Tolerances are that
+file's."""
 
 from __future__ import annotations
 
@@ -9,7 +10,7 @@ import pytest
 import torch
 
 from dsv4_amd import _lib
-from test_bounded import _fwd_args, _refused
+from test_bounded import Case, _check_grads, _fwd_args, _grads, _refused, _run
 
 
 def test_calls_without_first_rows_refuse_them():
@@ -42,3 +43,25 @@ def test_abi_key_major_sums_of_first_rows_are_refused_where_there_are_none():
         _refused(L.sas_bwd_first_v1, mk(**kw), "SAS_BWD_WINDOW_KEYS with first rows")
     assert L.sas_bwd_first_plan(C.byref(mk()), C.byref(direct), C.byref(ws)) == _lib.SAS_OK and ws.value > 0
     _refused(L.sas_bwd_first_v1, mk(), "or without it")
+
+
+# ---------------------------------------------------------------------------
+# GPU: gradients
+# ---------------------------------------------------------------------------
+
+GRAD = {
+    # 1525 compressed rows: below 14 times lists of 128, past 7 times lists of 144 (7 times
+    # those of 256 again not)
+    "topk_128": dict(kind="scfa", H=32, D=512, ql=[70], kl=[6100], K=128, F=9, win=70),
+    "topk_144": dict(kind="scfa", H=32, D=512, ql=[70], kl=[6100], K=144, F=9, win=70),
+    "topk_256": dict(kind="scfa", dt="fp16", H=96, D=576, ql=[70], kl=[6100], K=256, F=9, win=70),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(GRAD))
+def test_gpu_first_backward(name):
+    c = Case(**GRAD[name])
+    kw = c.kwargs()
+    out, lse = _run(c, **kw)
+    _check_grads(c, _grads(c, out, lse, kw), out, lse)
