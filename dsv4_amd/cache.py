@@ -263,6 +263,16 @@ def evict_kv_cache(
     positions of the rows that stay (-1 past the last): what else is kept by row moves by it.
     A row whose old or new place has no block is not moved. Sequences that share a block (a
     common prefix) must not be evicted from. No host sync.
+
+    Beside compressed rows: the attention finds a token's compressed rows by its position,
+    which ``seqused_kv`` gives it, so raw rows of a layer that has compressed ones are not to
+    be evicted (their number in ``seqused_kv``'s place hides compressed rows; a window and
+    ``ori_first`` bound them). Compressed rows may be, with their own lengths here
+    (``seqused_kv // cmp_ratio``, later what the last eviction returned and the rows since):
+    the attention goes on with ``seqused_kv`` as it was and ``cmp_sparse_indices`` that name
+    rows by their new places (the old row ``kept[b, i]`` is ``i``). Its dense form, without
+    lists, reads every row up to the threshold, also the bytes that an eviction leaves
+    behind: after one, give lists of all rows that are left.
     """
     if cache.dim() != 4 or cache.shape[2] != 1 or not cache.is_contiguous():
         raise ValueError(f"cache must be contiguous [num_blocks, block_size, 1, row], got {tuple(cache.shape)}")

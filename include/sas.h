@@ -365,6 +365,10 @@ int sas_row_weights_v1(const SasRowWeightsArgs* a, void* stream);
  * of the rows that stay, -1 past them; act_kv_out[b] is min(act_kv[b], budget), in memory of
  * its own. Sequences of at most `budget` rows stay as they are. A row whose source
  * or destination has no block is not moved. No two sequences may share a block.
+ * Raw rows of a layer with compressed rows are not to be evicted: act_kv is what a token's
+ * compressed rows are found by (its position, over cmp_ratio). Compressed rows may be, with
+ * their own lengths as act_kv here; SAS_SCFA's lists then name them by their new places and
+ * SasFwdArgs.act_kv stays as it was. SAS_CFA would read the bytes past the rows that stay.
  */
 typedef struct SasCacheEvictArgs {
   void* cache;                   /* [num_blocks, block_size, row_bytes] bytes */

@@ -1,5 +1,6 @@
 """Bounded caches, further forms of the calls that tests/test_bounded.py covers: what is
-refused, lists of compressed rows each side of the planner's limits. Tolerances are that
+refused, lists of compressed rows each side of the planner's limits, evictions of compressed
+rows. Tolerances are that
 file's."""
 
 from __future__ import annotations
@@ -65,3 +66,44 @@ def test_gpu_first_backward(name):
     kw = c.kwargs()
     out, lse = _run(c, **kw)
     _check_grads(c, _grads(c, out, lse, kw), out, lse)
+
+
+# ---------------------------------------------------------------------------
+# GPU: evictions of compressed rows
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense", [False, True])
+def test_gpu_evicted_compressed_rows(dense):
+    """Compressed rows cut down to a budget by their own lengths, then attended by lists of
+    their new places (of all of them after a dense call), lengths as before: what lists of the
+    old places give over the whole cache, weights too."""
+    from dsv4_amd.api import add_row_weights, sparse_attn_sharedkv
+    from dsv4_amd.cache import evict_kv_cache
+    budget, ratio = 40, 4
+    c = Case(kind="cfa" if dense else "scfa", H=32, D=576, ql=[1, 2, 1], kl=[600, 410, 90], K=60, ratio=ratio, win=64)
+    kw, q = c.kwargs(first=False), c.q.cuda()
+    out, lse = sparse_attn_sharedkv(q, return_softmax_lse=True, **kw)
+    weights = torch.zeros(3, c.ctable.shape[1] * c.bs, dtype=torch.float64, device="cuda")
+    add_row_weights(q, lse, cmp_weights=weights, **kw)
+    cut = kw["cmp_kv"].clone()
+    rows, kept = evict_kv_cache(cut, weights, kw["cmp_block_table"], kw["seqused_kv"] // ratio, budget=budget, keep_recent=4)
+    assert rows.tolist() == [budget, budget, 22]
+    seq = torch.tensor([0, 1, 1, 2], device="cuda")
+    new = torch.arange(budget, dtype=torch.int32, device="cuda").expand(4, budget)
+    new = torch.where(new < rows[seq][:, None], new, -1)
+    if not dense:
+        new = new[:, torch.randperm(budget, generator=torch.Generator().manual_seed(5))[:25].cuda()]
+    old = torch.where(new >= 0, kept[seq].gather(1, new.clamp(min=0).long()), -1)
+    # (of two tokens the earlier may not see the last row: lists hold what both see)
+    thr = torch.tensor([600, 409, 410, 90], device="cuda")[:, None] // ratio
+    new = torch.where(old < thr, new, -1)
+    lists = lambda x: dict(kw, cmp_sparse_indices=x.unsqueeze(1).contiguous())  # noqa: E731
+    want, want_lse = sparse_attn_sharedkv(q, return_softmax_lse=True, **lists(old))
+    got, got_lse = sparse_attn_sharedkv(q, return_softmax_lse=True, **dict(lists(new), cmp_kv=cut))
+    assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+    a, b = torch.zeros_like(weights), torch.zeros_like(weights)
+    add_row_weights(q, got_lse, cmp_weights=a, **dict(lists(new), cmp_kv=cut))
+    add_row_weights(q, want_lse, cmp_weights=b, **lists(old))
+    for i, n in enumerate(rows.tolist()):
+        assert torch.equal(a[i, :n], b[i, kept[i, :n].long()]) and not bool(a[i, n:].any())
