@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from dsv4_amd import _lib
-from test_bounded import Case, _check_grads, _fwd_args, _grads, _refused, _run
+from oracle import bounded_ref as R
+from test_bounded import Case, _check_grads, _evict, _evict_case, _fwd_args, _grads, _refused, _run, _same, _weights, _zeros
 
 
 def test_calls_without_first_rows_refuse_them():
@@ -56,6 +57,17 @@ GRAD = {
     "topk_128": dict(kind="scfa", H=32, D=512, ql=[70], kl=[6100], K=128, F=9, win=70),
     "topk_144": dict(kind="scfa", H=32, D=512, ql=[70], kl=[6100], K=144, F=9, win=70),
     "topk_256": dict(kind="scfa", dt="fp16", H=96, D=576, ql=[70], kl=[6100], K=256, F=9, win=70),
+    # more slots than a workgroup resolves (1280): two passes that divide the first rows (one
+    # sequence has none in the second), or the window; three, two of them without raw rows
+    "passes_first": dict(H=32, D=512, ql=[80, 70], kl=[1700, 70], F=1000, win=400),
+    "passes_window": dict(dt="fp16", H=32, D=576, ql=[70], kl=[1600], F=20, win=1300),
+    "passes_three": dict(kind="cfa", H=64, D=576, ql=[90], kl=[4000], ratio=2, F=300, win=700),
+    # slots in splits: a top-k prompt past 1280, decode steps
+    "splits_topk": dict(kind="scfa", H=32, D=512, ql=[70], kl=[1500], K=40, F=700, win=700),
+    "splits_decode": dict(H=64, D=576, ql=[1, 2], kl=[900, 700], F=100, win=300),
+    "splits_h16": dict(kind="scfa", dt="fp16", H=16, D=512, ql=[1, 1], kl=[1300, 100], K=200, F=150, win=200),
+    "sequences": dict(H=32, D=512, ql=[64 + i % 3 for i in range(70)], kl=[64 + (i * 37) % 90 + i % 3 for i in range(70)],
+                      F=5, win=20),
 }
 
 
@@ -66,6 +78,136 @@ def test_gpu_first_backward(name):
     kw = c.kwargs()
     out, lse = _run(c, **kw)
     _check_grads(c, _grads(c, out, lse, kw), out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [2, 5, 64])
+def test_gpu_first_backward_in_given_splits(splits):
+    c = Case(kind="scfa", H=32, D=576, ql=[2, 66], kl=[600, 330], K=100, F=50, win=150)
+    kw = c.kwargs()
+    out, lse = _run(c, **kw)
+    _check_grads(c, _grads(c, out, lse, dict(kw, num_splits=splits)), out, lse)
+
+
+def _segment(c, win, cus):
+    """plan_prefill's tokens a segment, without compressed rows."""
+    for seg in (96, 64, 32, 24):
+        if c.T / seg * (c.H // 32) * ((win - 1 + seg) / 64 + 1) >= 2.75 * cus:
+            break
+    return seg
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("F, dt, D", [(4, "bf16", 512), (70, "fp16", 576)])
+@pytest.mark.parametrize("seg, ql, kl", [(96, [430, 270], [2300, 1500]), (64, [201, 299], [1300, 2000]), (32, [300], [1777])])
+def test_gpu_first_backward_segments(seg, ql, kl, F, dt, D):
+    """Segments of 32 to 96 tokens, the last ones partly filled, with narrow and wide tiles of
+    first rows (the cases of tests/test_bounded.py take 24)."""
+    c = Case(dt=dt, H=160, D=D, ql=ql, kl=kl, F=F, win=1100)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert cus != 256 or _segment(c, 1100, cus) == seg
+    kw = c.kwargs()
+    out, lse = _run(c, **kw)
+    _check_grads(c, _grads(c, out, lse, kw), out, lse)
+
+
+@pytest.mark.gpu
+def test_gpu_first_of_many_sequences():
+    c = Case(kind="scfa", H=32, D=576, ql=[(i * 7) % 3 for i in range(150)], kl=[2 + (i * 41) % 300 for i in range(150)], K=40, F=9,
+             win=60, bs=16)
+    out, lse = _run(c)
+    c.check(out, lse)
+    _check_grads(c, _grads(c, out, lse, c.kwargs()), out, lse)
+
+
+# ---------------------------------------------------------------------------
+# weights
+# ---------------------------------------------------------------------------
+
+WEIGHTS = {
+    # segments of 64, 32, 16 and 8 tokens by the planner's rule on 256 CUs (`row_tiles`: its count of
+    # 128-row tiles), the last ones partly filled; tests/test_bounded.py's cases all take 4
+    "segment_64": (64, dict(H=64, D=576, ql=[150, 70, 0, 1, 129] + [(i * 5) % 4 for i in range(65)],
+                            kl=[600, 700, 5, 100, 130] + [3 + (i * 31) % 690 for i in range(65)], win=1000, F=0)),
+    "segment_32": (32, dict(H=16, D=512, ql=[130], kl=[10000], win=20000, F=0)),
+    "segment_16": (16, dict(dt="fp16", H=32, D=576, ql=[130], kl=[6000], win=7000, F=0)),
+    "segment_8": (8, dict(dt="fp8", H=16, D=576, ql=[130], kl=[3000], win=4000, F=0)),
+    # more than 64 sequences, with first and compressed rows, by rows and by slots
+    "sequences_by_rows": (4, dict(kind="cfa", H=16, D=512, ql=[(i * 5) % 13 for i in range(150)],
+                                  kl=[12 + (i * 41) % 500 for i in range(150)], ratio=4, F=150, win=20, bs=16)),
+    "sequences_by_slot": (0, dict(kind="scfa", H=16, D=576, ql=[(i * 7) % 3 for i in range(150)],
+                                  kl=[2 + (i * 41) % 300 for i in range(150)], K=40, F=9, win=60, bs=16, tail=3)),
+}
+
+
+def _weight_segment(c, win, cus):
+    """weights_impl's tokens a segment of a tile's rows, 0: slots of one token."""
+    B = len(c.ql)
+    if c.T < 4 * B:
+        return 0
+    up = lambda n, d: -(-n // d)  # noqa: E731
+    cap, mean = c.table.shape[1] * c.bs, max(1, c.T // B)
+    ncmp = min(c.ctable.shape[1] * c.bs, max(c.kl) // c.ratio) if c.kind == "cfa" else 0
+    row_tiles = B * (up(min(cap, mean + min(win - 1, cap)), 128) + up(ncmp, 128))
+    seg = 64
+    while seg > 4 and 2 * row_tiles * up(min(mean, win - 1 + 128), seg) < 3 * cus:
+        seg //= 2
+    return seg
+
+
+def _all_weights(c, lse):
+    """R.weights() with a row of adds at a time."""
+    z = lambda t: torch.zeros(len(c.ql), 1 if t is None else t.shape[1] * c.bs, dtype=torch.float64)  # noqa: E731
+    w, wc = z(c.table), z(c.ctable)
+    for t in range(c.T):
+        if c.keys.seq[t] < 0:
+            continue
+        p = torch.exp(c.q[t].double() @ R._k(c.keys, t, c.rows, c.crows).t() * c.scale - lse[t].double()[:, None]).mean(0)
+        n = len(c.keys.raw[t][0])
+        for to, at, part in ((w, c.keys.raw[t][0], p[:n]), (wc, c.keys.cmp[t][0], p[n:])):
+            to[c.keys.seq[t]].index_add_(0, torch.tensor(at, dtype=torch.long), part)
+    return w, wc
+
+
+def test_oracle_weights_by_rows_of_adds():
+    c = Case(kind="scfa", H=16, D=512, ql=[3, 0, 2], kl=[90, 4, 33], K=9, F=3, win=20, bs=8, tail=2)
+    lse = c.attention()[1]
+    for x, y in zip(_all_weights(c, lse), c.weights(lse)):
+        torch.testing.assert_close(x, y, atol=1e-13, rtol=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(WEIGHTS))
+def test_gpu_weights(name):
+    seg, case = WEIGHTS[name]
+    c = Case(**case)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert cus != 256 or _weight_segment(c, c.win, cus) == seg
+    lse = c.attention()[1].float().cuda()
+    got = _zeros(c)
+    _weights(c, lse, *got)
+    for x, ref in zip(got, _all_weights(c, lse.cpu())):
+        if x is None:
+            continue
+        x = x.cpu()
+        assert bool(((x - ref).abs() <= 2.0 ** -12 * ref + 2.0 ** -37 * c.T).all())
+        assert bool((x[ref == 0] == 0).all()) and torch.equal(torch.round(x * 2.0 ** 36), x * 2.0 ** 36)
+    again = _zeros(c)
+    _weights(c, lse, *again)
+    assert torch.equal(again[0], got[0]) and (got[1] is None or torch.equal(again[1], got[1]))
+
+
+# ---------------------------------------------------------------------------
+# GPU: long evictions
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget, zero", [(4096, 0.3), (118000, 0.3), (60000, 0.9)])
+def test_gpu_evict_of_131072_rows(budget, zero):
+    """A divided key among the heaviest, among rows without any weight, and all but one."""
+    for b in (budget, 131071):
+        a = _evict_case([131072, 33000, 100], b, 4, 64, bs=64, row=8, zero=zero)
+        _same(_evict(*a), R.evict(*a))
 
 
 # ---------------------------------------------------------------------------
