@@ -971,6 +971,11 @@ def _first_rows(ori_first) -> int:
     return ori_first
 
 
+def _held(ori_first, ori_kv, ori_block_table) -> int:
+    """As many first rows as the block table can hold: slots are planned for them all."""
+    return min(ori_first, ori_block_table.shape[1] * ori_kv.shape[1])
+
+
 def _signature(kind, q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q, seqused_kv,
                softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q):
     """The key of a call with first rows, less its sinks: geometries spelt out, as in
@@ -1022,7 +1027,7 @@ def sparse_attn_sharedkv_first(
     result are that function's. Its gradients (of rows in q's dtype):
     :func:`sparse_attn_sharedkv_first_backward`.
     """
-    ori_first = _first_rows(ori_first)
+    ori_first = _held(_first_rows(ori_first), ori_kv, ori_block_table)
     key = _signature("first", q, ori_kv, cmp_kv, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
                      seqused_kv, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q) + (
         sinks.shape, sinks.dtype, sinks.get_device(), sinks.is_contiguous())
@@ -1314,15 +1319,18 @@ def sparse_attn_sharedkv_first_backward(
     lse: torch.Tensor,
     *,
     ori_first: int,
+    ori_kv: torch.Tensor,
+    ori_block_table: torch.Tensor,
     **kwargs,
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], torch.Tensor]:
     """Gradients of :func:`sparse_attn_sharedkv_first`: as
-    :func:`sparse_attn_sharedkv_backward`, over that forward's keys; ``kwargs`` are
-    its keyword arguments, and ``window_pass`` as in
+    :func:`sparse_attn_sharedkv_backward`, over that forward's keys; the
+    keyword arguments are that forward's, and ``window_pass`` as in
     :func:`prepare_sparse_attn_sharedkv_backward`, but that True is refused where H is not
     a multiple of 32 or q or dout not 16-byte aligned (raw rows' gradients are summed
     key-major together with all others or not at all)."""
-    ori_first = _first_rows(ori_first)
+    ori_first = _held(_first_rows(ori_first), ori_kv, ori_block_table)
+    kwargs.update(ori_kv=ori_kv, ori_block_table=ori_block_table)
     if q.is_cuda and q.device.index != _device():
         with torch.cuda.device(q.device):
             return sparse_attn_sharedkv_first_backward(dout, q, out, lse, ori_first=ori_first, **kwargs)

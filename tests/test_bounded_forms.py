@@ -1,7 +1,15 @@
 """Bounded caches, further forms of the calls that tests/test_bounded.py covers: what is
 refused, lists of compressed rows each side of the planner's limits, evictions of compressed
-rows. Tolerances are that
-file's."""
+rows; slots in several passes and splits, every length of segment, more than 64 sequences.
+
+Tolerances are that file's, whose counts of fp32 adds hold here as follows. A cache row's
+gradient is summed over a segment of at most 96 tokens of 32 heads in a chain (96 matrix
+instructions of 32 products each), then over at most 13 segments of 5 head groups by
+atomic adds: a term takes part in at most 96 + 32 + 65 roundings, below 2^-16 of the terms'
+sum (0.13 h is 2^-11 in bf16, 2^-14 in fp16). Splits of dq add 64 more at most. d_sinks: 700
+adds of 2^-24 beside Delta's 512 and the exponential's 2^-20, below 2^-13 still; of 4550
+tokens a thread of the sink kernel sums 8, then 3 and 256 adds join them. A row weight's
+chain is at most 64 tokens of 4 tiles of heads."""
 
 from __future__ import annotations
 
@@ -87,6 +95,25 @@ def test_gpu_first_backward_in_given_splits(splits):
     kw = c.kwargs()
     out, lse = _run(c, **kw)
     _check_grads(c, _grads(c, out, lse, dict(kw, num_splits=splits)), out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [128, 129, 1 << 20, (1 << 31) - 1])
+def test_gpu_more_first_rows_than_the_table_holds(first):
+    """Every row is a first row; those past the block table's end are not there, and cost no
+    slots."""
+    from dsv4_amd.api import add_row_weights, sparse_attn_sharedkv_first
+    c = Case(kind="scfa", H=32, D=512, ql=[70], kl=[110], F=128, K=20, win=16)
+    kw, q = c.kwargs(), c.q.cuda()
+    out, lse = sparse_attn_sharedkv_first(q, return_softmax_lse=True, **dict(kw, ori_first=first))
+    c.check(out, lse)
+    again, _ = sparse_attn_sharedkv_first(q, return_softmax_lse=True, **dict(kw, ori_first=first))
+    assert torch.equal(again, out)
+    _check_grads(c, _grads(c, out, lse, dict(kw, ori_first=first)), out, lse)
+    w, ref = _zeros(c)[0], _zeros(c)[0]
+    add_row_weights(q, lse, ori_weights=w, **dict(kw, ori_first=first))
+    add_row_weights(q, lse, ori_weights=ref, **kw)
+    assert torch.equal(w, ref)
 
 
 def _segment(c, win, cus):
@@ -195,6 +222,41 @@ def test_gpu_weights(name):
     again = _zeros(c)
     _weights(c, lse, *again)
     assert torch.equal(again[0], got[0]) and (got[1] is None or torch.equal(again[1], got[1]))
+
+
+@pytest.mark.gpu
+def test_gpu_weights_of_two_calls_at_once():
+    """Calls on two streams that add to the same rows."""
+    c = Case(kind="scfa", H=32, D=576, ql=[5, 40], kl=[600, 300], K=64)
+    kw, q, lse = c.kwargs(), c.q.cuda(), c.attention()[1].float().cuda()
+    one, got = _zeros(c), _zeros(c)
+    _weights(c, lse, *one, kw=kw, q=q)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                _weights(c, lse, *got, kw=kw, q=q)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], 8 * one[0]) and torch.equal(got[1], 8 * one[1])
+
+
+@pytest.mark.gpu
+def test_gpu_calls_without_tokens():
+    """No query token in any sequence: empty outputs, no gradient, no weight."""
+    for kind in ("swa", "cfa", "scfa"):
+        c = Case(kind="swa" if kind == "swa" else "cfa", H=32, D=512, ql=[0, 0], kl=[90, 0])
+        kw = c.kwargs()
+        if kind == "scfa":
+            kw["cmp_sparse_indices"] = torch.zeros(0, 1, 9, dtype=torch.int32, device="cuda")
+        out, lse = _run(c, **kw)
+        assert out.shape == (0, 32, 512) and lse.shape == (0, 32)
+        dq, *rest = _grads(c, out, lse, kw)
+        assert dq.shape == (0, 32, 512) and not any(bool(x.any()) for x in rest if x is not None)
+        got = _zeros(c)
+        _weights(c, lse, *got, kw=kw)
+        assert not any(bool(x.any()) for x in got if x is not None)
 
 
 # ---------------------------------------------------------------------------
