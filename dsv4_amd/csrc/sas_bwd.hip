@@ -1109,7 +1109,9 @@ int bwd_impl(const SasBwdArgs* ba, long long first, void* stream) {
     return (kBwdFirst ? launch_bwd_prefill_first : launch_bwd_prefill)(bp, (int)a->D, a->q_dtype, (hipStream_t)stream);
   }
 #if SAS_BWD_FIRST
-  // (no window pass: first rows' adds would have to be told from window rows')
+  // no window pass, which knows no first rows: one add per token, row, 16 or 32 heads and channel.
+  // 4096 tokens of 576 channels, 16 / 48 / 80 heads 1.22 / 3.31 / 5.33 ms against 0.78 / 1.37 / 2.35
+  // without first rows and their window pass (key-major, 32 / 64 heads: 0.37 / 0.67 ms)
   return launch_tokens(bp, a, b64, ng, nblocks, (hipStream_t)stream);
 #else
   const bool win = (a->flags & SAS_BWD_WINDOW_KEYS) ||

@@ -8,8 +8,9 @@
 //     divides the candidates: passes of 2048 counts in LDS over the range of the weights or
 //     over 11 bits, until the bin in question holds at most 128 keys, which are ranked
 //     against each other, or one key alone. Then every wave lists the rows of its run that
-//     stay. 32 sequences of 2100 rows 8.5 us; four of 20000 to 32768 25 us, 6 of them one
-//     CU's load of 208 KB.
+//     stay. 32 sequences of 2100 rows 8.5 us; four of 20000 to 32768 26 us, 6 of them one
+//     CU's load of 208 KB. A call on 32768 / 33000 / 131072 rows 38 / 75 / 200 us, and where
+//     the cut falls among many rows of weight 0 72 / 134 / 418.
 //  evict_move_kernel    a workgroup owns one slice of the rows' bytes of one sequence
 //     and walks the list: since row i comes from a row at or behind i, the rows of a
 //     chunk are loaded before any of them is written, and later chunks read only rows
@@ -746,9 +747,10 @@ int evict_impl(const SasCacheEvictArgs* a, hipStream_t st) {
   p.nxcd = device_xcds();
   p.bs_log = (p.bs & (p.bs - 1)) ? -1 : __builtin_ctz(p.bs);
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)p.B), dim3(kSelThreads), 0, st, p);
-  // Slices of 64 bytes, or narrower where those leave CUs without work: 32 sequences of
-  // 2048 rows of 1152 bytes 64 / 32 / 16 bytes 21.9 / 25.8 / 28.7 us a call, 4 of 4096
-  // rows of 656 59.7 / 55.1 / 53.2 (when the selection took 10 us more).
+  // Slices of 64 bytes, or narrower where those leave CUs without work: calls with slices of 64
+  // / 32 / 16 bytes, 2048 rows of 1152 bytes of 1 / 8 / 16 / 32 sequences 17.2 / 16.5 / 15.5, 16.4
+  // / 18.0 / 18.3 (on the wrong side), 18.6 / 20.7 / 21.8 and 22.1 / 27.1 / 31.4 us, 4 of 4096 rows
+  // of 656 49.8 / 44.7 / 42.5.
   const long long quarters = (long long)p.B * ((p.row_bytes + 15) / 16);
   const int rc = quarters >= 4LL * device_cus() ? launch_move<4, 8>(p, st)
                : quarters >= 2LL * device_cus() ? launch_move<2, 8>(p, st) : launch_move<1, 4>(p, st);

@@ -281,9 +281,10 @@ __global__ void __launch_bounds__(256, 4) sas_weights_kernel(const WeightParams 
 // 128 consecutive rows of a sequence (raw ones of the windows, first ones that a window
 // has left behind, or compressed ones), 32 to a wave, and streams a segment of the tokens
 // that attend any of them, a tile of 16 heads at a time; the exponentials of one tile stand
-// between the MFMAs of the next. Two workgroups a CU: 64 tokens of 64 heads over 20000 and
-// 32768 rows of 512 channels at 1.05 PFLOP/s, the rate of a large matrix product; a wave
-// with 64 rows (half the LDS reads, but alone on its SIMD) 297 us for 228, with 48 rows 295.
+// between the MFMAs of the next. Two workgroups a CU: 64 tokens each of two sequences, 64 heads
+// over 57400 rows of 512 channels in all, 208 us, 1.16 PFLOP/s (a large matrix product: 1.20).
+// A wave with 64 rows (half the LDS reads, but alone on its SIMD) took 297 us where this took
+// 228, with 48 rows 295.
 // Tiles of at most 32 rows (a few first rows: keys of every token behind them) are held by
 // all four waves, which take four tiles of queries at once.
 
