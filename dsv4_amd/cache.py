@@ -270,8 +270,9 @@ def evict_kv_cache(
     ``ori_first`` bound them). Compressed rows may be, with their own lengths here
     (``seqused_kv // cmp_ratio``, later what the last eviction returned and the rows since):
     the attention goes on with ``seqused_kv`` as it was and ``cmp_sparse_indices`` that name
-    rows by their new places (the old row ``kept[b, i]`` is ``i``). Its dense form, without
-    lists, reads every row up to the threshold, also the bytes that an eviction leaves
+    rows by their new places (the old row ``kept[b, i]`` is ``i``). Places move forward, so
+    the threshold no longer hides a call's own new rows from its earlier tokens: their lists
+    leave those out. The attention's dense form, without lists, reads every row up to the threshold, also the bytes that an eviction leaves
     behind: after one, give lists of all rows that are left.
     """
     if cache.dim() != 4 or cache.shape[2] != 1 or not cache.is_contiguous():

@@ -367,8 +367,9 @@ int sas_row_weights_v1(const SasRowWeightsArgs* a, void* stream);
  * or destination has no block is not moved. No two sequences may share a block.
  * Raw rows of a layer with compressed rows are not to be evicted: act_kv is what a token's
  * compressed rows are found by (its position, over cmp_ratio). Compressed rows may be, with
- * their own lengths as act_kv here; SAS_SCFA's lists then name them by their new places and
- * SasFwdArgs.act_kv stays as it was. SAS_CFA would read the bytes past the rows that stay.
+ * their own lengths as act_kv here; SAS_SCFA's lists then name them by their new places (and
+ * leave out a call's new rows for its tokens before them: places move forward, past what the
+ * threshold hides) and SasFwdArgs.act_kv stays as it was. SAS_CFA would read the bytes past the rows that stay.
  */
 typedef struct SasCacheEvictArgs {
   void* cache;                   /* [num_blocks, block_size, row_bytes] bytes */
