@@ -272,8 +272,9 @@ def evict_kv_cache(
     the attention goes on with ``seqused_kv`` as it was and ``cmp_sparse_indices`` that name
     rows by their new places (the old row ``kept[b, i]`` is ``i``). Places move forward, so
     the threshold no longer hides a call's own new rows from its earlier tokens: their lists
-    leave those out. The attention's dense form, without lists, reads every row up to the threshold, also the bytes that an eviction leaves
-    behind: after one, give lists of all rows that are left.
+    leave those out. The attention's dense form, without lists, reads every row up to the
+    threshold, also the bytes that an eviction leaves behind: after one, give lists of all
+    rows that are left.
     """
     if cache.dim() != 4 or cache.shape[2] != 1 or not cache.is_contiguous():
         raise ValueError(f"cache must be contiguous [num_blocks, block_size, 1, row], got {tuple(cache.shape)}")
